@@ -10,7 +10,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DMN_HIP_LIB", os.path.join(_HERE, "lib", "libdmn_hip.so"))
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -55,10 +55,14 @@ SIGNATURES = {
     "dmn_channel_dot": [_p, _p, _p, _p, _i, _i, _i, _p],
     "dmn_dpn_stage_pass": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _ll, _p],
     "dmn_dpn_merge": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p],
+    "dmn_linear_attention_workspace_floats": [_i] * 10,
+    "dmn_linear_attention_fwd": [_i] + [_p] * 6 + [_i] + [_p] * 4 + [_i] * 8 + [_f, _p],
+    "dmn_linear_attention_bwd": [_i] + [_p] * 6 + [_i] + [_p] * 6 + [_i] + [_p] * 3 + [_i] * 8 + [_f, _p],
+    "dmn_linear_attention_step": [_i] + [_p] * 7 + [_i] * 7 + [_f, _p],
 }
 
 # entry points whose return VALUE is not a C int
-RESTYPES = {"dmn_mix_bwd_workspace_floats": _ll}
+RESTYPES = {"dmn_mix_bwd_workspace_floats": _ll, "dmn_linear_attention_workspace_floats": _ll}
 
 _lib = None
 

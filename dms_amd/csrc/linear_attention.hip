@@ -1,0 +1,526 @@
+// dms_amd/csrc/linear_attention.hip -- entry points of linear attention with a decay for each head, the small kernels
+// round the chunk kernels (linear_attention.inl), and the single-token step.
+#include "linear_attention.h"
+
+namespace dmn {
+namespace la {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// states[seg] = state after segment seg, from what each segment added: one thread for 4 elements of the state, in
+// segment order (at most a few dozen), so the same bits every time.  Bound by reading and writing the states once.
+__global__ void __launch_bounds__(256) combine_kernel(float *states, const float *decays, int nseg, int n4, long long total)
+{
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= total) return;
+    const long long row = e / n4;
+    f32x4 *p = reinterpret_cast<f32x4 *>(states) + row * nseg * n4 + e % n4;
+    const float *d = decays + row * nseg;
+    f32x4 s = p[0];
+    for (int i = 1; i < nseg - 1; ++i) {
+        s = s * d[i] + p[(long long)i * n4];
+        p[(long long)i * n4] = s;
+    }
+}
+
+// out (rows, heads, d) = sum over the group of in (rows, heads * group, d), in head order
+template <typename T>
+__global__ void __launch_bounds__(256) group_sum_kernel(const float *in, T *out, int heads, int group, int d, long long total)
+{
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= total) return;
+    const long long row = e / d;                          // (token, sample, head)
+    const float *p = in + row * group * d + e % d;
+    float s = 0.0f;
+    for (int u = 0; u < group; ++u) s += p[(long long)u * d];
+    out[e] = (T)s;
+}
+
+template <int N>
+__device__ __forceinline__ double block_sum(double v, double *sh)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int w = 0; w < N / 64; ++w) s += sh[w];
+    return s;
+}
+
+// Gradient of the log decays.  What flows over the border before token t is what came in with the first state less
+// what the tokens before t took out of the keys' side over the queries':
+//   dg_t = <S_0, dS_0> - sum_{i < t} (q_i . dq_i - k_i . dk_i)
+// One workgroup for each (sample, head) scans its dots in 64 bits; a decay of zero has no gradient.
+__global__ void __launch_bounds__(256)
+decay_grad_kernel(const float *dots_q, const float *dots_k, const float *s0, const float *ds0, const float *g, long long gt, long long gb,
+                  long long gh, const void *lengths, int lengths64, float *out, float *part, int T, int B, int H, int n)
+{
+    __shared__ double sh[4];
+    const int bh = blockIdx.x, b = bh / H, h = bh % H, tid = threadIdx.x;
+    const int len = valid_length(lengths, lengths64, b, T);
+    double run = 0.0, sum = 0.0;
+    if (s0) {
+        for (int i = tid; i < n; i += 256) run += (double)s0[(size_t)bh * n + i] * (double)ds0[(size_t)bh * n + i];
+        run = block_sum<256>(run, sh);
+    }
+    const float *pq = dots_q + (size_t)bh * T, *pk = dots_k + (size_t)bh * T, *pg = g + b * gb + h * gh;
+    for (int t0 = 0; t0 < T; t0 += 1024) {
+        double d[4], mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = t0 + tid * 4 + i;
+            d[i] = t < len ? (double)pq[t] - (double)pk[t] : 0.0;
+            mine += d[i];
+        }
+        double upto = mine;                               // inclusive over the threads of the wave
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double v = __shfl_up(upto, o);
+            if ((tid & 63) >= o) upto += v;
+        }
+        __syncthreads();
+        if ((tid & 63) == 63) sh[tid >> 6] = upto;
+        __syncthreads();
+        double before = upto - mine, tile = 0.0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w < (tid >> 6)) before += sh[w];
+            tile += sh[w];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = t0 + tid * 4 + i;
+            if (t < T) {
+                double v = run - before;
+                if (t >= len || log2_decay(pg[(long long)t * gt]) < -149.0) v = 0.0;
+                if (part) sum += v;
+                else out[((size_t)t * B + b) * H + h] = (float)v;
+            }
+            before += d[i];
+        }
+        run -= tile;
+    }
+    if (part) {
+        sum = block_sum<256>(sum, sh);
+        if (tid == 0) part[bh] = (float)sum;
+    }
+}
+
+// one decay for each head: its gradient is the samples' sum, in sample order
+__global__ void decay_grad_heads_kernel(const float *part, float *out, int B, int H)
+{
+    const int h = blockIdx.x * 64 + threadIdx.x;
+    if (h >= H) return;
+    double s = 0.0;
+    for (int b = 0; b < B; ++b) s += (double)part[(size_t)b * H + h];
+    out[h] = (float)s;
+}
+
+// One token: S = a S + k^T v in place, o = scale q S.  Bound by reading and writing the state once.  A workgroup takes
+// a head, or a slice of its columns where there are few heads (a row of S then still comes in whole 64-byte pieces);
+// V columns a thread (4 where every row is 16-byte aligned), rows over the threads, their partial o joined in LDS in
+// row order.
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+step_kernel(const T *q, const T *k, const T *v, const float *g, float *state, T *o, long long qb, long long qh, long long kb, long long kh,
+            long long vb, long long vh, long long gb, long long gh, long long sb, int H, int gq, int gk, int gv, int dk, int dv, int zb,
+            int lz, float scale)
+{
+    __shared__ float sq[128], sk[128], part[256 * V];
+    const int bh = blockIdx.x, b = bh / H, h = bh % H, tid = threadIdx.x;
+    if (tid < dk) {
+        sq[tid] = (float)q[b * qb + (h / gq) * qh + tid];
+        sk[tid] = (float)k[b * kb + (h / gk) * kh + tid];
+    }
+    const float a = fast_exp2((float)log2_decay(g[b * gb + h * gh]));
+    const int z_lanes = 1 << lz, rows = 256 >> lz, zi = tid & (z_lanes - 1), ci = tid >> lz;
+    const int z = blockIdx.y * zb + zi * V;
+    const bool ok = zi * V < zb && z < dv;
+    float vv[V], acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        vv[i] = ok ? (float)v[b * vb + (h / gv) * vh + z + i] : 0.0f;
+        acc[i] = 0.0f;
+    }
+    __syncthreads();
+    if (ok) {
+        struct alignas(4 * V) Vec { float x[V]; };
+        float *p = state + b * sb + (long long)h * dk * dv + z;
+#pragma unroll 8
+        for (int c = ci; c < dk; c += rows) {
+            Vec s = *reinterpret_cast<const Vec *>(p + (long long)c * dv);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                s.x[i] = s.x[i] * a + sk[c] * vv[i];
+                acc[i] += sq[c] * s.x[i];
+            }
+            *reinterpret_cast<Vec *>(p + (long long)c * dv) = s;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[(ci * z_lanes + zi) * V + i] = acc[i];
+    __syncthreads();
+    const int cols = min(zb, dv - (int)blockIdx.y * zb);
+    for (int c = tid; c < cols; c += 256) {
+        float s = 0.0f;
+        for (int r = 0; r < rows; ++r) s += part[r * z_lanes * V + c];
+        o[(long long)bh * dv + blockIdx.y * zb + c] = (T)(s * scale);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+struct Plan {
+    int DC, DZ, nchunks, nseg, seg_chunks;
+};
+
+static int padded(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
+
+static void pad_pair(int dc, int dz, int *DC, int *DZ)
+{
+    *DC = padded(dc);
+    *DZ = padded(dz);
+    if (*DC != *DZ) {                                      // 32 goes with 32 alone
+        if (*DC == 32) *DC = 64;
+        if (*DZ == 32) *DZ = 64;
+    }
+}
+
+// Segments: a sequence is cut where the (sample, head) pairs alone cannot fill the chip, at the cost of reading y and z
+// once more for the states between segments.
+static void plan_segments(int dtype, int T, long long passes, int *nseg, int *seg_chunks)
+{
+    const int C = chunk_tokens(dtype), nchunks = (T + C - 1) / C;
+    long long want = 1;
+    if (passes > 0 && passes < 2 * NUM_CU) want = (3 * NUM_CU + passes - 1) / passes;
+    const int most = nchunks / 2 > 1 ? nchunks / 2 : 1;    // two chunks at least: a shorter segment costs more than it hides
+    if (want > most) want = most;
+    *seg_chunks = nchunks ? (nchunks + (int)want - 1) / (int)want : 1;
+    *nseg = nchunks ? (nchunks + *seg_chunks - 1) / *seg_chunks : 1;
+}
+
+static Tensor tensor(const void *p, int dtype, int T, int B, int heads, int H, int d, const long long *s)
+{
+    Tensor t;
+    t.p = static_cast<char *>(const_cast<void *>(p));
+    t.st = T > 1 ? s[0] : 0;
+    t.sb = B > 1 ? s[1] : 0;
+    t.sh = heads > 1 ? s[2] : 0;
+    t.d = d;
+    t.group = H / heads;
+    t.f32 = 0;
+    const unsigned long long es = (unsigned long long)elem_size(dtype);
+    const unsigned long long bits = (unsigned long long)(size_t)p | (unsigned long long)t.st * es | (unsigned long long)t.sb * es |
+                                    (unsigned long long)t.sh * es | (unsigned long long)d * es;
+    t.vec = bits % 16 == 0 ? 2 : (bits % 8 == 0 ? 1 : 0);
+    return t;
+}
+
+static Tensor dense(void *p, int dtype, int T, int B, int H, int d)
+{
+    const long long s[3] = {(long long)B * H * d, (long long)H * d, d};
+    return tensor(p, dtype, T, B, H, H, d, s);
+}
+
+static long long up4(long long n) { return (n + 3) & ~3LL; }
+
+static int launch(int dtype, const Args &a, int DC, int DZ, bool state_only, hipStream_t stream)
+{
+    if (dtype == DTYPE_BF16) return launch_chunks<__bf16>(a, DC, DZ, state_only, stream);
+    if (dtype == DTYPE_F16) return launch_chunks<_Float16>(a, DC, DZ, state_only, stream);
+    return launch_chunks<float>(a, DC, DZ, state_only, stream);
+}
+
+// all passes of `a` (same DC, DZ): states between segments first where there are several
+static int run_passes(int dtype, Args &a, int DC, int DZ, float *ws, hipStream_t stream)
+{
+    if (a.nseg > 1) {
+        const long long rows = (long long)a.nroles * a.B * a.H;
+        a.states = ws;
+        a.decays = ws + rows * a.nseg * DC * DZ;
+        int rc = launch(dtype, a, DC, DZ, true, stream);
+        if (rc) return rc;
+        if (a.nseg > 2) {
+            const int n4 = DC * DZ / 4;
+            const long long total = rows * n4;
+            combine_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(a.states, a.decays, a.nseg, n4, total);
+            rc = launch_status("linear_attention combine");
+            if (rc) return rc;
+        }
+    }
+    return launch(dtype, a, DC, DZ, false, stream);
+}
+
+static long long passes_floats(int nroles, long long BH, int nseg, int DC, int DZ)
+{
+    return nseg > 1 ? up4((long long)nroles * BH * nseg * DC * DZ) + up4((long long)nroles * BH * nseg) : 0;
+}
+
+static int check(const char *who, int dtype, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)
+{
+    if (dtype < 0 || dtype > 2) return fail(-2, "%s: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16), got %d", who, dtype);
+    if (T < 0 || B < 0 || H < 1 || Hq < 1 || Hk < 1 || Hv < 1)
+        return fail(-3, "%s: bad sizes T=%d B=%d H=%d Hq=%d Hk=%d Hv=%d", who, T, B, H, Hq, Hk, Hv);
+    if (H % Hq || H % Hk || H % Hv) return fail(-4, "%s: the %d heads of the state must be a multiple of Hq=%d, Hk=%d and Hv=%d", who, H, Hq, Hk, Hv);
+    if (dk < 1 || dk > 128 || dv < 1 || dv > 128) return fail(-5, "%s: head widths must be 1 .. 128, got dk=%d dv=%d", who, dk, dv);
+    if ((long long)B * H > (1 << 22)) return fail(-6, "%s: B * H = %lld exceeds 2^22", who, (long long)B * H);
+    if (T > 0x3fffffff) return fail(-6, "%s: T = %d exceeds 2^30", who, T);
+    return 0;
+}
+
+static void fill_common(Args &a, const float *g, const long long *gs, const void *lengths, int lengths64, int T, int B, int H)
+{
+    a.g = g;
+    a.gt = gs[0];
+    a.gb = gs[1];
+    a.gh = gs[2];
+    a.lengths = lengths;
+    a.lengths64 = lengths64;
+    a.T = T;
+    a.B = B;
+    a.H = H;
+    a.states = nullptr;
+    a.decays = nullptr;
+}
+
+// the backward's passes: where each one's piece of the workspace begins
+struct BwdPlan {
+    int DCv, DZv, DCk, DZk, nseg, seg_chunks;             // of the (dq, dk) passes: contraction over dv; of the dv pass: over dk
+    long long pair, single, dots, dq, dk, dv, ds0, part, total;
+};
+
+static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)
+{
+    BwdPlan p;
+    pad_pair(dv, dk, &p.DCv, &p.DZv);
+    pad_pair(dk, dv, &p.DCk, &p.DZk);
+    const long long BH = (long long)B * H, rows = (long long)T * BH;
+    plan_segments(dtype, T, 3 * BH, &p.nseg, &p.seg_chunks);
+    long long at = 0;
+    const auto take = [&at](long long n) { const long long o = at; at += up4(n); return o; };
+    p.pair = take(passes_floats(3, BH, p.nseg, p.DCv, p.DZv));        // 3: one launch of all where dk and dv are padded alike
+    p.single = take(passes_floats(1, BH, p.nseg, p.DCk, p.DZk));
+    p.dots = take(2 * rows);
+    p.dq = take(Hq < H ? rows * dk : 0);
+    p.dk = take(Hk < H ? rows * dk : 0);
+    p.dv = take(Hv < H ? rows * dv : 0);
+    p.ds0 = take(BH * dk * dv);
+    p.part = take(BH);
+    p.total = at;
+    return p;
+}
+
+template <typename T>
+static void group_sum(const float *in, void *out, int heads, int H, int d, long long total, hipStream_t stream)
+{
+    group_sum_kernel<T><<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(in, static_cast<T *>(out), heads, H / heads, d, total);
+}
+
+static int group_sum(int dtype, const float *in, void *out, int T, int B, int heads, int H, int d, hipStream_t stream)
+{
+    const long long total = (long long)T * B * heads * d;
+    if (total == 0) return 0;
+    if ((total + 255) / 256 > 0x7fffffffLL) return fail(-6, "linear_attention: %lld gradients exceed one grid", total);
+    if (dtype == DTYPE_BF16) group_sum<__bf16>(in, out, heads, H, d, total, stream);
+    else if (dtype == DTYPE_F16) group_sum<_Float16>(in, out, heads, H, d, total, stream);
+    else group_sum<float>(in, out, heads, H, d, total, stream);
+    return launch_status("linear_attention group sum");
+}
+
+template <typename T>
+static int launch_step(const void *q, const void *k, const void *v, const float *g, float *state, void *o, const long long *s, int B, int H,
+                       int Hq, int Hk, int Hv, int dk, int dv, float scale, hipStream_t stream)
+{
+    const bool wide = dv % 4 == 0 && (size_t)state % 16 == 0 && s[8] % 4 == 0;
+    int zb = dv, nz = 1;                                   // few heads: slices of 16 columns and more
+    while ((long long)B * H * nz < 2 * NUM_CU && zb > 16) {
+        zb = ((zb + 1) / 2 + 15) & ~15;
+        nz = (dv + zb - 1) / zb;
+    }
+    const int lanes = wide ? (zb + 3) / 4 : zb;
+    int lz = 0;
+    while ((1 << lz) < lanes) ++lz;
+    const dim3 grid((unsigned)(B * H), (unsigned)nz);
+    if (wide)
+        step_kernel<T, 4><<<grid, 256, 0, stream>>>((const T *)q, (const T *)k, (const T *)v, g, state, (T *)o, s[0], s[1], s[2], s[3], s[4], s[5],
+                                                    s[6], s[7], s[8], H, H / Hq, H / Hk, H / Hv, dk, dv, zb, lz, scale);
+    else
+        step_kernel<T, 1><<<grid, 256, 0, stream>>>((const T *)q, (const T *)k, (const T *)v, g, state, (T *)o, s[0], s[1], s[2], s[3], s[4], s[5],
+                                                    s[6], s[7], s[8], H, H / Hq, H / Hk, H / Hv, dk, dv, zb, lz, scale);
+    return launch_status("linear_attention_step");
+}
+
+}  // namespace la
+}  // namespace dmn
+
+using namespace dmn;
+using namespace dmn::la;
+
+extern "C" long long dmn_linear_attention_workspace_floats(int dtype, int backward, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)
+{
+    if (check("dmn_linear_attention_workspace_floats", dtype, T, B, H, Hq, Hk, Hv, dk, dv)) return -1;
+    if (backward) return plan_bwd(dtype, T, B, H, Hq, Hk, Hv, dk, dv).total;
+    int DC, DZ, nseg, seg_chunks;
+    pad_pair(dk, dv, &DC, &DZ);
+    plan_segments(dtype, T, (long long)B * H, &nseg, &seg_chunks);
+    return passes_floats(1, (long long)B * H, nseg, DC, DZ);
+}
+
+extern "C" int dmn_linear_attention_fwd(int dtype, const void *q, const void *k, const void *v, const float *g, const float *state0,
+                                        const void *lengths, int lengths64, void *o, float *state, const long long *strides, float *workspace,
+                                        int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv, float scale, void *stream)
+{
+    const char *who = "dmn_linear_attention_fwd";
+    int rc = check(who, dtype, T, B, H, Hq, Hk, Hv, dk, dv);
+    if (rc) return rc;
+    if (!strides || (B > 0 && T > 0 && (!q || !k || !v || !g || !o))) return fail(-1, "%s: null pointer", who);
+    if (B == 0) return 0;
+    Args a;
+    fill_common(a, g, strides + 9, lengths, lengths64, T, B, H);
+    a.nroles = 1;
+    int DC, DZ;
+    pad_pair(dk, dv, &DC, &DZ);
+    plan_segments(dtype, T, (long long)B * H, &a.nseg, &a.seg_chunks);
+    if (a.nseg > 1 && (!workspace || (size_t)workspace % 16)) return fail(-7, "%s: this size needs a 16-byte aligned workspace", who);
+    Role &r = a.role[0];
+    r.X = tensor(q, dtype, T, B, Hq, H, dk, strides);
+    r.Y = tensor(k, dtype, T, B, Hk, H, dk, strides + 3);
+    r.Z = tensor(v, dtype, T, B, Hv, H, dv, strides + 6);
+    r.O = dense(o, dtype, T, B, H, dv);
+    r.W = r.X;
+    r.s_in = state0;
+    r.s_out = state;
+    r.in_c = r.out_c = dv;
+    r.in_z = r.out_z = 1;
+    r.dots = nullptr;
+    r.scale_p = r.scale_x = scale;
+    r.scale_z = 1.0f;
+    r.reverse = r.last_decay = 0;
+    a.role[1] = a.role[2] = r;
+    return run_passes(dtype, a, DC, DZ, workspace, (hipStream_t)stream);
+}
+
+extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k, const void *v, const float *g, const float *state0,
+                                        const void *lengths, int lengths64, const void *grad_o, const float *grad_state, void *grad_q, void *grad_k,
+                                        void *grad_v, float *grad_g, int grad_g_per_head, float *grad_state0, const long long *strides,
+                                        float *workspace, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv, float scale, void *stream)
+{
+    const char *who = "dmn_linear_attention_bwd";
+    int rc = check(who, dtype, T, B, H, Hq, Hk, Hv, dk, dv);
+    if (rc) return rc;
+    if (!strides || (B > 0 && T > 0 && (!q || !k || !v || !g || !grad_o))) return fail(-1, "%s: null pointer", who);
+    hipStream_t st = (hipStream_t)stream;
+    if (B == 0) {
+        if (grad_g && grad_g_per_head) {
+            decay_grad_heads_kernel<<<(H + 63) / 64, 64, 0, st>>>(nullptr, grad_g, 0, H);
+            return launch_status(who);
+        }
+        return 0;
+    }
+    if (!workspace || (size_t)workspace % 16) return fail(-7, "%s: needs a 16-byte aligned workspace", who);
+    const BwdPlan p = plan_bwd(dtype, T, B, H, Hq, Hk, Hv, dk, dv);
+    float *dots = workspace + p.dots, *ds0 = grad_state0;
+    const bool need_ds0 = grad_state0 || (grad_g && state0);
+    if (!ds0) ds0 = workspace + p.ds0;
+
+    const Tensor Q = tensor(q, dtype, T, B, Hq, H, dk, strides), K = tensor(k, dtype, T, B, Hk, H, dk, strides + 3),
+                 V = tensor(v, dtype, T, B, Hv, H, dv, strides + 6), D = tensor(grad_o, dtype, T, B, H, H, dv, strides + 12);
+    const auto output = [&](void *out, float *ws, int heads, int d) {
+        if (!out || heads == H) return dense(out, dtype, T, B, H, d);
+        Tensor t = dense(ws, DTYPE_F32, T, B, H, d);
+        t.f32 = 1;
+        return t;
+    };
+    Args a;
+    fill_common(a, g, strides + 9, lengths, lengths64, T, B, H);
+    a.nseg = p.nseg;
+    a.seg_chunks = p.seg_chunks;
+    a.nroles = 0;
+    if (grad_q || grad_g) {                               // dq: the operator on (dO, v, k)
+        Role &r = a.role[a.nroles++];
+        r.X = D; r.Y = V; r.Z = K; r.W = Q;
+        r.O = output(grad_q, workspace + p.dq, Hq, dk);
+        r.s_in = state0;
+        r.s_out = nullptr;
+        r.in_c = r.out_c = 1;
+        r.in_z = r.out_z = dv;
+        r.dots = grad_g ? dots : nullptr;
+        r.scale_p = r.scale_x = scale;
+        r.scale_z = 1.0f;
+        r.reverse = r.last_decay = 0;
+    }
+    if (grad_k || grad_g) {                               // dk: backwards in time, on (v, dO, q)
+        Role &r = a.role[a.nroles++];
+        r.X = V; r.Y = D; r.Z = Q; r.W = K;
+        r.O = output(grad_k, workspace + p.dk, Hk, dk);
+        r.s_in = grad_state;
+        r.s_out = nullptr;
+        r.in_c = r.out_c = 1;
+        r.in_z = r.out_z = dv;
+        r.dots = grad_g ? dots + (size_t)T * B * H : nullptr;
+        r.scale_p = r.scale_z = scale;
+        r.scale_x = 1.0f;
+        r.reverse = 1;
+        r.last_decay = 0;
+    }
+    const bool third = grad_v || need_ds0;
+    Role rv;
+    if (third) {                                          // dv and dS_0: backwards in time, on (k, q, dO)
+        rv.X = K; rv.Y = Q; rv.Z = D; rv.W = V;
+        rv.O = output(grad_v, workspace + p.dv, Hv, dv);
+        rv.s_in = grad_state;
+        rv.s_out = need_ds0 ? ds0 : nullptr;
+        rv.in_c = rv.out_c = dv;
+        rv.in_z = rv.out_z = 1;
+        rv.dots = nullptr;
+        rv.scale_p = rv.scale_z = scale;
+        rv.scale_x = 1.0f;
+        rv.reverse = rv.last_decay = 1;
+    }
+    if (third && p.DCv == p.DCk && p.DZv == p.DZk) {
+        a.role[a.nroles++] = rv;
+    } else if (third) {
+        Args one = a;
+        one.nroles = 1;
+        one.role[0] = rv;
+        rc = run_passes(dtype, one, p.DCk, p.DZk, workspace + p.single, st);
+        if (rc) return rc;
+    }
+    if (a.nroles > 0) {
+        rc = run_passes(dtype, a, p.DCv, p.DZv, workspace + p.pair, st);
+        if (rc) return rc;
+    }
+    if (grad_g) {
+        float *part = grad_g_per_head ? workspace + p.part : nullptr;
+        decay_grad_kernel<<<(unsigned)(B * H), 256, 0, st>>>(dots, dots + (size_t)T * B * H, state0, ds0, g, a.gt, a.gb, a.gh, lengths, lengths64,
+                                                             grad_g, part, T, B, H, dk * dv);
+        rc = launch_status("linear_attention decay gradient");
+        if (rc) return rc;
+        if (part) {
+            decay_grad_heads_kernel<<<(H + 63) / 64, 64, 0, st>>>(part, grad_g, B, H);
+            rc = launch_status("linear_attention decay gradient");
+            if (rc) return rc;
+        }
+    }
+    if (grad_q && Hq < H && (rc = group_sum(dtype, workspace + p.dq, grad_q, T, B, Hq, H, dk, st))) return rc;
+    if (grad_k && Hk < H && (rc = group_sum(dtype, workspace + p.dk, grad_k, T, B, Hk, H, dk, st))) return rc;
+    if (grad_v && Hv < H && (rc = group_sum(dtype, workspace + p.dv, grad_v, T, B, Hv, H, dv, st))) return rc;
+    return 0;
+}
+
+extern "C" int dmn_linear_attention_step(int dtype, const void *q, const void *k, const void *v, const float *g, float *state, void *o,
+                                         const long long *strides, int B, int H, int Hq, int Hk, int Hv, int dk, int dv, float scale,
+                                         void *stream)
+{
+    const char *who = "dmn_linear_attention_step";
+    const int rc = check(who, dtype, 1, B, H, Hq, Hk, Hv, dk, dv);
+    if (rc) return rc;
+    if (!strides || (B > 0 && (!q || !k || !v || !g || !state || !o))) return fail(-1, "%s: null pointer", who);
+    if (B == 0) return 0;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == DTYPE_BF16) return launch_step<__bf16>(q, k, v, g, state, o, strides, B, H, Hq, Hk, Hv, dk, dv, scale, st);
+    if (dtype == DTYPE_F16) return launch_step<_Float16>(q, k, v, g, state, o, strides, B, H, Hq, Hk, Hv, dk, dv, scale, st);
+    return launch_step<float>(q, k, v, g, state, o, strides, B, H, Hq, Hk, Hv, dk, dv, scale, st);
+}

@@ -2,10 +2,11 @@
 """Torch-facing wrappers of the HIP entry points (include/dmn_hip.h).
 
 PyTorch is plumbing here: it owns device memory, streams and autograd bookkeeping; every
-operator below runs in libdmn_hip.so.  Tensors must be fp32 and on a ROCm device --
-anything else raises (there is no CPU or eager fallback).
+operator below runs in libdmn_hip.so.  Tensors must be fp32 (the linear-attention operators:
+fp32, bf16 or fp16) and on a ROCm device -- anything else raises (there is no CPU or eager fallback).
 """
 import contextlib
+import ctypes
 import os
 import tempfile
 
@@ -780,3 +781,180 @@ def dpn_merge(base, y, c1c, bn=None):
         _lib.call("dmn_dpn_merge", _ptr(base), _ptr(y), _ptr(out), _ptr(act), _ptr(mean),
                   _ptr(scale), _ptr(bias), N, Cb, Cy, int(c1c), H * W, _stream())
     return out, act
+
+
+# ------------------------------------------------------------------------------------
+# linear attention with a decay for each head
+# ------------------------------------------------------------------------------------
+_DTYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LINEAR_ATTENTION_MAX_WIDTH = 128
+
+
+def _chk_rows(name, what, t, shape, dtype, device):
+    """A tensor with unit stride along its last axis and any other strides."""
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise RuntimeError("dms_amd.%s: %s must be a tensor on a ROCm device (no CPU fallback exists)" % (name, what))
+    if t.dtype != dtype:
+        raise RuntimeError("dms_amd.%s: expected %s for %s, got %s" % (name, dtype, what, t.dtype))
+    if t.device != device:
+        raise RuntimeError("dms_amd.%s: %s is on %s, the other tensors on %s" % (name, what, t.device, device))
+    if t.shape != shape:
+        raise RuntimeError("dms_amd.%s: expected shape %s for %s, got %s" % (name, tuple(shape), what, tuple(t.shape)))
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise RuntimeError("dms_amd.%s: %s must have unit stride along its last axis" % (name, what))
+
+
+def _chk_heads(name, q, k, v, H):
+    """Type and widths of q, k, v (..., heads, width) beside a state of H heads."""
+    if not torch.is_tensor(q) or q.dtype not in _DTYPE_IDS:
+        raise RuntimeError("dms_amd.%s: q, k and v must be float32, bfloat16 or float16 tensors" % name)
+    lead = q.shape[:-2]
+    _chk_rows(name, "q", q, q.shape, q.dtype, q.device)
+    for what, t, width in (("k", k, q.shape[-1]), ("v", v, None)):
+        if not torch.is_tensor(t) or t.dim() != q.dim():
+            raise RuntimeError("dms_amd.%s: %s must have %d axes like q" % (name, what, q.dim()))
+        _chk_rows(name, what, t, lead + (t.shape[-2], t.shape[-1] if width is None else width), q.dtype, q.device)
+    for what, t in (("q", q), ("k", k), ("v", v)):
+        if t.shape[-2] < 1 or H % t.shape[-2]:
+            raise RuntimeError("dms_amd.%s: the %d heads of the state must be a multiple of the %d heads of %s"
+                               % (name, H, t.shape[-2], what))
+        if not 1 <= t.shape[-1] <= LINEAR_ATTENTION_MAX_WIDTH:
+            raise RuntimeError("dms_amd.%s: head widths of 1 .. %d are supported, %s has %d"
+                               % (name, LINEAR_ATTENTION_MAX_WIDTH, what, t.shape[-1]))
+
+
+def _strides(*groups):
+    flat = [s for g in groups for s in g]
+    return (ctypes.c_longlong * len(flat))(*flat)
+
+
+def _linear_attention_sizes(q, k, v, H):
+    T, B, Hq, dk = q.shape
+    return T, B, H, Hq, k.shape[2], v.shape[2], dk, v.shape[3]
+
+
+def _decay_strides(g):
+    return (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
+
+
+def _linear_attention_raw(q, k, v, g, state0, lengths, scale):
+    T, B, H, Hq, Hk, Hv, dk, dv = sizes = _linear_attention_sizes(q, k, v, g.shape[-1])
+    dt = _DTYPE_IDS[q.dtype]
+    with torch.cuda.device(q.device):
+        o = torch.empty((T, B, H, dv), device=q.device, dtype=q.dtype)
+        state = torch.empty((B, H, dk, dv), device=q.device, dtype=torch.float32)
+        n = _lib.query("dmn_linear_attention_workspace_floats", dt, 0, *sizes)
+        ws = torch.empty(n, device=q.device, dtype=torch.float32) if n > 0 else None
+        _lib.call("dmn_linear_attention_fwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state0), _ptr(lengths),
+                  int(lengths is not None and lengths.dtype == torch.int64), _ptr(o), _ptr(state),
+                  _strides(q.stride()[:3], k.stride()[:3], v.stride()[:3], _decay_strides(g)), _ptr(ws), *sizes, scale, _stream())
+    return o, state
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, state0, lengths, scale):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, g, state0, lengths)
+        ctx.scale = scale
+        return _linear_attention_raw(q, k, v, g, state0, lengths, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_o, grad_state):
+        q, k, v, g, state0, lengths = ctx.saved_tensors
+        if grad_o is None and grad_state is None:
+            return (None,) * 7
+        T, B, H, Hq, Hk, Hv, dk, dv = sizes = _linear_attention_sizes(q, k, v, g.shape[-1])
+        dt, dev = _DTYPE_IDS[q.dtype], q.device
+        need = ctx.needs_input_grad
+        with torch.cuda.device(dev):
+            if grad_o is None:
+                grad_o = torch.zeros(dv, device=dev, dtype=q.dtype).expand(T, B, H, dv)
+            elif dv > 1 and grad_o.stride(3) != 1:
+                grad_o = grad_o.contiguous()
+            if grad_state is not None:
+                grad_state = grad_state.contiguous()
+            gq = torch.empty((T, B, Hq, dk), device=dev, dtype=q.dtype) if need[0] else None
+            gk = torch.empty((T, B, Hk, dk), device=dev, dtype=q.dtype) if need[1] else None
+            gv = torch.empty((T, B, Hv, dv), device=dev, dtype=q.dtype) if need[2] else None
+            gg = torch.empty(g.shape, device=dev, dtype=torch.float32) if need[3] else None
+            gs = torch.empty((B, H, dk, dv), device=dev, dtype=torch.float32) if state0 is not None and need[4] else None
+            ws = torch.empty(max(_lib.query("dmn_linear_attention_workspace_floats", dt, 1, *sizes), 4), device=dev,
+                             dtype=torch.float32)
+            _lib.call("dmn_linear_attention_bwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state0), _ptr(lengths),
+                      int(lengths is not None and lengths.dtype == torch.int64), _ptr(grad_o), _ptr(grad_state), _ptr(gq),
+                      _ptr(gk), _ptr(gv), _ptr(gg), int(g.dim() == 1), _ptr(gs),
+                      _strides(q.stride()[:3], k.stride()[:3], v.stride()[:3], _decay_strides(g), grad_o.stride()[:3]),
+                      _ptr(ws), *sizes, ctx.scale, _stream())
+        return gq, gk, gv, gg, gs, None, None
+
+
+def linear_attention(q, k, v, g, state0=None, lengths=None, scale=None):
+    """Linear attention with a decay for each head: S_t = exp(g_t) S_{t-1} + k_t^T v_t, o_t = scale * q_t S_t.
+
+    q (T, B, Hq, dk), k (T, B, Hk, dk), v (T, B, Hv, dv) in float32, bfloat16 or float16, with unit stride along the last
+    axis and any other strides; g (T, B, H) or (H,) float32 log decays (<= 0; -inf empties the state before that token, so
+    sequences can be packed one behind the other).  H, the heads of the state, is a multiple of Hq, Hk and Hv: head h
+    reads head h // (H // Hq) of q, and so on.  Head widths up to 128.  state0 (B, H, dk, dv) float32 or None (zeros);
+    lengths (B,) int32 or int64 on the device, or None: tokens of each sample, rows behind them are neither read nor do
+    they change the state, and their outputs and gradients are zero.  scale: dk ** -0.5 if None.
+    Returns o (T, B, H, dv) and the state (B, H, dk, dv) after the last token, both under autograd (once)."""
+    name = "linear_attention"
+    if not torch.is_tensor(g) or g.dim() not in (1, 3):
+        raise RuntimeError("dms_amd.%s: g must be (T, B, H) or (H,)" % name)
+    if not torch.is_tensor(q) or q.dim() != 4:
+        raise RuntimeError("dms_amd.%s: q must be (T, B, heads, width)" % name)
+    T, B, H = q.shape[0], q.shape[1], g.shape[-1]
+    _chk_heads(name, q, k, v, H)
+    if not g.is_cuda or g.dtype != torch.float32 or g.device != q.device or (g.dim() == 3 and g.shape != (T, B, H)):
+        raise RuntimeError("dms_amd.%s: g must be float32 (T, B, H) or (H,) on %s, got %s %s on %s"
+                           % (name, q.device, g.dtype, tuple(g.shape), g.device))
+    if state0 is not None:
+        _chk(name, state0, (B, H, q.shape[3], v.shape[3]))
+        if state0.device != q.device:
+            raise RuntimeError("dms_amd.%s: state0 is on %s, q on %s" % (name, state0.device, q.device))
+    if lengths is not None:
+        if (not lengths.is_cuda or lengths.device != q.device or lengths.dtype not in (torch.int32, torch.int64)
+                or lengths.shape != (B,) or not lengths.is_contiguous()):
+            raise RuntimeError("dms_amd.%s: lengths must be a contiguous int32 or int64 tensor of shape (%d,) on %s"
+                               % (name, B, q.device))
+    scale = float(q.shape[3]) ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                    or (state0 is not None and state0.requires_grad)):
+        return _LinearAttention.apply(q, k, v, g, state0, lengths, scale)
+    return _linear_attention_raw(q, k, v, g, state0, lengths, scale)
+
+
+def linear_attention_step(q, k, v, g, state, scale=None):
+    """One token of linear_attention (inference): q (B, Hq, dk), k (B, Hk, dk), v (B, Hv, dv), g (B, H) or (H,) float32,
+    state (B, H, dk, dv) float32, UPDATED IN PLACE (its samples may be strided, each one contiguous).  Returns o (B, H, dv)."""
+    name = "linear_attention_step"
+    if not torch.is_tensor(g) or g.dim() not in (1, 2):
+        raise RuntimeError("dms_amd.%s: g must be (B, H) or (H,)" % name)
+    if not torch.is_tensor(q) or q.dim() != 3:
+        raise RuntimeError("dms_amd.%s: q must be (B, heads, width)" % name)
+    B, H = q.shape[0], g.shape[-1]
+    _chk_heads(name, q, k, v, H)
+    dk, dv = q.shape[2], v.shape[2]
+    if not g.is_cuda or g.dtype != torch.float32 or g.device != q.device or (g.dim() == 2 and g.shape != (B, H)):
+        raise RuntimeError("dms_amd.%s: g must be float32 (B, H) or (H,) on %s, got %s %s on %s"
+                           % (name, q.device, g.dtype, tuple(g.shape), g.device))
+    if not torch.is_tensor(state) or not state.is_cuda or state.dtype != torch.float32 or state.device != q.device:
+        raise RuntimeError("dms_amd.%s: state must be a float32 tensor on %s" % (name, q.device))
+    if state.shape != (B, H, dk, dv):
+        raise RuntimeError("dms_amd.%s: expected shape %s for state, got %s" % (name, (B, H, dk, dv), tuple(state.shape)))
+    if B and (not state[0].is_contiguous() or (B > 1 and state.stride(0) < H * dk * dv)):
+        raise RuntimeError("dms_amd.%s: every sample of the state must be contiguous" % name)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, state)):
+        raise RuntimeError("dms_amd.%s: inference only (the state is updated in place): call it under no_grad, or use "
+                           "linear_attention" % name)
+    scale = float(dk) ** -0.5 if scale is None else float(scale)
+    with torch.cuda.device(q.device):
+        o = torch.empty((B, H, dv), device=q.device, dtype=q.dtype)
+        _lib.call("dmn_linear_attention_step", _DTYPE_IDS[q.dtype], _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state), _ptr(o),
+                  _strides(q.stride()[:2], k.stride()[:2], v.stride()[:2], (0, g.stride(0)) if g.dim() == 1 else g.stride(),
+                           state.stride()[:1]), B, H, q.shape[1], k.shape[1], v.shape[1], dk, dv, scale, _stream())
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)      # a graph that saved the state must notice
+    return o

@@ -6,7 +6,8 @@
  * plain device pointers + sizes, and replaces the reference interface cited above it.
  *
  * Conventions (all entry points)
- *   - All tensors are fp32, contiguous, row-major, resident in device memory and OWNED
+ *   - All tensors are fp32, contiguous, row-major (entry points with a `dtype` or `strides` argument say
+ *     what else they take), resident in device memory and OWNED
  *     BY THE CALLER; the library never allocates, frees or retains them.
  *   - `stream` is a hipStream_t (NULL = default stream).  Calls are asynchronous on it;
  *     nothing inside synchronises the device.  The caller's current device is used.
@@ -23,7 +24,7 @@
 extern "C" {
 #endif
 
-#define DMN_ABI_VERSION 3
+#define DMN_ABI_VERSION 4
 
 /* activation ids of the SRU cell (upstream `use_tanh` / `use_relu` switches) */
 #define DMN_ACT_IDENTITY 0
@@ -396,6 +397,54 @@ int dmn_dpn_merge(const float *base, const float *yv, float *out, float *act,
 int dmn_dpn_stage_pass(float *buf, float *act, float *out,
                        const float *mean, const float *scale, const float *bias,
                        int N, int rows, int c1c, int inc, int Co, int HW, long long out_bs, void *stream);
+
+/*
+ * Linear attention with a decay for each head: the recurrence with a matrix state that stands beside the SRU's diagonal
+ * one (no counterpart in the reference).  For every sample b and head h, from the state S_{-1} = state0 (or zero),
+ *     S_t = exp(g[t,b,h]) S_{t-1} + k[t,b,h]^T v[t,b,h]            (dk x dv)
+ *     o[t,b,h] = scale * q[t,b,h] S_t
+ *   dtype    0: fp32, 1: bf16, 2: fp16 -- of q, k, v, o and their gradients.  g, the states and grad_g are fp32.
+ *   q (T,B,Hq,dk), k (T,B,Hk,dk), v (T,B,Hv,dv): unit stride along the last axis, any other strides (a slice of a fused
+ *            projection, an expanded tensor).  Head h of the H heads of the state reads head h / (H/Hq) of q, and so on: H
+ *            is a multiple of Hq, Hk and Hv.  1 <= dk, dv <= 128.
+ *   g        log decay, <= 0 in any sensible use; -inf empties the state before the token (sequences packed one behind the
+ *            other).  strides of 0 over t and b: one decay for each head.
+ *   state0, state (B,H,dk,dv) contiguous or NULL; they may not overlap.
+ *   lengths  (B) int32 (lengths64 = 0) or int64 (1), or NULL: sample b has min(max(lengths[b], 0), T) tokens.  Rows behind them
+ *            are not read; their o (and gradients) are zero, and `state` is the state after the last token.
+ *   o        (T,B,H,dv) contiguous.
+ *   strides  HOST array of 12, in elements: t, b, h of q, of k, of v, of g.
+ *   workspace  dmn_linear_attention_workspace_floats(dtype, 0, ...) floats, 16-byte aligned (NULL when that is 0).  Calls that
+ *            overlap need one each.
+ * Sums and states are fp32; products run on bf16 planes that together carry at least 16 bits beside bf16 and fp16 inputs and 24
+ * beside fp32 ones, so an infinity in a token that counts makes NaN.  A token that is not finite spoils its chunk's outputs.
+ */
+long long dmn_linear_attention_workspace_floats(int dtype, int backward, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv);
+int dmn_linear_attention_fwd(int dtype, const void *q, const void *k, const void *v, const float *g, const float *state0,
+                             const void *lengths, int lengths64, void *o, float *state, const long long *strides, float *workspace,
+                             int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv, float scale, void *stream);
+/*
+ * Its gradients.  grad_o (T,B,H,dv) with unit stride along the last axis; grad_state (B,H,dk,dv) contiguous or NULL = 0.
+ *   strides  HOST array of 15: the 12 above, then t, b, h of grad_o.
+ *   grad_q (T,B,Hq,dk), grad_k (T,B,Hk,dk), grad_v (T,B,Hv,dv), grad_state0 (B,H,dk,dv): contiguous, or NULL if not wanted;
+ *            of shared heads: the sum over the heads that read them, in head order.
+ *   grad_g   (T,B,H) contiguous, or (H) with grad_g_per_head = 1 (summed over t and b, in that order), or NULL.  Zero where exp(g)
+ *            is zero in 32 bits.
+ *   workspace  dmn_linear_attention_workspace_floats(dtype, 1, ...) floats, 16-byte aligned.
+ * No atomics: the same inputs give the same bits.
+ */
+int dmn_linear_attention_bwd(int dtype, const void *q, const void *k, const void *v, const float *g, const float *state0,
+                             const void *lengths, int lengths64, const void *grad_o, const float *grad_state, void *grad_q, void *grad_k,
+                             void *grad_v, float *grad_g, int grad_g_per_head, float *grad_state0, const long long *strides,
+                             float *workspace, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv, float scale, void *stream);
+/*
+ * One token of it, for serving: state (B,H,dk,dv) is updated IN PLACE and o (B,H,dv), contiguous, is returned.
+ *   strides  HOST array of 9, in elements: b, h of q (B,Hq,dk), of k (B,Hk,dk), of v (B,Hv,dv), of g (B,H); b of the state
+ *            (its heads are contiguous).
+ */
+int dmn_linear_attention_step(int dtype, const void *q, const void *k, const void *v, const float *g, float *state, void *o,
+                              const long long *strides, int B, int H, int Hq, int Hk, int Hv, int dk, int dv, float scale,
+                              void *stream);
 
 #ifdef __cplusplus
 }
