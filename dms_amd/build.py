@@ -17,17 +17,18 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libdmn_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 SOURCES = ["abi.hip", "sru.hip", "sru_bwd.hip", "sru_fwd_k2.hip", "sru_fwd_k3.hip", "sru_fwd_k4.hip", "dynfilter.hip", "mix.hip", "mix_sru.hip", "glue.hip", "wino.hip", "tapconv.hip", "metrics.hip", "dpn_glue.hip", "gconv.hip",
-           "linear_attention.hip", "linear_attention_f32.hip", "linear_attention_bf16.hip", "linear_attention_f16.hip"]
+           "linear_attention.hip", "linear_attention_f32.hip", "linear_attention_bf16.hip", "linear_attention_f16.hip",
+           "head_norm_rotary.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
 # sru_bwd.hip: its register ring is loaded by inline asm that hipcc does not count.  With SLP
 # vectorisation on, hipcc packs the step's scalar maths into v_pk_* pairs and MOVES ring registers
 # into pair positions before their counted wait (copies of registers whose loads are still in
 # flight; tools/check_asm_waits.py shows them).  Scalar code keeps every slot in its own register.
 EXTRA_FLAGS = {"sru_bwd.hip": ["-fno-slp-vectorize"]}
-# the linear-attention sources are compiled without packed fp32 instructions (hipcc forms them from ordinary
+# the linear-attention and head-norm sources are compiled without packed fp32 instructions (hipcc forms them from ordinary
 # float code; some of their forms have given wrong results on gfx950)
 for _s in SOURCES:
-    if _s.startswith("linear_attention"):
+    if _s.startswith(("linear_attention", "head_norm")):
         EXTRA_FLAGS[_s] = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

@@ -958,3 +958,113 @@ def linear_attention_step(q, k, v, g, state, scale=None):
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)      # a graph that saved the state must notice
     return o
+
+
+# ------------------------------------------------------------------------------------
+# RMS norm and multi-axis rotation of query and key heads
+# ------------------------------------------------------------------------------------
+HEAD_NORM_ROTARY_MAX_WIDTH = 256
+
+
+def _head_norm_rotary_args(q, k, wq, wk, positions, sections, base, eps):
+    T, B = q.shape[:2]
+    pos = (0, 0, 0) if positions is None else ((positions.stride(0), 0, positions.stride(1)) if positions.dim() == 2
+                                               else positions.stride())
+    weight = wq if wq is not None else wk
+    return (_ptr(q), _ptr(k), _ptr(wq), _ptr(wk), int(weight is not None and weight.dtype == torch.float32), _ptr(positions),
+            int(positions is not None and positions.dtype == torch.int64), (ctypes.c_int * max(len(sections), 1))(*sections),
+            len(sections), base, eps), pos, (T, B, q.shape[2], k.shape[2], q.shape[3])
+
+
+def _head_norm_rotary_raw(q, k, wq, wk, positions, sections, base, eps):
+    args, pos, sizes = _head_norm_rotary_args(q, k, wq, wk, positions, sections, base, eps)
+    with torch.cuda.device(q.device):
+        yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        yk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        _lib.call("dmn_head_norm_rotary_fwd", _DTYPE_IDS[q.dtype], *args, _ptr(yq), _ptr(yk),
+                  _strides(q.stride()[:3], k.stride()[:3], pos), *sizes, _stream())
+    return yq, yk
+
+
+class _HeadNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, positions, sections, base, eps):
+        ctx.save_for_backward(q, k, wq, wk, positions)
+        ctx.consts = sections, base, eps
+        return _head_norm_rotary_raw(q, k, wq, wk, positions, sections, base, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gyq, gyk):
+        q, k, wq, wk, positions = ctx.saved_tensors
+        need, dev = ctx.needs_input_grad, q.device
+        args, pos, sizes = _head_norm_rotary_args(q, k, wq, wk, positions, *ctx.consts)
+        gyq, gyk = (x if x.shape[3] == 1 or x.stride(3) == 1 else x.contiguous() for x in (gyq, gyk))
+        with torch.cuda.device(dev):
+            gq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+            gk = torch.empty(k.shape, device=dev, dtype=q.dtype)
+            gwq = torch.empty(wq.shape, device=dev, dtype=wq.dtype) if wq is not None and need[2] else None
+            gwk = torch.empty(wk.shape, device=dev, dtype=wk.dtype) if wk is not None and need[3] else None
+            ws = None
+            if gwq is not None or gwk is not None:
+                ws = torch.empty(_lib.query("dmn_head_norm_rotary_workspace_floats", *sizes[2:]), device=dev, dtype=torch.float32)
+            _lib.call("dmn_head_norm_rotary_bwd", _DTYPE_IDS[q.dtype], *args, _ptr(gyq), _ptr(gyk), _ptr(gq), _ptr(gk), _ptr(gwq),
+                      _ptr(gwk), _strides(q.stride()[:3], k.stride()[:3], pos, gyq.stride()[:3], gyk.stride()[:3]), _ptr(ws),
+                      *sizes, _stream())
+        return gq if need[0] else None, gk if need[1] else None, gwq, gwk, None, None, None, None
+
+
+def head_norm_rotary(q, k, q_weight, k_weight, positions, sections, base=10000.0, eps=1e-6):
+    """RMS norm of every query and key head, then its rotation by positions on several axes, in one pass; under autograd (once).
+
+    q (T, B, Hq, D), k (T, B, Hk, D) in float32, bfloat16 or float16, unit stride along the last axis; D up to 256.
+    q_weight, k_weight (D,) in float32 or the type of q (both alike), or None.  positions (T, B, axes), or (T, axes) for all
+    samples, int32 or int64; sections: how many of the D // 2 pairs (2i, 2i + 1) each axis turns, in order -- pair j of a
+    section of n turns by position * base ** (-j / n), angles formed in 64 bits; pairs behind the sections are not turned.
+    For the (pixel, word) sequence of the mSRU (token n = s * L + t) `map_positions` gives (word, row, column).
+    Returns the new q and k, contiguous."""
+    name = "head_norm_rotary"
+    if not torch.is_tensor(q) or q.dim() != 4 or q.dtype not in _DTYPE_IDS:
+        raise RuntimeError("dms_amd.%s: q must be a float32, bfloat16 or float16 tensor (T, B, heads, width)" % name)
+    T, B, _, D = q.shape
+    _chk_rows(name, "q", q, q.shape, q.dtype, q.device)
+    if not torch.is_tensor(k) or k.dim() != 4:
+        raise RuntimeError("dms_amd.%s: k must have 4 axes like q" % name)
+    _chk_rows(name, "k", k, (T, B, k.shape[2], D), q.dtype, q.device)
+    if q.shape[2] < 1 or k.shape[2] < 1 or not 1 <= D <= HEAD_NORM_ROTARY_MAX_WIDTH:
+        raise RuntimeError("dms_amd.%s: at least one head each, of width 1 .. %d, got %s and %s"
+                           % (name, HEAD_NORM_ROTARY_MAX_WIDTH, tuple(q.shape), tuple(k.shape)))
+    for what, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        if not torch.is_tensor(w) or w.dtype not in (torch.float32, q.dtype):
+            raise RuntimeError("dms_amd.%s: %s must be float32 or %s" % (name, what, q.dtype))
+        _chk_rows(name, what, w, (D,), w.dtype, q.device)
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise RuntimeError("dms_amd.%s: q_weight and k_weight must have the same type" % name)
+    sections = tuple(int(n) for n in sections)
+    if len(sections) > 4 or any(n < 0 for n in sections) or sum(sections) > D // 2:
+        raise RuntimeError("dms_amd.%s: up to 4 sections of together at most %d pairs, got %s" % (name, D // 2, sections))
+    if sections:
+        if (not torch.is_tensor(positions) or not positions.is_cuda or positions.device != q.device
+                or positions.dtype not in (torch.int32, torch.int64)
+                or positions.shape not in ((T, B, len(sections)), (T, len(sections)))):
+            raise RuntimeError("dms_amd.%s: positions must be an int32 or int64 tensor (%d, %d, %d) or (%d, %d) on %s"
+                               % (name, T, B, len(sections), T, len(sections), q.device))
+    else:
+        positions = None
+    base, eps = float(base), float(eps)
+    if not base > 0.0:
+        raise RuntimeError("dms_amd.%s: base must be positive" % name)
+    args = (q, k, q_weight, k_weight, positions, sections, base, eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return _HeadNormRotary.apply(*args)
+    return _head_norm_rotary_raw(*args)
+
+
+def map_positions(H, W, L, device):
+    """(H*W*L, 3) int32 positions (word, row, column) of the (pixel, word) sequence n = (y*W + x)*L + t that mix_bcast_add
+    writes and the mSRU runs over."""
+    n = torch.arange(H * W * L, device=device, dtype=torch.int32)
+    s = n // L
+    return torch.stack([n - s * L, s // W, s % W], -1)
