@@ -28,7 +28,7 @@ struct Role {
 };
 
 struct Args {
-    Role role[3];
+    Role role[2];
     const float *g;
     long long gt, gb, gh;
     const void *lengths;
@@ -58,12 +58,15 @@ inline int elem_size(int dtype) { return dtype == DTYPE_F32 ? 4 : 2; }
 // tokens of a chunk: see linear_attention.inl
 inline int chunk_tokens(int dtype) { return dtype == DTYPE_BF16 ? 64 : 32; }
 
-// state_only: the states after each segment (from s_in for segment 0, from zero for the others) and nothing else.
-// DC, DZ in {32/32, 64/64, 64/128, 128/64, 128/128}.  Returns launch_status.
-template <typename T> int launch_chunks(const Args &a, int DC, int DZ, bool state_only, hipStream_t stream);
-extern template int launch_chunks<float>(const Args &, int, int, bool, hipStream_t);
-extern template int launch_chunks<__bf16>(const Args &, int, int, bool, hipStream_t);
-extern template int launch_chunks<_Float16>(const Args &, int, int, bool, hipStream_t);
+// kind, bits:
+constexpr int STATES = 1;      // the states after each segment (from s_in for segment 0, from zero for the others), nothing else
+constexpr int PAIR = 2;        // role[0] and role[1] are dv and dk: one workgroup does both
+constexpr int FINE_PASS = 4;   // 16-bit types: x S to 24 bits, for outputs whose dots are summed over the sequence
+// DC, DZ (of role[0]) in {32/32, 64/64, 64/128, 128/64, 128/128}.  Returns launch_status.
+template <typename T> int launch_chunks(const Args &a, int DC, int DZ, int kind, hipStream_t stream);
+extern template int launch_chunks<float>(const Args &, int, int, int, hipStream_t);
+extern template int launch_chunks<__bf16>(const Args &, int, int, int, hipStream_t);
+extern template int launch_chunks<_Float16>(const Args &, int, int, int, hipStream_t);
 
 }  // namespace la
 }  // namespace dmn

@@ -201,6 +201,15 @@ static void plan_segments(int dtype, int T, long long passes, int *nseg, int *se
     *nseg = nchunks ? (nchunks + *seg_chunks - 1) / *seg_chunks : 1;
 }
 
+// a chunk of tokens has to lie within the 4 GiB that a buffer access reaches
+static bool reaches(const long long *s, int T, int tensors)
+{
+    if (T <= 1) return true;
+    for (int i = 0; i < tensors; ++i)
+        if (s[3 * i] < 0 || s[3 * i] > (1LL << 24) + (1 << 20)) return false;
+    return true;
+}
+
 static Tensor tensor(const void *p, int dtype, int T, int B, int heads, int H, int d, const long long *s)
 {
     Tensor t;
@@ -226,21 +235,21 @@ static Tensor dense(void *p, int dtype, int T, int B, int H, int d)
 
 static long long up4(long long n) { return (n + 3) & ~3LL; }
 
-static int launch(int dtype, const Args &a, int DC, int DZ, bool state_only, hipStream_t stream)
+static int launch(int dtype, const Args &a, int DC, int DZ, int kind, hipStream_t stream)
 {
-    if (dtype == DTYPE_BF16) return launch_chunks<__bf16>(a, DC, DZ, state_only, stream);
-    if (dtype == DTYPE_F16) return launch_chunks<_Float16>(a, DC, DZ, state_only, stream);
-    return launch_chunks<float>(a, DC, DZ, state_only, stream);
+    if (dtype == DTYPE_BF16) return launch_chunks<__bf16>(a, DC, DZ, kind, stream);
+    if (dtype == DTYPE_F16) return launch_chunks<_Float16>(a, DC, DZ, kind, stream);
+    return launch_chunks<float>(a, DC, DZ, kind, stream);
 }
 
 // all passes of `a` (same DC, DZ): states between segments first where there are several
-static int run_passes(int dtype, Args &a, int DC, int DZ, float *ws, hipStream_t stream)
+static int run_passes(int dtype, Args &a, int DC, int DZ, int kind, float *ws, hipStream_t stream)
 {
     if (a.nseg > 1) {
         const long long rows = (long long)a.nroles * a.B * a.H;
         a.states = ws;
         a.decays = ws + rows * a.nseg * DC * DZ;
-        int rc = launch(dtype, a, DC, DZ, true, stream);
+        int rc = launch(dtype, a, DC, DZ, kind | STATES, stream);
         if (rc) return rc;
         if (a.nseg > 2) {
             const int n4 = DC * DZ / 4;
@@ -250,7 +259,7 @@ static int run_passes(int dtype, Args &a, int DC, int DZ, float *ws, hipStream_t
             if (rc) return rc;
         }
     }
-    return launch(dtype, a, DC, DZ, false, stream);
+    return launch(dtype, a, DC, DZ, kind, stream);
 }
 
 static long long passes_floats(int nroles, long long BH, int nseg, int DC, int DZ)
@@ -265,7 +274,7 @@ static int check(const char *who, int dtype, int T, int B, int H, int Hq, int Hk
         return fail(-3, "%s: bad sizes T=%d B=%d H=%d Hq=%d Hk=%d Hv=%d", who, T, B, H, Hq, Hk, Hv);
     if (H % Hq || H % Hk || H % Hv) return fail(-4, "%s: the %d heads of the state must be a multiple of Hq=%d, Hk=%d and Hv=%d", who, H, Hq, Hk, Hv);
     if (dk < 1 || dk > 128 || dv < 1 || dv > 128) return fail(-5, "%s: head widths must be 1 .. 128, got dk=%d dv=%d", who, dk, dv);
-    if ((long long)B * H > (1 << 22)) return fail(-6, "%s: B * H = %lld exceeds 2^22", who, (long long)B * H);
+    if ((long long)B * H > (1 << 17)) return fail(-6, "%s: B * H = %lld exceeds 2^17", who, (long long)B * H);
     if (T > 0x3fffffff) return fail(-6, "%s: T = %d exceeds 2^30", who, T);
     return 0;
 }
@@ -287,21 +296,20 @@ static void fill_common(Args &a, const float *g, const long long *gs, const void
 
 // the backward's passes: where each one's piece of the workspace begins
 struct BwdPlan {
-    int DCv, DZv, DCk, DZk, nseg, seg_chunks;             // of the (dq, dk) passes: contraction over dv; of the dv pass: over dk
-    long long pair, single, dots, dq, dk, dv, ds0, part, total;
+    int DK, DV, nseg, seg_chunks;
+    long long one, pair, dots, dq, dk, dv, ds0, part, total;
 };
 
 static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)
 {
     BwdPlan p;
-    pad_pair(dv, dk, &p.DCv, &p.DZv);
-    pad_pair(dk, dv, &p.DCk, &p.DZk);
+    pad_pair(dk, dv, &p.DK, &p.DV);
     const long long BH = (long long)B * H, rows = (long long)T * BH;
-    plan_segments(dtype, T, 3 * BH, &p.nseg, &p.seg_chunks);
+    plan_segments(dtype, T, BH, &p.nseg, &p.seg_chunks);
     long long at = 0;
     const auto take = [&at](long long n) { const long long o = at; at += up4(n); return o; };
-    p.pair = take(passes_floats(3, BH, p.nseg, p.DCv, p.DZv));        // 3: one launch of all where dk and dv are padded alike
-    p.single = take(passes_floats(1, BH, p.nseg, p.DCk, p.DZk));
+    p.one = take(passes_floats(1, BH, p.nseg, p.DK, p.DV));
+    p.pair = take(passes_floats(2, BH, p.nseg, p.DK, p.DV));
     p.dots = take(2 * rows);
     p.dq = take(Hq < H ? rows * dk : 0);
     p.dk = take(Hk < H ? rows * dk : 0);
@@ -376,6 +384,7 @@ extern "C" int dmn_linear_attention_fwd(int dtype, const void *q, const void *k,
     int rc = check(who, dtype, T, B, H, Hq, Hk, Hv, dk, dv);
     if (rc) return rc;
     if (!strides || (B > 0 && T > 0 && (!q || !k || !v || !g || !o))) return fail(-1, "%s: null pointer", who);
+    if (!reaches(strides, T, 3)) return fail(-8, "%s: a token's stride must be 0 .. 2^24 + 2^20 elements", who);
     if (B == 0) return 0;
     Args a;
     fill_common(a, g, strides + 9, lengths, lengths64, T, B, H);
@@ -398,8 +407,7 @@ extern "C" int dmn_linear_attention_fwd(int dtype, const void *q, const void *k,
     r.scale_p = r.scale_x = scale;
     r.scale_z = 1.0f;
     r.reverse = r.last_decay = 0;
-    a.role[1] = a.role[2] = r;
-    return run_passes(dtype, a, DC, DZ, workspace, (hipStream_t)stream);
+    return run_passes(dtype, a, DC, DZ, 0, workspace, (hipStream_t)stream);
 }
 
 extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k, const void *v, const float *g, const float *state0,
@@ -411,6 +419,7 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
     int rc = check(who, dtype, T, B, H, Hq, Hk, Hv, dk, dv);
     if (rc) return rc;
     if (!strides || (B > 0 && T > 0 && (!q || !k || !v || !g || !grad_o))) return fail(-1, "%s: null pointer", who);
+    if (!reaches(strides, T, 3) || !reaches(strides + 12, T, 1)) return fail(-8, "%s: a token's stride must be 0 .. 2^24 + 2^20 elements", who);
     hipStream_t st = (hipStream_t)stream;
     if (B == 0) {
         if (grad_g && grad_g_per_head) {
@@ -433,13 +442,14 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         t.f32 = 1;
         return t;
     };
+    const int fine = grad_g ? FINE_PASS : 0;
     Args a;
     fill_common(a, g, strides + 9, lengths, lengths64, T, B, H);
     a.nseg = p.nseg;
     a.seg_chunks = p.seg_chunks;
-    a.nroles = 0;
     if (grad_q || grad_g) {                               // dq: the operator on (dO, v, k)
-        Role &r = a.role[a.nroles++];
+        a.nroles = 1;
+        Role &r = a.role[0];
         r.X = D; r.Y = V; r.Z = K; r.W = Q;
         r.O = output(grad_q, workspace + p.dq, Hq, dk);
         r.s_in = state0;
@@ -450,25 +460,13 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         r.scale_p = r.scale_x = scale;
         r.scale_z = 1.0f;
         r.reverse = r.last_decay = 0;
+        rc = run_passes(dtype, a, p.DV, p.DK, fine, workspace + p.one, st);
+        if (rc) return rc;
     }
-    if (grad_k || grad_g) {                               // dk: backwards in time, on (v, dO, q)
-        Role &r = a.role[a.nroles++];
-        r.X = V; r.Y = D; r.Z = Q; r.W = K;
-        r.O = output(grad_k, workspace + p.dk, Hk, dk);
-        r.s_in = grad_state;
-        r.s_out = nullptr;
-        r.in_c = r.out_c = 1;
-        r.in_z = r.out_z = dv;
-        r.dots = grad_g ? dots + (size_t)T * B * H : nullptr;
-        r.scale_p = r.scale_z = scale;
-        r.scale_x = 1.0f;
-        r.reverse = 1;
-        r.last_decay = 0;
-    }
-    const bool third = grad_v || need_ds0;
-    Role rv;
-    if (third) {                                          // dv and dS_0: backwards in time, on (k, q, dO)
-        rv.X = K; rv.Y = Q; rv.Z = D; rv.W = V;
+    if (grad_k || grad_v || grad_g || grad_state0) {
+        a.nroles = 2;
+        Role &rv = a.role[0], &rk = a.role[1];
+        rv.X = K; rv.Y = Q; rv.Z = D; rv.W = V;           // dv and dS_0: backwards in time, on (k, q, dO)
         rv.O = output(grad_v, workspace + p.dv, Hv, dv);
         rv.s_in = grad_state;
         rv.s_out = need_ds0 ? ds0 : nullptr;
@@ -478,18 +476,14 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         rv.scale_p = rv.scale_z = scale;
         rv.scale_x = 1.0f;
         rv.reverse = rv.last_decay = 1;
-    }
-    if (third && p.DCv == p.DCk && p.DZv == p.DZk) {
-        a.role[a.nroles++] = rv;
-    } else if (third) {
-        Args one = a;
-        one.nroles = 1;
-        one.role[0] = rv;
-        rc = run_passes(dtype, one, p.DCk, p.DZk, workspace + p.single, st);
-        if (rc) return rc;
-    }
-    if (a.nroles > 0) {
-        rc = run_passes(dtype, a, p.DCv, p.DZv, workspace + p.pair, st);
+        rk = rv;
+        rk.X = V; rk.Y = D; rk.Z = Q; rk.W = K;           // dk: the same on (v, dO, q), with the states transposed
+        rk.O = output(grad_k, workspace + p.dk, Hk, dk);
+        rk.s_out = nullptr;
+        rk.in_c = rk.out_c = 1;
+        rk.in_z = rk.out_z = dv;
+        rk.dots = grad_g ? dots + (size_t)T * B * H : nullptr;
+        rc = run_passes(dtype, a, p.DK, p.DV, fine | PAIR, workspace + p.pair, st);
         if (rc) return rc;
     }
     if (grad_g) {

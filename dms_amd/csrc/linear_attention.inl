@@ -25,74 +25,49 @@
 namespace dmn {
 namespace la {
 
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Kind;      // planes of an operand of the call's type, and of a computed one
 template <> struct Kind<float> { static constexpr int NP = 3, NC = 3; };
 template <> struct Kind<__bf16> { static constexpr int NP = 1, NC = 2; };
 template <> struct Kind<_Float16> { static constexpr int NP = 2, NC = 2; };
+constexpr int NS = 3;                   // planes of 2^{G_C - G_j} z_j in the state: the state is an fp32 output
 
-template <typename T> struct alignas(16) Row8 { T v[8]; };
-
-// eight elements of a row from column c on, zero behind column d
-template <typename T>
-__device__ __forceinline__ Row8<T> fetch8(const T *row, int c, int d, int vec)
-{
-    Row8<T> r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = (T)0.0f;
-    if (vec == 2) {
-        constexpr int W = 16 / (int)sizeof(T);
-        struct alignas(16) V { T v[W]; };
-#pragma unroll
-        for (int i = 0; i < 8; i += W)
-            if (c + i < d) {
-                const V t = *reinterpret_cast<const V *>(row + c + i);
-#pragma unroll
-                for (int j = 0; j < W; ++j) r.v[i + j] = t.v[j];
-            }
-    } else if (vec == 1) {
-        constexpr int W = 8 / (int)sizeof(T);
-        struct alignas(8) V { T v[W]; };
-#pragma unroll
-        for (int i = 0; i < 8; i += W)
-            if (c + i < d) {
-                const V t = *reinterpret_cast<const V *>(row + c + i);
-#pragma unroll
-                for (int j = 0; j < W; ++j) r.v[i + j] = t.v[j];
-            }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < d) r.v[i] = row[c + i];
-    }
-    return r;
-}
-
-// x as a sum of N bf16 numbers, each the rounded rest of the ones before it
+// two numbers as sums of N bf16 pairs, each the rounded rest of the ones before it
 template <int N>
-__device__ __forceinline__ void split(float x, __bf16 (&p)[N])
+__device__ __forceinline__ void split2(float x, float y, unsigned (&p)[N])
 {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        p[i] = (__bf16)x;
-        x -= (float)p[i];
+        p[i] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){x, y}, b16x2));
+        if (i + 1 < N) {
+            x -= __builtin_bit_cast(float, p[i] << 16);
+            y -= __builtin_bit_cast(float, p[i] & 0xffff0000u);
+        }
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void split8(const Row8<T> &r, b16x8 (&p)[Kind<T>::NP])
+// eight numbers as N planes, the operand of a matrix instruction
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], b16x8 (&p)[N])
 {
+    u32x4 w[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        __bf16 q[Kind<T>::NP];
-        split<Kind<T>::NP>((float)r.v[i], q);
+    for (int j = 0; j < 4; ++j) {
+        unsigned q[N];
+        split2<N>(x[2 * j], x[2 * j + 1], q);
 #pragma unroll
-        for (int k = 0; k < Kind<T>::NP; ++k) p[k][i] = q[k];
+        for (int k = 0; k < N; ++k) w[k][j] = q[k];
     }
+#pragma unroll
+    for (int k = 0; k < N; ++k) p[k] = __builtin_bit_cast(b16x8, w[k]);
 }
 
 // acc += sum of a[i] b[j] over the pairs that reach the precision of the finer operand
@@ -116,28 +91,461 @@ __device__ __forceinline__ b16x4 read_tr(const __bf16 *p)
     return __builtin_bit_cast(b16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p)));
 }
 
-template <typename T, int DC, int DZ, int C, bool STATE_ONLY>
-struct Shared {
-    static constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC;
-    static constexpr int LC = DC + 8, LZ = DZ + 8, LP = C + 8;
-    alignas(16) __bf16 X[STATE_ONLY ? 1 : NP][STATE_ONLY ? 1 : C][LC];
-    alignas(16) __bf16 Y[NP][C][LC];
-    alignas(16) __bf16 Z[NP][C][LZ];
-    alignas(16) __bf16 P[STATE_ONLY ? 1 : NC][STATE_ONLY ? 1 : C][LP];
-    float Gh[C], Gl[C], E[C], R[C];     // G_i as two floats, 2^{G_i}, 2^{G_C - G_i}
-    float tot;                          // 2^{G_C}
-    float dot[8][C];
+__device__ __forceinline__ b16x8 join(b16x4 a, b16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// Buffer accesses: an offset of NOWHERE reads zero and writes nothing, so rows and columns that do not exist cost no branch.
+constexpr unsigned NOWHERE = 0xffffffffu;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *p)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, 0xfffffff0u, 0x00027000);
+}
+
+// A tile of C tokens x D elements of one tensor, on its way from memory to LDS: 16 bytes a thread and unit.
+// VEC: the pieces that every row's start and width allow (2: 16 bytes, 1: 8 bytes, 0: single elements).
+template <typename T, int D, int C, int NTHR, int VEC>
+struct Tile {
+    static constexpr int UE = 16 / (int)sizeof(T), PER = D / UE, N = C * PER, U = (N + NTHR - 1) / NTHR, LD = D + 8;
+    static constexpr int NP = Kind<T>::NP;
+    u32x4 raw[U];
+    const char *p;             // token 0 of the sample and head
+    long long st;              // bytes from token to token
+    unsigned off, step;
+    int row, dcol, lds, lds_step;
+
+    // backwards: token t0 + r goes into row C - 1 - r
+    __device__ __forceinline__ void init(const Tensor &x, int b, int h, int tid, int reverse)
+    {
+        p = x.p + ((long long)b * x.sb + (long long)(h / x.group) * x.sh) * (int)sizeof(T);
+        st = x.st * (int)sizeof(T);
+        const int c = (tid % PER) * UE;
+        row = tid / PER;
+        off = (unsigned)row * (unsigned)st + (unsigned)(c * (int)sizeof(T));
+        step = (unsigned)(NTHR / PER) * (unsigned)st;
+        dcol = x.d - c;
+        lds = (reverse ? C - 1 - row : row) * LD + c;
+        lds_step = (reverse ? -1 : 1) * (NTHR / PER) * LD;
+        if (dcol <= 0 || row >= C) row = 1 << 20;
+    }
+    // tokens t0 .. t0 + n - 1, zeros behind them
+    __device__ __forceinline__ void fetch(long long t0, int n)
+    {
+        const __amdgpu_buffer_rsrc_t rs = buffer(p + t0 * st);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool ok = row + u * (NTHR / PER) < n;
+            const unsigned o = off + u * step;
+            if (VEC == 2) {
+                raw[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, ok ? o : NOWHERE, 0, 0);
+            } else if (VEC == 1) {
+                const u32x2 a = __builtin_amdgcn_raw_buffer_load_b64(rs, ok ? o : NOWHERE, 0, 0);
+                const u32x2 b = __builtin_amdgcn_raw_buffer_load_b64(rs, ok && UE / 2 < dcol ? o + 8 : NOWHERE, 0, 0);
+                raw[u] = (u32x4){a.x, a.y, b.x, b.y};
+            } else if (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[u][i] = __builtin_amdgcn_raw_buffer_load_b32(rs, ok && i < dcol ? o + 4 * i : NOWHERE, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned lo = __builtin_amdgcn_raw_buffer_load_b16(rs, ok && 2 * i < dcol ? o + 4 * i : NOWHERE, 0, 0);
+                    const unsigned hi = __builtin_amdgcn_raw_buffer_load_b16(rs, ok && 2 * i + 1 < dcol ? o + 4 * i + 2 : NOWHERE, 0, 0);
+                    raw[u][i] = lo | hi << 16;
+                }
+            }
+        }
+    }
+    // into LDS planes of C rows of LD elements; the last thread's units may lie behind the tile
+    __device__ __forceinline__ void store(__bf16 *tile, int tid) const
+    {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (U * NTHR > N && tid + u * NTHR >= N) break;
+            __bf16 *q = tile + lds + u * lds_step;
+            if constexpr (sizeof(T) == 4) {
+                unsigned a[NP], b[NP];
+                const f32x4 x = __builtin_bit_cast(f32x4, raw[u]);
+                split2<NP>(x[0], x[1], a);
+                split2<NP>(x[2], x[3], b);
+#pragma unroll
+                for (int k = 0; k < NP; ++k) *reinterpret_cast<u32x2 *>(q + k * C * LD) = (u32x2){a[k], b[k]};
+            } else if constexpr (NP == 1) {
+                *reinterpret_cast<u32x4 *>(q) = raw[u];
+            } else {
+                typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+                const h16x8 h = __builtin_bit_cast(h16x8, raw[u]);
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+                b16x8 w[NP];
+                dmn::la::split8<NP>(x, w);
+#pragma unroll
+                for (int k = 0; k < NP; ++k) *reinterpret_cast<b16x8 *>(q + k * C * LD) = w[k];
+            }
+        }
+    }
 };
 
-template <typename T, int DC, int DZ, int C, int NW, bool STATE_ONLY>
-__global__ void __launch_bounds__(64 * NW) chunk_kernel(const Args a)
+// The decays of a chunk, in the order in which its rows are walked (row r is token r, or C - 1 - r where time runs backwards)
+template <int C>
+struct alignas(16) Decays {
+    float Gh[C], Gl[C];        // G_i as two floats
+    float E[C], R[C];          // 2^{G_i} scale_x, 2^{G_C - G_i} scale_z
+    float F[C];                // 2^{G_e - G_i}, e the last row of i's 16
+    float tot;                 // 2^{G_C}
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double shifted(double v)
 {
-    constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC;
-    constexpr int NT = DZ / 16 / NW;                 // 16-column tiles of a wave
-    constexpr int NTHR = 64 * NW;
-    constexpr int UC = (C * DC / 8 + NTHR - 1) / NTHR, UZ = (C * DZ / 8 + NTHR - 1) / NTHR;
-    constexpr int CT = C / 16;
-    __shared__ Shared<T, DC, DZ, C, STATE_ONLY> sm;
+    const unsigned long long x = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+__device__ __forceinline__ double lane_value(double v, int lane)
+{
+    const unsigned long long x = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+// one wave; returns G_C
+template <int C>
+__device__ __forceinline__ double decays(float g, int lane, float scale_x, float scale_z, Decays<C> &d)
+{
+    double G = log2_decay(g);
+    G += shifted<0x111, 0xf>(G);                   // row_shr 1, 2, 4, 8: inclusive sums of 16 lanes
+    G += shifted<0x112, 0xf>(G);
+    G += shifted<0x114, 0xf>(G);
+    G += shifted<0x118, 0xf>(G);
+    G += shifted<0x142, 0xa>(G);                   // row_bcast 15, 31: of 64
+    if (C > 32) G += shifted<0x143, 0xc>(G);
+    const double tot = lane_value(G, C - 1);
+    const double ends[4] = {lane_value(G, 15), lane_value(G, 31), lane_value(G, C > 32 ? 47 : 15), lane_value(G, C > 32 ? 63 : 15)};
+    const double end = lane < 16 ? ends[0] : lane < 32 ? ends[1] : lane < 48 ? ends[2] : ends[3];
+    if (lane < C) {
+        const float hi = (float)G;
+        d.Gh[lane] = hi;
+        d.Gl[lane] = (float)(G - (double)hi);
+        d.E[lane] = fast_exp2(hi) * scale_x;
+        d.R[lane] = fast_exp2((float)(tot - G)) * scale_z;
+        d.F[lane] = fast_exp2((float)(end - G));
+        if (lane == 0) d.tot = fast_exp2((float)tot);
+    }
+    return tot;
+}
+
+// The part of a chunk that one pass (one Role) does, by its NW waves; x, y, z are LDS tiles of NP planes.
+template <typename T, int DC, int DZ, int C, int NW, int NX, bool STATE_ONLY>
+struct Pass {
+    static constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC;
+    static constexpr int NT = DZ / 16 / NW, CT = C / 16, KT = DC / 16;     // tiles of 16: a wave's columns, tokens, rows of S
+    static constexpr int LC = DC + 8, LZ = DZ + 8, LP = C + 8;
+    f32x4 S[KT][NT];
+    f32x4 O[STATE_ONLY ? 1 : CT][NT];
+
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) S[t][n] = (f32x4){0, 0, 0, 0};
+    }
+    // tile t, row r of S is row 16 t + r
+    __device__ __forceinline__ void load_state(const float *p, int dc, int dz, int in_c, int in_z, int z0, int lr, int lg)
+    {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = 16 * t + 4 * lg + i, z = z0 + 16 * n + lr;
+                    if (c < dc && z < dz) S[t][n][i] = p[c * in_c + z * in_z];
+                }
+    }
+    __device__ __forceinline__ void store_state(float *p, int dc, int dz, int out_c, int out_z, int z0, int lr, int lg, float more) const
+    {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = 16 * t + 4 * lg + i, z = z0 + 16 * n + lr;
+                    if (c < dc && z < dz) p[c * out_c + z * out_z] = S[t][n][i] * more;
+                }
+    }
+
+    // 2^{G_i - G_j} (x_i . y_j) scale_p for j <= i, into P[plane][i][j].  The 16 x 16 tiles on and below the diagonal go round the
+    // waves, and so do the tiles right of a diagonal one that a product 32 wide reads: zeros.  The tiles are computed
+    // transposed: a lane holds one row i and 4 adjacent j.  Off the diagonal the decay is 2^{G_i - G_e} 2^{G_e - G_j}, e the last
+    // token of j's 16, both factors at most 1: an exponential for 4 numbers in place of one for each.
+    __device__ __forceinline__ void scores(const __bf16 *x, const __bf16 *y, __bf16 *P, const Decays<C> &d, float scale_p, int wave, int lr, int lg)
+    {
+        constexpr int NTILE = CT * (CT + 1) / 2, ALL = NTILE + CT / 2;
+#pragma unroll
+        for (int k0 = 0; k0 < (ALL + NW - 1) / NW; ++k0) {
+            const int e = wave + k0 * NW;
+            if (e >= ALL) break;
+            if (e >= NTILE) {
+                const int I = 2 * (e - NTILE);
+#pragma unroll
+                for (int k = 0; k < NC; ++k) *reinterpret_cast<u32x2 *>(P + (k * C + I * 16 + lr) * LP + (I + 1) * 16 + 4 * lg) = (u32x2){0, 0};
+                continue;
+            }
+            const int I = (e >= 1) + (e >= 3) + (e >= 6), J = e - I * (I + 1) / 2;
+            f32x4 p = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < DC / 32; ++s) {
+                b16x8 xf[NP], yf[NP];
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    xf[k] = *reinterpret_cast<const b16x8 *>(x + (k * C + I * 16 + lr) * LC + 32 * s + 8 * lg);
+                    yf[k] = *reinterpret_cast<const b16x8 *>(y + (k * C + J * 16 + lr) * LC + 32 * s + 8 * lg);
+                }
+                p = mma<NP, NP>(yf, xf, p);
+            }
+            const int i = I * 16 + lr, j0 = J * 16 + 4 * lg;
+            const float gh = d.Gh[i], gl = d.Gl[i];
+            if (I == J) {
+                const f32x4 jh = *reinterpret_cast<const f32x4 *>(&d.Gh[j0]), jl = *reinterpret_cast<const f32x4 *>(&d.Gl[j0]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[r] = j0 + r > i ? 0.0f : p[r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
+            } else {
+                const f32x4 f = *reinterpret_cast<const f32x4 *>(&d.F[j0]);
+                const float row = fast_exp2((gh - d.Gh[J * 16 + 15]) + (gl - d.Gl[J * 16 + 15])) * scale_p;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[r] *= row * f[r];
+            }
+            unsigned a[NC], b[NC];
+            split2<NC>(p[0], p[1], a);
+            split2<NC>(p[2], p[3], b);
+#pragma unroll
+            for (int k = 0; k < NC; ++k) *reinterpret_cast<u32x2 *>(P + (k * C + i) * LP + j0) = (u32x2){a[k], b[k]};
+        }
+    }
+
+    // O^T = 2^{G_i} S^T x^T.  The accumulators of S, converted, are the operand: slots 4u + i of lane group g are row
+    // 32 s + 16 u + 4 g + i of S, and x is read in that order.
+    __device__ __forceinline__ void from_state(const __bf16 *x, const Decays<C> &d, int lr, int lg)
+    {
+#pragma unroll
+        for (int I = 0; I < CT; ++I)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) O[I][n] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < DC / 32; ++s) {
+            b16x8 st[NT][NX];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = S[2 * s + j / 4][n][j % 4];
+                split8<NX>(w, st[n]);
+            }
+#pragma unroll
+            for (int I = 0; I < CT; ++I) {
+                b16x8 xf[NP];
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    const __bf16 *q = x + (k * C + I * 16 + lr) * LC + 32 * s + 4 * lg;
+                    xf[k] = join(*reinterpret_cast<const b16x4 *>(q), *reinterpret_cast<const b16x4 *>(q + 16));
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) O[I][n] = mma<NX, NP>(st[n], xf, O[I][n]);
+            }
+        }
+#pragma unroll
+        for (int I = 0; I < CT; ++I) {
+            const float e = d.E[I * 16 + lr];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) O[I][n] *= e;
+        }
+    }
+
+    // by 32 tokens: O^T += z^T P^T;  S = 2^{G_C} S + y^T (2^{G_C - G_j} z_j)
+    __device__ __forceinline__ void from_chunk(const __bf16 *y, const __bf16 *z, const __bf16 *P, const Decays<C> &d, int z0, int lr, int lg)
+    {
+        const float tot = d.tot;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) S[t][n] *= tot;
+#pragma unroll
+        for (int s = 0; s < C / 32; ++s) {
+            b16x8 zs[NT][NS];
+            const int row = 32 * s + 8 * lg;
+            const f32x4 r0 = *reinterpret_cast<const f32x4 *>(&d.R[row]), r1 = *reinterpret_cast<const f32x4 *>(&d.R[row + 4]);
+            b16x8 zf[NT][NP];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    const __bf16 *q = z + (k * C + row + lr / 4) * LZ + z0 + 16 * n + 4 * (lr % 4);
+                    zf[n][k] = join(read_tr(q), read_tr(q + 4 * LZ));
+                }
+            }
+            if (!STATE_ONLY) {
+#pragma unroll
+                for (int I = 2 * s; I < CT; ++I) {
+                    b16x8 pf[NC];
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) pf[k] = *reinterpret_cast<const b16x8 *>(P + (k * C + I * 16 + lr) * LP + row);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) O[I][n] = mma<NP, NC>(zf[n], pf, O[I][n]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = (float)zf[n][NP - 1][j];
+#pragma unroll
+                    for (int k = NP - 2; k >= 0; --k) w[j] += (float)zf[n][k][j];
+                    w[j] *= j < 4 ? r0[j % 4] : r1[j % 4];
+                }
+                split8<NS>(w, zs[n]);
+            }
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                b16x8 yf[NP];
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    const __bf16 *q = y + (k * C + row + lr / 4) * LC + 16 * t + 4 * (lr % 4);
+                    yf[k] = join(read_tr(q), read_tr(q + 4 * LC));
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) S[t][n] = mma<NP, NS>(yf, zs[n], S[t][n]);
+            }
+        }
+    }
+
+    // rows of o: row r is token t0 + r, or t0 + C - 1 - r where time runs backwards; valid ones lie before token `len`
+    __device__ __forceinline__ void store_rows(const Role &ro, long long t0, int len, int b, int h, int z0, int lr, int lg, float *dots)
+    {
+        const Tensor &o = ro.O;
+        if (o.p) {
+            const int es = o.f32 ? 4 : (int)sizeof(T);
+            const __amdgpu_buffer_rsrc_t rs = buffer(o.p + (t0 * o.st + (long long)b * o.sb + (long long)h * o.sh) * es);
+            const unsigned st = (unsigned)o.st * es;
+#pragma unroll
+            for (int I = 0; I < CT; ++I) {
+                const int r = I * 16 + lr, at = ro.reverse ? C - 1 - r : r;
+                const bool ok = t0 + at < len;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int c = z0 + 16 * n + 4 * lg;
+                    const unsigned off = (unsigned)at * st + (unsigned)(c * es);
+                    if (sizeof(T) == 4 || o.f32) {
+                        if (o.vec == 2) {
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O[I][n]), rs, ok && c < o.d ? off : NOWHERE, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float v = O[I][n][i];          // by value: a bit cast of a vector's element names the vector
+                                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rs, ok && c + i < o.d ? off + 4 * i : NOWHERE,
+                                                                      0, 0);
+                            }
+                        }
+                    } else if constexpr (sizeof(T) == 2) {
+                        typedef T tx4 __attribute__((ext_vector_type(4)));
+                        typedef unsigned short hx4 __attribute__((ext_vector_type(4)));
+                        const tx4 w = __builtin_convertvector(O[I][n], tx4);
+                        if (o.vec >= 1) {
+                            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, w), rs, ok && c < o.d ? off : NOWHERE, 0, 0);
+                        } else {
+                            const hx4 e = __builtin_bit_cast(hx4, w);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                __builtin_amdgcn_raw_buffer_store_b16(e[i], rs, ok && c + i < o.d ? off + 2 * i : NOWHERE, 0, 0);
+                        }
+                    }
+                }
+            }
+        }
+        if (ro.dots) {
+            const Tensor &w = ro.W;
+            const __amdgpu_buffer_rsrc_t rs =
+                buffer(w.p + (t0 * w.st + (long long)b * w.sb + (long long)(h / w.group) * w.sh) * (int)sizeof(T));
+            const unsigned st = (unsigned)w.st * (unsigned)sizeof(T);
+#pragma unroll
+            for (int I = 0; I < CT; ++I) {
+                const int r = I * 16 + lr, at = ro.reverse ? C - 1 - r : r;
+                const bool ok = t0 + at < len;
+                float dot = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int c = z0 + 16 * n + 4 * lg;
+                    const unsigned off = (unsigned)at * st + (unsigned)(c * (int)sizeof(T));
+                    f32x4 x;
+                    if constexpr (sizeof(T) == 4) {
+                        if (w.vec == 2) {
+                            x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, ok && c < w.d ? off : NOWHERE, 0, 0));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, ok && c + i < w.d ? off + 4 * i : NOWHERE, 0, 0));
+                        }
+                    } else {
+                        typedef T tx4 __attribute__((ext_vector_type(4)));
+                        typedef unsigned short hx4 __attribute__((ext_vector_type(4)));
+                        tx4 y;
+                        if (w.vec >= 1) {
+                            y = __builtin_bit_cast(tx4, __builtin_amdgcn_raw_buffer_load_b64(rs, ok && c < w.d ? off : NOWHERE, 0, 0));
+                        } else {
+                            hx4 e;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, ok && c + i < w.d ? off + 2 * i : NOWHERE, 0, 0);
+                            y = __builtin_bit_cast(tx4, e);
+                        }
+                        x = __builtin_convertvector(y, f32x4);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dot += x[i] * O[I][n][i];
+                }
+                dot += __shfl_xor(dot, 16);
+                dot += __shfl_xor(dot, 32);
+                if (lg == 0) dots[at] = dot;
+            }
+        }
+    }
+};
+
+// Waves of a pass: one 16-column tile of the state each where three planes fill the registers (fp32 with 128 columns), two
+// tiles elsewhere.
+template <typename T, int DZ> constexpr int waves() { return DZ / 16 < 4 ? DZ / 16 : (DZ == 128 && Kind<T>::NP == 3 ? 8 : 4); }
+template <typename T> constexpr int chunk() { return Kind<T>::NP == 1 ? 64 : 32; }       // chunk_tokens()
+
+// rows first .. behind - 1 of o that lie behind the sample's length: zeros
+template <typename T>
+__device__ __forceinline__ void zero_rows(const Role &ro, int len, int first, int behind, int b, int h, int tid, int nthr)
+{
+    if (!ro.O.p) return;
+    const int r0 = max(first, len), d = ro.O.d;
+    for (long long e = tid; e < (long long)(behind - r0) * d; e += nthr) {
+        const long long at = (r0 + e / d) * ro.O.st + b * ro.O.sb + h * ro.O.sh + e % d;
+        if (ro.O.f32) reinterpret_cast<float *>(ro.O.p)[at] = 0.0f;
+        else reinterpret_cast<T *>(ro.O.p)[at] = (T)0.0f;
+    }
+}
+
+template <typename T, int DC, int DZ, int VEC, bool FINE, bool STATE_ONLY>
+__global__ void __launch_bounds__((64 * waves<T, DZ>())) chunk_kernel(const Args a)
+{
+    constexpr int C = chunk<T>(), NW = waves<T, DZ>(), NTHR = 64 * NW;
+    constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
+    typedef Pass<T, DC, DZ, C, NW, NX, STATE_ONLY> P;
+    struct Shared {
+        alignas(16) __bf16 x[STATE_ONLY ? 8 : NP * C * P::LC];
+        alignas(16) __bf16 y[NP * C * P::LC];
+        alignas(16) __bf16 z[NP * C * P::LZ];
+        alignas(16) __bf16 p[STATE_ONLY ? 8 : NC * C * P::LP];
+        alignas(16) Decays<C> d[2];
+        float dots[NW][C];
+    };
+    __shared__ Shared sm;
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
     const int BH = a.B * a.H;
@@ -146,380 +554,293 @@ __global__ void __launch_bounds__(64 * NW) chunk_kernel(const Args a)
     if (STATE_ONLY && seg == a.nseg - 1) return;     // the last segment's state is nobody's first
     const Role &ro = a.role[ri];
     const int b = bh / a.H, h = bh % a.H;
-    const int len = valid_length(a.lengths, a.lengths64, b, a.T);
-    const int dc = ro.Y.d, dz = ro.Z.d;
-    const int first = seg * a.seg_chunks * C, behind = min(a.T, first + a.seg_chunks * C);   // steps of this segment
-    const int n_live = len > first ? (min(len, behind) - first + C - 1) / C : 0;
-    const int zcol0 = wave * 16 * NT;
-
-    const T *px = STATE_ONLY ? nullptr : reinterpret_cast<const T *>(ro.X.p) + b * ro.X.sb + (h / ro.X.group) * ro.X.sh;
-    const T *py = reinterpret_cast<const T *>(ro.Y.p) + b * ro.Y.sb + (h / ro.Y.group) * ro.Y.sh;
-    const T *pz = reinterpret_cast<const T *>(ro.Z.p) + b * ro.Z.sb + (h / ro.Z.group) * ro.Z.sh;
+    const int len = __builtin_amdgcn_readfirstlane(valid_length(a.lengths, a.lengths64, b, a.T));
+    const int live = (len + C - 1) / C;              // chunks with tokens; backwards the first one is the partial one
+    const int c0 = seg * a.seg_chunks, c1 = min(live, c0 + a.seg_chunks);
+    const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
     const float *pg = a.g + b * a.gb + h * a.gh;
+    const auto token0 = [&](int ci) { return (ro.reverse ? live - 1 - ci : ci) * C; };
 
-    // ---- the state before the segment
-    f32x4 S[DC / 16][NT];
-#pragma unroll
-    for (int t = 0; t < DC / 16; ++t)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) S[t][n] = (f32x4){0, 0, 0, 0};
+    P ps;
+    ps.zero();
     const size_t slot = ((size_t)(ri * BH + bh) * a.nseg + seg) * (DC * DZ);
+    f32x4 *const states = reinterpret_cast<f32x4 *>(a.states + (STATE_ONLY ? slot : slot - DC * DZ)) + wave * P::KT * P::NT * 64 + lane;
     if (seg == 0) {
-        if (ro.s_in) {
-            const float *si = ro.s_in + (size_t)bh * dc * dz;
-#pragma unroll
-            for (int t = 0; t < DC / 16; ++t)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = 32 * (t / 2) + 8 * lg + 4 * (t % 2) + i, z = zcol0 + 16 * n + lr;
-                        if (c < dc && z < dz) S[t][n][i] = si[c * ro.in_c + z * ro.in_z];
-                    }
-        }
+        if (ro.s_in) ps.load_state(ro.s_in + (size_t)bh * dc * dz, dc, dz, ro.in_c, ro.in_z, z0, lr, lg);
     } else if (!STATE_ONLY) {
-        const f32x4 *si = reinterpret_cast<const f32x4 *>(a.states + slot - DC * DZ) + (wave * (DC / 16) * NT) * 64 + lane;
 #pragma unroll
-        for (int t = 0; t < DC / 16; ++t)
+        for (int t = 0; t < P::KT; ++t)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) S[t][n] = si[(t * NT + n) * 64];
+            for (int n = 0; n < P::NT; ++n) ps.S[t][n] = states[(t * P::NT + n) * 64];
     }
 
-    // ---- rows in flight
-    Row8<T> rx[STATE_ONLY ? 1 : UC], ry[UC], rz[UZ];
-    float gnext = 0.0f;
-    auto fetch = [&](int s0) {
-#pragma unroll
-        for (int u = 0; u < UC; ++u) {
-            const int e = tid + u * NTHR, r = e / (DC / 8), c = (e % (DC / 8)) * 8, s = s0 + r;
-            const bool ok = e < C * DC / 8 && s < len;
-            const long long t = ro.reverse ? len - 1 - s : s;
-            if (!STATE_ONLY) rx[u] = fetch8<T>(px + t * ro.X.st, ok ? c : 1 << 20, ro.X.d, ro.X.vec);
-            ry[u] = fetch8<T>(py + t * ro.Y.st, ok ? c : 1 << 20, ro.Y.d, ro.Y.vec);
-        }
-#pragma unroll
-        for (int u = 0; u < UZ; ++u) {
-            const int e = tid + u * NTHR, r = e / (DZ / 8), c = (e % (DZ / 8)) * 8, s = s0 + r;
-            const bool ok = e < C * DZ / 8 && s < len;
-            const long long t = ro.reverse ? len - 1 - s : s;
-            rz[u] = fetch8<T>(pz + t * ro.Z.st, ok ? c : 1 << 20, ro.Z.d, ro.Z.vec);
-        }
-        if (wave == 0) {
-            const int s = s0 + lane;
-            gnext = 0.0f;
-            if (lane < C && s < len) {
-                if (!ro.reverse) gnext = pg[(long long)s * a.gt];
-                else if (s > 0) gnext = pg[(long long)(len - s) * a.gt];
-            }
-        }
-    };
-    auto flush_dots = [&](int s0) {
-        if (tid < C && s0 + tid < len) {
-            float d = 0.0f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) d += sm.dot[w][tid];
-            const int s = s0 + tid;
-            ro.dots[(size_t)bh * a.T + (ro.reverse ? len - 1 - s : s)] = d;
-        }
-    };
+    Tile<T, DC, C, NTHR, VEC> tx, ty;
+    Tile<T, DZ, C, NTHR, VEC> tz;
+    if (!STATE_ONLY) tx.init(ro.X, b, h, tid, ro.reverse);
+    ty.init(ro.Y, b, h, tid, ro.reverse);
+    tz.init(ro.Z, b, h, tid, ro.reverse);
+    float g = 0.0f;
     double gsum = 0.0;
-    if (n_live > 0) fetch(first);
-
-    for (int ci = 0; ci < n_live; ++ci) {
-        const int s0 = first + ci * C;
+    const auto fetch = [&](int ci) {
+        const int t0 = token0(ci), n = len - t0;
+        if (!STATE_ONLY) tx.fetch(t0, n);
+        ty.fetch(t0, n);
+        tz.fetch(t0, n);
+    };
+    const auto fetch_g = [&](int ci) {
+        const int t0 = token0(ci);
+        const int t = ro.reverse ? t0 + C - lane : t0 + lane;      // backwards a step decays by the token after it
+        g = lane < C && t < len ? pg[(long long)t * a.gt] : 0.0f;
+    };
+    const auto flush_dots = [&](int ci) {
+        const int t = token0(ci) + tid;
+        if (tid < C && t < len) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) s += sm.dots[w][tid];
+            ro.dots[(size_t)bh * a.T + t] = s;
+        }
+    };
+    if (c0 < c1) {
+        fetch(c0);
+        if (wave == NW - 1) {
+            fetch_g(c0);
+            gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[c0 & 1]);
+        }
+    }
+    for (int ci = c0; ci < c1; ++ci) {
+        const Decays<C> &d = sm.d[ci & 1];
         __syncthreads();                              // nobody reads the last chunk's tiles any more
-        if (!STATE_ONLY && ro.dots && ci > 0) flush_dots(s0 - C);
-#pragma unroll
-        for (int u = 0; u < UC; ++u) {
-            const int e = tid + u * NTHR, r = e / (DC / 8), c = (e % (DC / 8)) * 8;
-            if (e < C * DC / 8) {
-                b16x8 p[NP];
-                if (!STATE_ONLY) {
-                    split8<T>(rx[u], p);
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) *reinterpret_cast<b16x8 *>(&sm.X[k][r][c]) = p[k];
-                }
-                split8<T>(ry[u], p);
-#pragma unroll
-                for (int k = 0; k < NP; ++k) *reinterpret_cast<b16x8 *>(&sm.Y[k][r][c]) = p[k];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < UZ; ++u) {
-            const int e = tid + u * NTHR, r = e / (DZ / 8), c = (e % (DZ / 8)) * 8;
-            if (e < C * DZ / 8) {
-                b16x8 p[NP];
-                split8<T>(rz[u], p);
-#pragma unroll
-                for (int k = 0; k < NP; ++k) *reinterpret_cast<b16x8 *>(&sm.Z[k][r][c]) = p[k];
-            }
-        }
-        if (wave == 0) {
-            double G = log2_decay(gnext);
-#pragma unroll
-            for (int o = 1; o < C; o <<= 1) {
-                const double up = __shfl_up(G, o);
-                if (lane >= o) G += up;
-            }
-            const double tot = __shfl(G, C - 1);
-            if (lane < C) {
-                const float hi = (float)G;
-                sm.Gh[lane] = hi;
-                sm.Gl[lane] = (float)(G - (double)hi);
-                sm.E[lane] = fast_exp2(hi);
-                sm.R[lane] = fast_exp2((float)(tot - G));
-                if (lane == 0) sm.tot = fast_exp2((float)tot);
-            }
-            gsum += tot;
-        }
+        if (!STATE_ONLY && ro.dots && ci > c0) flush_dots(ci - 1);
+        if (!STATE_ONLY) tx.store(sm.x, tid);
+        ty.store(sm.y, tid);
+        tz.store(sm.z, tid);
         __syncthreads();
-        if (ci + 1 < n_live) fetch(s0 + C);
-        const float tot = sm.tot;
-
-        f32x4 O[STATE_ONLY ? 1 : CT][NT];
+        if (ci + 1 < c1) {
+            fetch(ci + 1);
+            if (wave == NW - 1) fetch_g(ci + 1);
+        }
         if (!STATE_ONLY) {
-            // ---- P^T tiles: rows j = the lane's 4 registers, column i = the lane; the 16 x 16 tiles on and below the diagonal
-            // go round the waves, and so do the tiles right of a diagonal one that a 32-wide product reads: zeros
-            constexpr int NTILE = CT * (CT + 1) / 2;
-            for (int e = wave; e < NTILE + CT / 2; e += NW) {
-                if (e >= NTILE) {
-                    const int I = 2 * (e - NTILE);
-#pragma unroll
-                    for (int k = 0; k < NC; ++k) *reinterpret_cast<b16x4 *>(&sm.P[k][I * 16 + lr][(I + 1) * 16 + 4 * lg]) = (b16x4){};
-                    continue;
-                }
-                const int I = (e >= 1) + (e >= 3) + (e >= 6), J = e - I * (I + 1) / 2;
-                f32x4 p = {0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < DC / 32; ++s) {
-                    b16x8 x[NP], y[NP];
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) {
-                        x[k] = *reinterpret_cast<const b16x8 *>(&sm.X[k][I * 16 + lr][32 * s + 8 * lg]);
-                        y[k] = *reinterpret_cast<const b16x8 *>(&sm.Y[k][J * 16 + lr][32 * s + 8 * lg]);
-                    }
-                    p = mma<NP, NP>(y, x, p);
-                }
-                const int i = I * 16 + lr;
-                const float gh = sm.Gh[i], gl = sm.Gl[i];
-                b16x4 q[NC];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = J * 16 + 4 * lg + r;
-                    const float d = fast_exp2((gh - sm.Gh[j]) + (gl - sm.Gl[j]));
-                    __bf16 w[NC];
-                    split<NC>(j > i ? 0.0f : p[r] * ro.scale_p * d, w);
-#pragma unroll
-                    for (int k = 0; k < NC; ++k) q[k][r] = w[k];
-                }
-#pragma unroll
-                for (int k = 0; k < NC; ++k) *reinterpret_cast<b16x4 *>(&sm.P[k][i][J * 16 + 4 * lg]) = q[k];
-            }
-            // ---- O^T = S^T x^T, scaled by 2^{G_i}
-#pragma unroll
-            for (int I = 0; I < CT; ++I)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) O[I][n] = (f32x4){0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < DC / 32; ++s) {
-                b16x8 st[NT][NC];
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        __bf16 w[NC];
-                        split<NC>(S[2 * s + j / 4][n][j % 4], w);
-#pragma unroll
-                        for (int k = 0; k < NC; ++k) st[n][k][j] = w[k];
-                    }
-#pragma unroll
-                for (int I = 0; I < CT; ++I) {
-                    b16x8 x[NP];
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) x[k] = *reinterpret_cast<const b16x8 *>(&sm.X[k][I * 16 + lr][32 * s + 8 * lg]);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) O[I][n] = mma<NC, NP>(st[n], x, O[I][n]);
-                }
-            }
-#pragma unroll
-            for (int I = 0; I < CT; ++I) {
-                const float e = sm.E[I * 16 + lr] * ro.scale_x;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) O[I][n] *= e;
-            }
-            __syncthreads();                          // P is whole
+            ps.scores(sm.x, sm.y, sm.p, d, ro.scale_p, wave, lr, lg);
+            ps.from_state(sm.x, d, lr, lg);
+            __syncthreads();                          // the scores are whole
         }
-#pragma unroll
-        for (int t = 0; t < DC / 16; ++t)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) S[t][n] *= tot;
-
-        // ---- by 32 tokens: O^T += z^T P^T, S += y^T (2^{G_C - G_j} z_j)
-#pragma unroll
-        for (int s = 0; s < C / 32; ++s) {
-            b16x8 zs[NT][NC];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                b16x8 z[NP];
-#pragma unroll
-                for (int k = 0; k < NP; ++k)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const b16x4 q = read_tr(&sm.Z[k][32 * s + 8 * lg + 4 * u + lr / 4][zcol0 + 16 * n + 4 * (lr % 4)]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) z[k][4 * u + j] = q[j];
-                    }
-                if (!STATE_ONLY) {
-#pragma unroll
-                    for (int I = 2 * s; I < CT; ++I) {
-                        b16x8 p[NC];
-#pragma unroll
-                        for (int k = 0; k < NC; ++k) p[k] = *reinterpret_cast<const b16x8 *>(&sm.P[k][I * 16 + lr][32 * s + 8 * lg]);
-                        O[I][n] = mma<NP, NC>(z, p, O[I][n]);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float v = 0.0f;
-#pragma unroll
-                    for (int k = NP - 1; k >= 0; --k) v += (float)z[k][j];
-                    __bf16 w[NC];
-                    split<NC>(v * (sm.R[32 * s + 8 * lg + j] * ro.scale_z), w);
-#pragma unroll
-                    for (int k = 0; k < NC; ++k) zs[n][k][j] = w[k];
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < DC / 16; ++t) {
-                b16x8 y[NP];
-#pragma unroll
-                for (int k = 0; k < NP; ++k)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const b16x4 q = read_tr(&sm.Y[k][32 * s + 8 * lg + 4 * u + lr / 4][32 * (t / 2) + 8 * (lr % 4) + 4 * (t % 2)]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) y[k][4 * u + j] = q[j];
-                    }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) S[t][n] = mma<NP, NC>(y, zs[n], S[t][n]);
-            }
-        }
-
-        if (!STATE_ONLY) {
-            // ---- the chunk's rows of o
-#pragma unroll
-            for (int I = 0; I < CT; ++I) {
-                const int s = s0 + I * 16 + lr;
-                const bool ok = s < len;
-                const long long t = ro.reverse ? len - 1 - s : s;
-                float dot = 0.0f;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int c = zcol0 + 16 * n + 4 * lg;
-                    if (ok && ro.O.p) {
-                        const long long at = t * ro.O.st + b * ro.O.sb + h * ro.O.sh + c;
-                        if (ro.O.f32) {
-                            float *po = reinterpret_cast<float *>(ro.O.p) + at;
-                            if (ro.O.vec == 2 && c < dz) *reinterpret_cast<f32x4 *>(po) = O[I][n];
-                            else
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    if (c + r < dz) po[r] = O[I][n][r];
-                        } else {
-                            T *po = reinterpret_cast<T *>(ro.O.p) + at;
-                            struct alignas(4 * sizeof(T)) V { T v[4]; } w;
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) w.v[r] = (T)O[I][n][r];
-                            if (ro.O.vec >= (sizeof(T) == 4 ? 2 : 1)) {
-                                if (c < dz) *reinterpret_cast<V *>(po) = w;
-                            } else
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    if (c + r < dz) po[r] = w.v[r];
-                        }
-                    }
-                    if (ok && ro.dots) {
-                        const T *pw = reinterpret_cast<const T *>(ro.W.p) + t * ro.W.st + b * ro.W.sb + (h / ro.W.group) * ro.W.sh + c;
-                        if (ro.W.vec >= (sizeof(T) == 4 ? 2 : 1)) {
-                            if (c < dz) {
-                                struct alignas(4 * sizeof(T)) V { T v[4]; };
-                                const V w = *reinterpret_cast<const V *>(pw);
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) dot += (float)w.v[r] * O[I][n][r];
-                            }
-                        } else
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (c + r < dz) dot += (float)pw[r] * O[I][n][r];
-                    }
-                }
-                if (ro.dots) {
-                    dot += __shfl_xor(dot, 16);
-                    dot += __shfl_xor(dot, 32);
-                    if (lg == 0) sm.dot[wave][I * 16 + lr] = dot;
-                }
-            }
-        }
+        ps.from_chunk(sm.y, sm.z, sm.p, d, z0, lr, lg);
+        if (!STATE_ONLY) ps.store_rows(ro, token0(ci), len, b, h, z0, lr, lg, sm.dots[wave]);
+        if (wave == NW - 1 && ci + 1 < c1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[(ci + 1) & 1]);
     }
 
     if (STATE_ONLY) {
-        f32x4 *so = reinterpret_cast<f32x4 *>(a.states + slot) + (wave * (DC / 16) * NT) * 64 + lane;
 #pragma unroll
-        for (int t = 0; t < DC / 16; ++t)
+        for (int t = 0; t < P::KT; ++t)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) so[(t * NT + n) * 64] = S[t][n];
-        if (tid == 0) a.decays[(size_t)(ri * BH + bh) * a.nseg + seg] = fast_exp2((float)gsum);
+            for (int n = 0; n < P::NT; ++n) states[(t * P::NT + n) * 64] = ps.S[t][n];
+        if (tid == NTHR - 64) a.decays[(size_t)(ri * BH + bh) * a.nseg + seg] = fast_exp2((float)gsum);
         return;
     }
-    if (ro.dots && n_live > 0) {
+    if (ro.dots && c0 < c1) {
         __syncthreads();
-        flush_dots(first + (n_live - 1) * C);
+        flush_dots(c1 - 1);
     }
-    // ---- rows behind the sample's length: zeros
-    if (ro.O.p) {
-        const int r0 = max(first, len);
-        for (long long e = tid; e < (long long)(behind - r0) * dz; e += NTHR) {
-            const long long at = (r0 + e / dz) * ro.O.st + b * ro.O.sb + h * ro.O.sh + e % dz;
-            if (ro.O.f32) reinterpret_cast<float *>(ro.O.p)[at] = 0.0f;
-            else reinterpret_cast<T *>(ro.O.p)[at] = (T)0.0f;
+    zero_rows<T>(ro, len, c0 * C, min(a.T, (c0 + a.seg_chunks) * C), b, h, tid, NTHR);
+    if (ro.s_out && seg == a.nseg - 1)
+        ps.store_state(ro.s_out + (size_t)bh * dc * dz, dc, dz, ro.out_c, ro.out_z, z0, lr, lg,
+                       ro.last_decay && len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f);
+}
+
+// The two passes of the backward that run against time, dv and dk, in one workgroup: they read the same four tensors, each
+// into one tile, and walk the same decays.  Waves 0 .. do dv (x = k, y = q, z = dO), the others dk (x = v, y = dO, z = q).
+template <typename T, int DK, int DV, int VEC, bool FINE, bool STATE_ONLY>
+struct Pair {
+    static constexpr int C = chunk<T>(), NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
+    static constexpr int NW0 = DV / 16 < 4 ? DV / 16 : 4, NW1 = DK / 16 < 4 ? DK / 16 : 4, NTHR = 64 * (NW0 + NW1);
+    typedef Pass<T, DK, DV, C, NW0, NX, STATE_ONLY> P0;
+    typedef Pass<T, DV, DK, C, NW1, NX, STATE_ONLY> P1;
+    struct Shared {
+        alignas(16) __bf16 q[NP * C * P0::LC];
+        alignas(16) __bf16 k[STATE_ONLY ? 8 : NP * C * P0::LC];
+        alignas(16) __bf16 v[STATE_ONLY ? 8 : NP * C * P1::LC];
+        alignas(16) __bf16 o[NP * C * P1::LC];
+        alignas(16) __bf16 p[2][STATE_ONLY ? 8 : NC * C * P0::LP];
+        alignas(16) Decays<C> d[2];
+        float dots[NW1][C];
+    };
+
+    template <typename P, int GROUP, int NW>
+    static __device__ __forceinline__ void walk(const Args &a, Shared &sm, int group, int wave, int tid)
+    {
+        const int lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+        const int BH = a.B * a.H, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
+        if (STATE_ONLY && seg == a.nseg - 1) return;
+        const int gr = GROUP < 0 ? group : GROUP;
+        const Role &ro = a.role[gr], &r0 = a.role[0], &r1 = a.role[1];
+        const int b = bh / a.H, h = bh % a.H;
+        const int len = __builtin_amdgcn_readfirstlane(valid_length(a.lengths, a.lengths64, b, a.T));
+        const int live = (len + C - 1) / C, c0 = seg * a.seg_chunks, c1 = min(live, c0 + a.seg_chunks);
+        const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
+        const bool clock = gr == 1 && wave == NW - 1;        // the wave that keeps the decays
+        const float *pg = a.g + b * a.gb + h * a.gh;
+        const auto token0 = [&](int ci) { return (live - 1 - ci) * C; };
+        const __bf16 *x = gr ? sm.v : sm.k, *y = gr ? sm.o : sm.q, *z = gr ? sm.q : sm.o;
+        __bf16 *const p = sm.p[gr];
+
+        P ps;
+        ps.zero();
+        const size_t slot = ((size_t)(gr * BH + bh) * a.nseg + seg) * (DK * DV);
+        f32x4 *const states = reinterpret_cast<f32x4 *>(a.states + (STATE_ONLY ? slot : slot - DK * DV)) + wave * P::KT * P::NT * 64 + lane;
+        if (seg == 0) {
+            if (ro.s_in) ps.load_state(ro.s_in + (size_t)bh * dc * dz, dc, dz, ro.in_c, ro.in_z, z0, lr, lg);
+        } else if (!STATE_ONLY) {
+#pragma unroll
+            for (int t = 0; t < P::KT; ++t)
+#pragma unroll
+                for (int n = 0; n < P::NT; ++n) ps.S[t][n] = states[(t * P::NT + n) * 64];
         }
+        Tile<T, DK, C, NTHR, VEC> tq, tk;
+        Tile<T, DV, C, NTHR, VEC> tv, to;
+        tq.init(r0.Y, b, h, tid, 1);
+        to.init(r0.Z, b, h, tid, 1);
+        if (!STATE_ONLY) {
+            tk.init(r0.X, b, h, tid, 1);
+            tv.init(r1.X, b, h, tid, 1);
+        }
+        float g = 0.0f;
+        double gsum = 0.0;
+        const auto fetch = [&](int ci) {
+            const int t0 = token0(ci), n = len - t0;
+            tq.fetch(t0, n);
+            to.fetch(t0, n);
+            if (!STATE_ONLY) {
+                tk.fetch(t0, n);
+                tv.fetch(t0, n);
+            }
+        };
+        const auto fetch_g = [&](int ci) {
+            const int t = token0(ci) + C - lane;             // a step decays by the token after it
+            g = lane < C && t < len ? pg[(long long)t * a.gt] : 0.0f;
+        };
+        const auto flush_dots = [&](int ci) {
+            const int t = token0(ci) + tid;
+            if (tid < C && t < len) {
+                float s = 0.0f;
+#pragma unroll
+                for (int w = 0; w < NW1; ++w) s += sm.dots[w][tid];
+                r1.dots[(size_t)bh * a.T + t] = s;
+            }
+        };
+        if (c0 < c1) {
+            fetch(c0);
+            if (clock) {
+                fetch_g(c0);
+                gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[c0 & 1]);
+            }
+        }
+        for (int ci = c0; ci < c1; ++ci) {
+            const Decays<C> &d = sm.d[ci & 1];
+            __syncthreads();                              // nobody reads the last chunk's tiles any more
+            if (!STATE_ONLY && r1.dots && ci > c0) flush_dots(ci - 1);
+            tq.store(sm.q, tid);
+            to.store(sm.o, tid);
+            if (!STATE_ONLY) {
+                tk.store(sm.k, tid);
+                tv.store(sm.v, tid);
+            }
+            __syncthreads();
+            if (ci + 1 < c1) {
+                fetch(ci + 1);
+                if (clock) fetch_g(ci + 1);
+            }
+            if (!STATE_ONLY) {
+                ps.scores(x, y, p, d, ro.scale_p, wave, lr, lg);
+                ps.from_state(x, d, lr, lg);
+                __syncthreads();                          // the scores are whole
+            }
+            ps.from_chunk(y, z, p, d, z0, lr, lg);
+            if (!STATE_ONLY) ps.store_rows(ro, token0(ci), len, b, h, z0, lr, lg, sm.dots[gr ? wave : 0]);
+            if (clock && ci + 1 < c1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[(ci + 1) & 1]);
+        }
+        if (STATE_ONLY) {
+#pragma unroll
+            for (int t = 0; t < P::KT; ++t)
+#pragma unroll
+                for (int n = 0; n < P::NT; ++n) states[(t * P::NT + n) * 64] = ps.S[t][n];
+            if (clock && lane == 0) {
+                const float e = fast_exp2((float)gsum);
+                a.decays[(size_t)bh * a.nseg + seg] = e;
+                a.decays[(size_t)(BH + bh) * a.nseg + seg] = e;
+            }
+            return;
+        }
+        if (r1.dots && c0 < c1) {
+            __syncthreads();
+            flush_dots(c1 - 1);
+        }
+        const int first = c0 * C, behind = min(a.T, (c0 + a.seg_chunks) * C);
+        zero_rows<T>(r0, len, first, behind, b, h, tid, NTHR);
+        zero_rows<T>(r1, len, first, behind, b, h, tid, NTHR);
+        if (ro.s_out && seg == a.nseg - 1)
+            ps.store_state(ro.s_out + (size_t)bh * dc * dz, dc, dz, ro.out_c, ro.out_z, z0, lr, lg,
+                           ro.last_decay && len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f);
     }
-    if (ro.s_out && seg == a.nseg - 1) {
-        const float more = ro.last_decay && len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f;
-        float *so = ro.s_out + (size_t)bh * dc * dz;
-#pragma unroll
-        for (int t = 0; t < DC / 16; ++t)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = 32 * (t / 2) + 8 * lg + 4 * (t % 2) + i, z = zcol0 + 16 * n + lr;
-                    if (c < dc && z < dz) so[c * ro.out_c + z * ro.out_z] = S[t][n][i] * more;
-                }
+};
+
+template <typename T, int DK, int DV, int VEC, bool FINE, bool STATE_ONLY>
+__global__ void __launch_bounds__((Pair<T, DK, DV, VEC, FINE, STATE_ONLY>::NTHR)) pair_kernel(const Args a)
+{
+    typedef Pair<T, DK, DV, VEC, FINE, STATE_ONLY> K;
+    __shared__ typename K::Shared sm;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int group = wave >= K::NW0, w = group ? wave - K::NW0 : wave;
+    if constexpr (DK == DV) {
+        K::template walk<typename K::P0, -1, K::NW0>(a, sm, group, w, tid);
+    } else {
+        if (group == 0) K::template walk<typename K::P0, 0, K::NW0>(a, sm, 0, w, tid);
+        else K::template walk<typename K::P1, 1, K::NW1>(a, sm, 1, w, tid);
     }
 }
 
-template <typename T, int DC, int DZ, int NW>
-static int launch_one(const Args &a, bool state_only, hipStream_t stream)
+template <typename T, int DC, int DZ, int VEC>
+static int launch_one(const Args &a, int kind, hipStream_t stream)
 {
-    constexpr int C = Kind<T>::NP == 1 ? 64 : 32;     // chunk_tokens()
-    const unsigned grid = (unsigned)((size_t)a.B * a.H * a.nseg * a.nroles);
-    if (state_only) chunk_kernel<T, DC, DZ, C, NW, true><<<grid, 64 * NW, 0, stream>>>(a);
-    else chunk_kernel<T, DC, DZ, C, NW, false><<<grid, 64 * NW, 0, stream>>>(a);
+    const unsigned grid = (unsigned)((size_t)a.B * a.H * a.nseg * (kind & PAIR ? 1 : a.nroles));
+    const bool fine = Kind<T>::NC < 3 && (kind & FINE_PASS);
+    if (kind & PAIR) {
+        constexpr int n = Pair<T, DC, DZ, VEC, false, true>::NTHR;
+        if (kind & STATES) pair_kernel<T, DC, DZ, VEC, false, true><<<grid, n, 0, stream>>>(a);
+        else if (fine) pair_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3, false><<<grid, n, 0, stream>>>(a);
+        else pair_kernel<T, DC, DZ, VEC, false, false><<<grid, n, 0, stream>>>(a);
+    } else {
+        constexpr int n = 64 * waves<T, DZ>();
+        if (kind & STATES) chunk_kernel<T, DC, DZ, VEC, false, true><<<grid, n, 0, stream>>>(a);
+        else if (fine) chunk_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3, false><<<grid, n, 0, stream>>>(a);
+        else chunk_kernel<T, DC, DZ, VEC, false, false><<<grid, n, 0, stream>>>(a);
+    }
     return launch_status("linear_attention");
 }
 
-template <typename T>
-int launch_chunks(const Args &a, int DC, int DZ, bool state_only, hipStream_t stream)
+template <typename T, int VEC>
+static int launch_width(const Args &a, int DC, int DZ, int kind, hipStream_t stream)
 {
-    // Waves: one 16-column tile of the state each where three planes fill the registers and the LDS leaves room for one
-    // workgroup of 128 columns (fp32), two tiles elsewhere.
-    constexpr int W128 = Kind<T>::NP == 3 ? 8 : 4;
-    if (DC == 32) return launch_one<T, 32, 32, 2>(a, state_only, stream);
-    if (DC == 64 && DZ == 64) return launch_one<T, 64, 64, 4>(a, state_only, stream);
-    if (DC == 64) return launch_one<T, 64, 128, W128>(a, state_only, stream);
-    if (DZ == 64) return launch_one<T, 128, 64, 4>(a, state_only, stream);
-    return launch_one<T, 128, 128, W128>(a, state_only, stream);
+    if (DC == 32) return launch_one<T, 32, 32, VEC>(a, kind, stream);
+    if (DC == 64 && DZ == 64) return launch_one<T, 64, 64, VEC>(a, kind, stream);
+    if (DC == 64) return launch_one<T, 64, 128, VEC>(a, kind, stream);
+    if (DZ == 64) return launch_one<T, 128, 64, VEC>(a, kind, stream);
+    return launch_one<T, 128, 128, VEC>(a, kind, stream);
+}
+
+template <typename T>
+int launch_chunks(const Args &a, int DC, int DZ, int kind, hipStream_t stream)
+{
+    int vec = 2;                                     // of the tensors that go through tiles
+    for (int r = 0; r < a.nroles; ++r) {
+        const int y = a.role[r].Y.vec, z = a.role[r].Z.vec, x = kind & STATES ? 2 : a.role[r].X.vec;
+        vec = vec < x ? vec : x;
+        vec = vec < y ? vec : y;
+        vec = vec < z ? vec : z;
+    }
+    if (vec == 2) return launch_width<T, 2>(a, DC, DZ, kind, stream);
+    if (vec == 1) return launch_width<T, 1>(a, DC, DZ, kind, stream);
+    return launch_width<T, 0>(a, DC, DZ, kind, stream);
 }
 
 }  // namespace la

@@ -3,6 +3,6 @@
 
 namespace dmn {
 namespace la {
-template int launch_chunks<float>(const Args &, int, int, bool, hipStream_t);
+template int launch_chunks<float>(const Args &, int, int, int, hipStream_t);
 }
 }

@@ -441,7 +441,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     assert size(*ok) == 0
     assert int(lib.dmn_linear_attention_workspace_floats(ok[0], 1, *ok[1:])) > 0
     for at, value, word in ((0, 3, b"dtype"), (1, -1, b"bad sizes"), (2, -1, b"bad sizes"), (3, 0, b"bad sizes"), (4, 3, b"multiple"),
-                            (7, 0, b"widths"), (7, 129, b"widths"), (8, 200, b"widths"), (2, 1 << 22, b"2^22")):
+                            (7, 0, b"widths"), (7, 129, b"widths"), (8, 200, b"widths"), (2, 1 << 17, b"2^17")):
         bad = list(ok)
         bad[at] = value
         assert size(*bad) == -1 and word in lib.dmn_last_error(), (at, value)
