@@ -209,6 +209,14 @@ __device__ __forceinline__ double lane_value(double v, int lane)
     return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 
+// the log decay of a lane's step: of its token, or backwards of the token after it
+template <int C>
+__device__ __forceinline__ float fetch_decay(const float *pg, long long gt, int t0, int len, int reverse, int lane)
+{
+    const int t = reverse ? t0 + C - lane : t0 + lane;
+    return lane < C && t < len ? pg[(long long)t * gt] : 0.0f;
+}
+
 // one wave; returns G_C
 template <int C>
 __device__ __forceinline__ double decays(float g, int lane, float scale_x, float scale_z, Decays<C> &d)
@@ -251,6 +259,21 @@ struct Pass {
 #pragma unroll
             for (int n = 0; n < NT; ++n) S[t][n] = (f32x4){0, 0, 0, 0};
     }
+    // between kernels: in the order of the registers
+    __device__ __forceinline__ void save(f32x4 *p) const
+    {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) p[(t * NT + n) * 64] = S[t][n];
+    }
+    __device__ __forceinline__ void resume(const f32x4 *p)
+    {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) S[t][n] = p[(t * NT + n) * 64];
+    }
     // tile t, row r of S is row 16 t + r
     __device__ __forceinline__ void load_state(const float *p, int dc, int dz, int in_c, int in_z, int z0, int lr, int lg)
     {
@@ -277,24 +300,15 @@ struct Pass {
                 }
     }
 
-    // 2^{G_i - G_j} (x_i . y_j) scale_p for j <= i, into P[plane][i][j].  The 16 x 16 tiles on and below the diagonal go round the
-    // waves, and so do the tiles right of a diagonal one that a product 32 wide reads: zeros.  The tiles are computed
-    // transposed: a lane holds one row i and 4 adjacent j.  Off the diagonal the decay is 2^{G_i - G_e} 2^{G_e - G_j}, e the last
-    // token of j's 16, both factors at most 1: an exponential for 4 numbers in place of one for each.
-    __device__ __forceinline__ void scores(const __bf16 *x, const __bf16 *y, __bf16 *P, const Decays<C> &d, float scale_p, int wave, int lr, int lg)
+    // 2^{G_i - G_j} (x_i . y_j) scale_p for j <= i, into P[plane][i][j].  16 x 16 tiles, computed transposed: a lane holds one row
+    // i and 4 adjacent j.  A diagonal tile takes the exponential of every difference; below it the decay is
+    // 2^{G_i - G_e} 2^{G_e - G_j}, e the last token of j's 16, both factors at most 1: one exponential a lane.  The tiles right of
+    // a diagonal one that a product 32 wide reads are zeros.  The diagonal goes round the W waves from the first on, the rest
+    // from the last on.
+    template <int W>
+    static __device__ __forceinline__ void scores(const __bf16 *x, const __bf16 *y, __bf16 *P, const Decays<C> &d, float scale_p, int wave, int lr, int lg)
     {
-        constexpr int NTILE = CT * (CT + 1) / 2, ALL = NTILE + CT / 2;
-#pragma unroll
-        for (int k0 = 0; k0 < (ALL + NW - 1) / NW; ++k0) {
-            const int e = wave + k0 * NW;
-            if (e >= ALL) break;
-            if (e >= NTILE) {
-                const int I = 2 * (e - NTILE);
-#pragma unroll
-                for (int k = 0; k < NC; ++k) *reinterpret_cast<u32x2 *>(P + (k * C + I * 16 + lr) * LP + (I + 1) * 16 + 4 * lg) = (u32x2){0, 0};
-                continue;
-            }
-            const int I = (e >= 1) + (e >= 3) + (e >= 6), J = e - I * (I + 1) / 2;
+        const auto tile = [&](int I, int J) {
             f32x4 p = {0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < DC / 32; ++s) {
@@ -306,23 +320,39 @@ struct Pass {
                 }
                 p = mma<NP, NP>(yf, xf, p);
             }
-            const int i = I * 16 + lr, j0 = J * 16 + 4 * lg;
-            const float gh = d.Gh[i], gl = d.Gl[i];
-            if (I == J) {
-                const f32x4 jh = *reinterpret_cast<const f32x4 *>(&d.Gh[j0]), jl = *reinterpret_cast<const f32x4 *>(&d.Gl[j0]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) p[r] = j0 + r > i ? 0.0f : p[r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
-            } else {
-                const f32x4 f = *reinterpret_cast<const f32x4 *>(&d.F[j0]);
-                const float row = fast_exp2((gh - d.Gh[J * 16 + 15]) + (gl - d.Gl[J * 16 + 15])) * scale_p;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) p[r] *= row * f[r];
-            }
+            return p;
+        };
+        const auto keep = [&](int I, int J, const f32x4 &p) {
             unsigned a[NC], b[NC];
             split2<NC>(p[0], p[1], a);
             split2<NC>(p[2], p[3], b);
 #pragma unroll
-            for (int k = 0; k < NC; ++k) *reinterpret_cast<u32x2 *>(P + (k * C + i) * LP + j0) = (u32x2){a[k], b[k]};
+            for (int k = 0; k < NC; ++k) *reinterpret_cast<u32x2 *>(P + (k * C + I * 16 + lr) * LP + J * 16 + 4 * lg) = (u32x2){a[k], b[k]};
+        };
+        constexpr int OFF = CT * (CT - 1) / 2, ALL = OFF + CT / 2;
+#pragma unroll
+        for (int k0 = 0; k0 < (CT + W - 1) / W; ++k0) {
+            const int I = wave + k0 * W;
+            if (CT % W && I >= CT) break;
+            f32x4 p = tile(I, I);
+            const float gh = d.Gh[I * 16 + lr], gl = d.Gl[I * 16 + lr];
+            const f32x4 jh = *reinterpret_cast<const f32x4 *>(&d.Gh[I * 16 + 4 * lg]), jl = *reinterpret_cast<const f32x4 *>(&d.Gl[I * 16 + 4 * lg]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[r] = 4 * lg + r > lr ? 0.0f : p[r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
+            keep(I, I, p);
+        }
+#pragma unroll
+        for (int k0 = 0; k0 < (ALL + W - 1) / W; ++k0) {
+            const int e = W - 1 - wave + k0 * W;
+            if (ALL % W && e >= ALL) break;
+            const bool below = e < OFF;
+            const int I = below ? 1 + (e >= 1) + (e >= 3) : 2 * (e - OFF), J = below ? e - I * (I - 1) / 2 : I + 1;
+            f32x4 p = tile(I, J);
+            const f32x4 f = *reinterpret_cast<const f32x4 *>(&d.F[J * 16 + 4 * lg]);
+            const float row = fast_exp2((d.Gh[I * 16 + lr] - d.Gh[J * 16 + 15]) + (d.Gl[I * 16 + lr] - d.Gl[J * 16 + 15])) * scale_p;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[r] = below ? p[r] * (row * f[r]) : 0.0f;
+            keep(I, J, p);
         }
     }
 
@@ -513,10 +543,10 @@ struct Pass {
     }
 };
 
-// Waves of a pass: one 16-column tile of the state each where three planes fill the registers (fp32 with 128 columns), two
-// tiles elsewhere.
-template <typename T, int DZ> constexpr int waves() { return DZ / 16 < 4 ? DZ / 16 : (DZ == 128 && Kind<T>::NP == 3 ? 8 : 4); }
 template <typename T> constexpr int chunk() { return Kind<T>::NP == 1 ? 64 : 32; }       // chunk_tokens()
+// waves that own columns of the state, a 16-column tile each (two of them where 128 columns leave the registers for it)
+template <int DZ> constexpr int feeders() { return DZ == 32 ? 2 : 4; }
+template <typename T, int DZ> constexpr int owners() { return DZ / 16 < 4 ? DZ / 16 : (DZ == 128 ? 8 : 4); }
 
 // rows first .. behind - 1 of o that lie behind the sample's length: zeros
 template <typename T>
@@ -531,121 +561,175 @@ __device__ __forceinline__ void zero_rows(const Role &ro, int len, int first, in
     }
 }
 
-template <typename T, int DC, int DZ, int VEC, bool FINE, bool STATE_ONLY>
-__global__ void __launch_bounds__((64 * waves<T, DZ>())) chunk_kernel(const Args a)
+// What one workgroup of a pass works on.
+template <int C>
+struct Place {
+    int bh, seg, ri, b, h, len, live, c0, c1;
+
+    __device__ __forceinline__ Place(const Args &a, int passes)
+    {
+        const int BH = a.B * a.H, rest = blockIdx.x / BH;
+        bh = blockIdx.x % BH;
+        seg = rest % a.nseg;
+        ri = passes > 1 ? rest / a.nseg : 0;
+        b = bh / a.H;
+        h = bh % a.H;
+        len = __builtin_amdgcn_readfirstlane(valid_length(a.lengths, a.lengths64, b, a.T));
+        live = (len + C - 1) / C;                    // chunks with tokens; backwards the first one walked is the partial one
+        c0 = seg * a.seg_chunks;
+        c1 = min(live, c0 + a.seg_chunks);
+    }
+};
+
+// The states after each segment but the last, from s_in for the first and from zero for the others.
+template <typename T, int DC, int DZ, int VEC>
+__global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Args a)
 {
-    constexpr int C = chunk<T>(), NW = waves<T, DZ>(), NTHR = 64 * NW;
-    constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
-    typedef Pass<T, DC, DZ, C, NW, NX, STATE_ONLY> P;
+    constexpr int C = chunk<T>(), NW = owners<T, DZ>(), NTHR = 64 * NW, NP = Kind<T>::NP;
+    typedef Pass<T, DC, DZ, C, NW, 1, true> P;
     struct Shared {
-        alignas(16) __bf16 x[STATE_ONLY ? 8 : NP * C * P::LC];
         alignas(16) __bf16 y[NP * C * P::LC];
         alignas(16) __bf16 z[NP * C * P::LZ];
-        alignas(16) __bf16 p[STATE_ONLY ? 8 : NC * C * P::LP];
-        alignas(16) Decays<C> d[2];
-        float dots[NW][C];
+        Decays<C> d[2];
+    };
+    __shared__ Shared sm;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+    const Place<C> w(a, a.nroles);
+    if (w.seg == a.nseg - 1) return;
+    const Role &ro = a.role[w.ri];
+    const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT, BH = a.B * a.H;
+    const float *pg = a.g + w.b * a.gb + w.h * a.gh;
+    const auto token0 = [&](int ci) { return (ro.reverse ? w.live - 1 - ci : ci) * C; };
+    P ps;
+    ps.zero();
+    if (w.seg == 0 && ro.s_in) ps.load_state(ro.s_in + (size_t)w.bh * dc * dz, dc, dz, ro.in_c, ro.in_z, z0, lr, lg);
+    Tile<T, DC, C, NTHR, VEC> ty;
+    Tile<T, DZ, C, NTHR, VEC> tz;
+    ty.init(ro.Y, w.b, w.h, tid, ro.reverse);
+    tz.init(ro.Z, w.b, w.h, tid, ro.reverse);
+    float g = 0.0f;
+    double gsum = 0.0;
+    const auto fetch = [&](int ci) {
+        const int t0 = token0(ci);
+        ty.fetch(t0, w.len - t0);
+        tz.fetch(t0, w.len - t0);
+        if (wave == NW - 1) g = fetch_decay<C>(pg, a.gt, t0, w.len, ro.reverse, lane);
+    };
+    if (w.c0 < w.c1) fetch(w.c0);
+    for (int ci = w.c0; ci < w.c1; ++ci) {
+        if (wave == NW - 1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[ci & 1]);
+        __syncthreads();                              // nobody reads the last chunk's tiles any more
+        ty.store(sm.y, tid);
+        tz.store(sm.z, tid);
+        __syncthreads();
+        if (ci + 1 < w.c1) fetch(ci + 1);
+        ps.from_chunk(sm.y, sm.z, nullptr, sm.d[ci & 1], z0, lr, lg);
+    }
+    f32x4 *const states = reinterpret_cast<f32x4 *>(a.states + ((size_t)(w.ri * BH + w.bh) * a.nseg + w.seg) * (DC * DZ)) + wave * P::KT * P::NT * 64 + lane;
+    ps.save(states);
+    if (tid == NTHR - 64) a.decays[(size_t)(w.ri * BH + w.bh) * a.nseg + w.seg] = fast_exp2((float)gsum);
+}
+
+// One pass.  The first waves own the state's columns, the others feed them: they fetch and lay out the tiles, keep the
+// decays and compute the scores.  A chunk has two phases, a barrier behind each:
+//   1  feeders: z into its tile, scores of this chunk         owners: o from the state
+//   2  feeders: x, y of the next chunk, its decays            owners: o and the state from this chunk, rows of o out
+// so that y alone needs two tiles, and either side's waits are hidden behind the other.
+template <typename T, int DC, int DZ, int VEC, bool FINE>
+__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>()))) chunk_kernel(const Args a)
+{
+    constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<DZ>(), NTHR = 64 * (NO + NF);
+    constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
+    typedef Pass<T, DC, DZ, C, NO, NX, false> P;
+    struct Shared {
+        alignas(16) __bf16 x[NP * C * P::LC];
+        alignas(16) __bf16 y[2][NP * C * P::LC];
+        alignas(16) __bf16 z[NP * C * P::LZ];
+        alignas(16) __bf16 p[NC * C * P::LP];
+        Decays<C> d[2];
+        float dots[NO][C];
     };
     __shared__ Shared sm;
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-    const int BH = a.B * a.H;
-    const int bh = blockIdx.x % BH, rest = blockIdx.x / BH;
-    const int seg = rest % a.nseg, ri = rest / a.nseg;
-    if (STATE_ONLY && seg == a.nseg - 1) return;     // the last segment's state is nobody's first
-    const Role &ro = a.role[ri];
-    const int b = bh / a.H, h = bh % a.H;
-    const int len = __builtin_amdgcn_readfirstlane(valid_length(a.lengths, a.lengths64, b, a.T));
-    const int live = (len + C - 1) / C;              // chunks with tokens; backwards the first one is the partial one
-    const int c0 = seg * a.seg_chunks, c1 = min(live, c0 + a.seg_chunks);
-    const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
-    const float *pg = a.g + b * a.gb + h * a.gh;
-    const auto token0 = [&](int ci) { return (ro.reverse ? live - 1 - ci : ci) * C; };
+    const Place<C> w(a, a.nroles);
+    const Role &ro = a.role[w.ri];
+    const int c0 = w.c0, c1 = w.c1;
+    const float *pg = a.g + w.b * a.gb + w.h * a.gh;
+    const auto token0 = [&](int ci) { return (ro.reverse ? w.live - 1 - ci : ci) * C; };
 
-    P ps;
-    ps.zero();
-    const size_t slot = ((size_t)(ri * BH + bh) * a.nseg + seg) * (DC * DZ);
-    f32x4 *const states = reinterpret_cast<f32x4 *>(a.states + (STATE_ONLY ? slot : slot - DC * DZ)) + wave * P::KT * P::NT * 64 + lane;
-    if (seg == 0) {
-        if (ro.s_in) ps.load_state(ro.s_in + (size_t)bh * dc * dz, dc, dz, ro.in_c, ro.in_z, z0, lr, lg);
-    } else if (!STATE_ONLY) {
+    if (wave >= NO) {
+        const int fw = wave - NO, ft = tid - 64 * NO;
+        Tile<T, DC, C, 64 * NF, VEC> tx, ty;
+        Tile<T, DZ, C, 64 * NF, VEC> tz;
+        tx.init(ro.X, w.b, w.h, ft, ro.reverse);
+        ty.init(ro.Y, w.b, w.h, ft, ro.reverse);
+        tz.init(ro.Z, w.b, w.h, ft, ro.reverse);
+        float g = 0.0f;
+        const auto fetch_xy = [&](int ci) {
+            const int t0 = token0(ci);
+            tx.fetch(t0, w.len - t0);
+            ty.fetch(t0, w.len - t0);
+            if (fw == 0) g = fetch_decay<C>(pg, a.gt, t0, w.len, ro.reverse, lane);
+        };
+        const auto store_xy = [&](int ci) {
+            tx.store(sm.x, ft);
+            ty.store(sm.y[ci & 1], ft);
+            if (fw == 0) decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[ci & 1]);
+        };
+        const auto flush_dots = [&](int ci) {
+            const int t = token0(ci) + ft;
+            if (ft < C && t < w.len) {
+                float s = 0.0f;
 #pragma unroll
-        for (int t = 0; t < P::KT; ++t)
-#pragma unroll
-            for (int n = 0; n < P::NT; ++n) ps.S[t][n] = states[(t * P::NT + n) * 64];
-    }
-
-    Tile<T, DC, C, NTHR, VEC> tx, ty;
-    Tile<T, DZ, C, NTHR, VEC> tz;
-    if (!STATE_ONLY) tx.init(ro.X, b, h, tid, ro.reverse);
-    ty.init(ro.Y, b, h, tid, ro.reverse);
-    tz.init(ro.Z, b, h, tid, ro.reverse);
-    float g = 0.0f;
-    double gsum = 0.0;
-    const auto fetch = [&](int ci) {
-        const int t0 = token0(ci), n = len - t0;
-        if (!STATE_ONLY) tx.fetch(t0, n);
-        ty.fetch(t0, n);
-        tz.fetch(t0, n);
-    };
-    const auto fetch_g = [&](int ci) {
-        const int t0 = token0(ci);
-        const int t = ro.reverse ? t0 + C - lane : t0 + lane;      // backwards a step decays by the token after it
-        g = lane < C && t < len ? pg[(long long)t * a.gt] : 0.0f;
-    };
-    const auto flush_dots = [&](int ci) {
-        const int t = token0(ci) + tid;
-        if (tid < C && t < len) {
-            float s = 0.0f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) s += sm.dots[w][tid];
-            ro.dots[(size_t)bh * a.T + t] = s;
+                for (int i = 0; i < NO; ++i) s += sm.dots[i][ft];
+                ro.dots[(size_t)w.bh * a.T + t] = s;
+            }
+        };
+        if (c0 < c1) {
+            fetch_xy(c0);
+            tz.fetch(token0(c0), w.len - token0(c0));
+            store_xy(c0);
+            if (c0 + 1 < c1) fetch_xy(c0 + 1);
         }
-    };
-    if (c0 < c1) {
-        fetch(c0);
-        if (wave == NW - 1) {
-            fetch_g(c0);
-            gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[c0 & 1]);
-        }
-    }
-    for (int ci = c0; ci < c1; ++ci) {
-        const Decays<C> &d = sm.d[ci & 1];
-        __syncthreads();                              // nobody reads the last chunk's tiles any more
-        if (!STATE_ONLY && ro.dots && ci > c0) flush_dots(ci - 1);
-        if (!STATE_ONLY) tx.store(sm.x, tid);
-        ty.store(sm.y, tid);
-        tz.store(sm.z, tid);
         __syncthreads();
-        if (ci + 1 < c1) {
-            fetch(ci + 1);
-            if (wave == NW - 1) fetch_g(ci + 1);
+        for (int ci = c0; ci < c1; ++ci) {
+            tz.store(sm.z, ft);
+            if (ci + 1 < c1) tz.fetch(token0(ci + 1), w.len - token0(ci + 1));
+            if (ro.dots && ci > c0) flush_dots(ci - 1);
+            P::template scores<NF>(sm.x, sm.y[ci & 1], sm.p, sm.d[ci & 1], ro.scale_p, fw, lr, lg);
+            __syncthreads();
+            if (ci + 1 < c1) {
+                store_xy(ci + 1);
+                if (ci + 2 < c1) fetch_xy(ci + 2);
+            }
+            __syncthreads();
         }
-        if (!STATE_ONLY) {
-            ps.scores(sm.x, sm.y, sm.p, d, ro.scale_p, wave, lr, lg);
+        if (ro.dots && c0 < c1) flush_dots(c1 - 1);
+    } else {
+        const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
+        P ps;
+        ps.zero();
+        if (w.seg == 0) {
+            if (ro.s_in) ps.load_state(ro.s_in + (size_t)w.bh * dc * dz, dc, dz, ro.in_c, ro.in_z, z0, lr, lg);
+        } else {
+            ps.resume(reinterpret_cast<const f32x4 *>(a.states + ((size_t)(w.ri * a.B * a.H + w.bh) * a.nseg + w.seg - 1) * (DC * DZ)) +
+                      wave * P::KT * P::NT * 64 + lane);
+        }
+        __syncthreads();
+        for (int ci = c0; ci < c1; ++ci) {
+            const Decays<C> &d = sm.d[ci & 1];
             ps.from_state(sm.x, d, lr, lg);
-            __syncthreads();                          // the scores are whole
+            __syncthreads();
+            ps.from_chunk(sm.y[ci & 1], sm.z, sm.p, d, z0, lr, lg);
+            ps.store_rows(ro, token0(ci), w.len, w.b, w.h, z0, lr, lg, sm.dots[wave]);
+            __syncthreads();
         }
-        ps.from_chunk(sm.y, sm.z, sm.p, d, z0, lr, lg);
-        if (!STATE_ONLY) ps.store_rows(ro, token0(ci), len, b, h, z0, lr, lg, sm.dots[wave]);
-        if (wave == NW - 1 && ci + 1 < c1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[(ci + 1) & 1]);
+        if (ro.s_out && w.seg == a.nseg - 1)
+            ps.store_state(ro.s_out + (size_t)w.bh * dc * dz, dc, dz, ro.out_c, ro.out_z, z0, lr, lg,
+                           ro.last_decay && w.len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f);
     }
-
-    if (STATE_ONLY) {
-#pragma unroll
-        for (int t = 0; t < P::KT; ++t)
-#pragma unroll
-            for (int n = 0; n < P::NT; ++n) states[(t * P::NT + n) * 64] = ps.S[t][n];
-        if (tid == NTHR - 64) a.decays[(size_t)(ri * BH + bh) * a.nseg + seg] = fast_exp2((float)gsum);
-        return;
-    }
-    if (ro.dots && c0 < c1) {
-        __syncthreads();
-        flush_dots(c1 - 1);
-    }
-    zero_rows<T>(ro, len, c0 * C, min(a.T, (c0 + a.seg_chunks) * C), b, h, tid, NTHR);
-    if (ro.s_out && seg == a.nseg - 1)
-        ps.store_state(ro.s_out + (size_t)bh * dc * dz, dc, dz, ro.out_c, ro.out_z, z0, lr, lg,
-                       ro.last_decay && len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f);
+    zero_rows<T>(ro, w.len, c0 * C, min(a.T, (c0 + a.seg_chunks) * C), w.b, w.h, tid, NTHR);
 }
 
 // The two passes of the backward that run against time, dv and dk, in one workgroup: they read the same four tensors, each
@@ -670,13 +754,11 @@ struct Pair {
     static __device__ __forceinline__ void walk(const Args &a, Shared &sm, int group, int wave, int tid)
     {
         const int lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-        const int BH = a.B * a.H, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
+        const Place<C> w(a, 1);
+        const int BH = a.B * a.H, bh = w.bh, seg = w.seg, b = w.b, h = w.h, len = w.len, live = w.live, c0 = w.c0, c1 = w.c1;
         if (STATE_ONLY && seg == a.nseg - 1) return;
         const int gr = GROUP < 0 ? group : GROUP;
         const Role &ro = a.role[gr], &r0 = a.role[0], &r1 = a.role[1];
-        const int b = bh / a.H, h = bh % a.H;
-        const int len = __builtin_amdgcn_readfirstlane(valid_length(a.lengths, a.lengths64, b, a.T));
-        const int live = (len + C - 1) / C, c0 = seg * a.seg_chunks, c1 = min(live, c0 + a.seg_chunks);
         const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
         const bool clock = gr == 1 && wave == NW - 1;        // the wave that keeps the decays
         const float *pg = a.g + b * a.gb + h * a.gh;
@@ -691,10 +773,7 @@ struct Pair {
         if (seg == 0) {
             if (ro.s_in) ps.load_state(ro.s_in + (size_t)bh * dc * dz, dc, dz, ro.in_c, ro.in_z, z0, lr, lg);
         } else if (!STATE_ONLY) {
-#pragma unroll
-            for (int t = 0; t < P::KT; ++t)
-#pragma unroll
-                for (int n = 0; n < P::NT; ++n) ps.S[t][n] = states[(t * P::NT + n) * 64];
+            ps.resume(states);
         }
         Tile<T, DK, C, NTHR, VEC> tq, tk;
         Tile<T, DV, C, NTHR, VEC> tv, to;
@@ -715,16 +794,13 @@ struct Pair {
                 tv.fetch(t0, n);
             }
         };
-        const auto fetch_g = [&](int ci) {
-            const int t = token0(ci) + C - lane;             // a step decays by the token after it
-            g = lane < C && t < len ? pg[(long long)t * a.gt] : 0.0f;
-        };
+        const auto fetch_g = [&](int ci) { g = fetch_decay<C>(pg, a.gt, token0(ci), len, 1, lane); };
         const auto flush_dots = [&](int ci) {
             const int t = token0(ci) + tid;
             if (tid < C && t < len) {
                 float s = 0.0f;
 #pragma unroll
-                for (int w = 0; w < NW1; ++w) s += sm.dots[w][tid];
+                for (int i = 0; i < NW1; ++i) s += sm.dots[i][tid];
                 r1.dots[(size_t)bh * a.T + t] = s;
             }
         };
@@ -751,7 +827,7 @@ struct Pair {
                 if (clock) fetch_g(ci + 1);
             }
             if (!STATE_ONLY) {
-                ps.scores(x, y, p, d, ro.scale_p, wave, lr, lg);
+                P::template scores<NW>(x, y, p, d, ro.scale_p, wave, lr, lg);
                 ps.from_state(x, d, lr, lg);
                 __syncthreads();                          // the scores are whole
             }
@@ -760,10 +836,7 @@ struct Pair {
             if (clock && ci + 1 < c1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[(ci + 1) & 1]);
         }
         if (STATE_ONLY) {
-#pragma unroll
-            for (int t = 0; t < P::KT; ++t)
-#pragma unroll
-                for (int n = 0; n < P::NT; ++n) states[(t * P::NT + n) * 64] = ps.S[t][n];
+            ps.save(states);
             if (clock && lane == 0) {
                 const float e = fast_exp2((float)gsum);
                 a.decays[(size_t)bh * a.nseg + seg] = e;
@@ -810,10 +883,10 @@ static int launch_one(const Args &a, int kind, hipStream_t stream)
         else if (fine) pair_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3, false><<<grid, n, 0, stream>>>(a);
         else pair_kernel<T, DC, DZ, VEC, false, false><<<grid, n, 0, stream>>>(a);
     } else {
-        constexpr int n = 64 * waves<T, DZ>();
-        if (kind & STATES) chunk_kernel<T, DC, DZ, VEC, false, true><<<grid, n, 0, stream>>>(a);
-        else if (fine) chunk_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3, false><<<grid, n, 0, stream>>>(a);
-        else chunk_kernel<T, DC, DZ, VEC, false, false><<<grid, n, 0, stream>>>(a);
+        constexpr int n = 64 * (owners<T, DZ>() + feeders<DZ>());
+        if (kind & STATES) state_kernel<T, DC, DZ, VEC><<<grid, 64 * owners<T, DZ>(), 0, stream>>>(a);
+        else if (fine) chunk_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3><<<grid, n, 0, stream>>>(a);
+        else chunk_kernel<T, DC, DZ, VEC, false><<<grid, n, 0, stream>>>(a);
     }
     return launch_status("linear_attention");
 }
