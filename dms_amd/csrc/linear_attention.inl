@@ -14,11 +14,10 @@
 // fp32 ones.  Six bf16 products take 96 cycles where the fp32 instruction takes 256 for the same product.
 //
 // A workgroup takes one (sample, head, segment) and walks its chunks; a wave owns 16 * NT columns of z, and with them
-// that part of S, which stays in its accumulators from the first chunk to the last.  Each accumulator tile holds the
-// rows of S in an order that makes it, converted, the operand of the next chunk's x S without any exchange:
-// row r of tile t is row 32 (t/2) + 8 (r/4) + 4 (t%2) + r%4 of S.
-// x, y, z planes are staged in LDS (rows padded by 16 bytes: 16 rows at one column fall into 64 different banks),
-// the next chunk's rows are in flight meanwhile.  Transposed fragments come from the transposing LDS read.
+// that part of S, which stays in its accumulators from the first chunk to the last: converted, they are the operand of the
+// next chunk's x S without any exchange, because the order of a product's inner index is free.
+// x, y, z planes are staged in LDS, the next chunk's rows are in flight meanwhile.  Transposed fragments come from the
+// transposing LDS read.
 #pragma once
 #include "linear_attention.h"
 
@@ -100,17 +99,27 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *p)
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, 0xfffffff0u, 0x00027000);
 }
 
+// Element (row, col) of an LDS tile D elements wide: rows are not padded, their 16-byte pieces are permuted by the row instead.
+// With the 64 banks that a read spans, 16 rows at one column and 4 adjacent rows of 16 columns (the transposing read) both
+// meet every bank once; rows padded by 16 bytes cost every one of these reads a second turn.
+template <int D>
+__device__ __forceinline__ int at(int row, int col)
+{
+    const int f = D == 32 ? 2 * ((row >> 2) & 1) : (D == 64 ? row & 7 : 2 * (row & 7));
+    return row * D + ((((col >> 3) ^ f) << 3) | (col & 7));
+}
+
 // A tile of C tokens x D elements of one tensor, on its way from memory to LDS: 16 bytes a thread and unit.
 // VEC: the pieces that every row's start and width allow (2: 16 bytes, 1: 8 bytes, 0: single elements).
 template <typename T, int D, int C, int NTHR, int VEC>
 struct Tile {
-    static constexpr int UE = 16 / (int)sizeof(T), PER = D / UE, N = C * PER, U = (N + NTHR - 1) / NTHR, LD = D + 8;
+    static constexpr int UE = 16 / (int)sizeof(T), PER = D / UE, N = C * PER, U = (N + NTHR - 1) / NTHR;
     static constexpr int NP = Kind<T>::NP;
     u32x4 raw[U];
     const char *p;             // token 0 of the sample and head
     long long st;              // bytes from token to token
     unsigned off, step;
-    int row, dcol, lds, lds_step;
+    int row, dcol, lds, lds_step;      // lds: of unit 0; the others lie whole multiples of 8 rows from it, so in the same permutation
 
     // backwards: token t0 + r goes into row C - 1 - r
     __device__ __forceinline__ void init(const Tensor &x, int b, int h, int tid, int reverse)
@@ -122,8 +131,9 @@ struct Tile {
         off = (unsigned)row * (unsigned)st + (unsigned)(c * (int)sizeof(T));
         step = (unsigned)(NTHR / PER) * (unsigned)st;
         dcol = x.d - c;
-        lds = (reverse ? C - 1 - row : row) * LD + c;
-        lds_step = (reverse ? -1 : 1) * (NTHR / PER) * LD;
+        static_assert((NTHR / PER) % 8 == 0, "units have to keep the row's permutation");
+        lds = at<D>(reverse ? C - 1 - row : row, c);
+        lds_step = (reverse ? -1 : 1) * (NTHR / PER) * D;
         if (dcol <= 0 || row >= C) row = 1 << 20;
     }
     // tokens t0 .. t0 + n - 1, zeros behind them
@@ -153,7 +163,7 @@ struct Tile {
             }
         }
     }
-    // into LDS planes of C rows of LD elements; the last thread's units may lie behind the tile
+    // into LDS planes of C rows of D elements; the last thread's units may lie behind the tile
     __device__ __forceinline__ void store(__bf16 *tile, int tid) const
     {
 #pragma unroll
@@ -166,7 +176,7 @@ struct Tile {
                 split2<NP>(x[0], x[1], a);
                 split2<NP>(x[2], x[3], b);
 #pragma unroll
-                for (int k = 0; k < NP; ++k) *reinterpret_cast<u32x2 *>(q + k * C * LD) = (u32x2){a[k], b[k]};
+                for (int k = 0; k < NP; ++k) *reinterpret_cast<u32x2 *>(q + k * C * D) = (u32x2){a[k], b[k]};
             } else if constexpr (NP == 1) {
                 *reinterpret_cast<u32x4 *>(q) = raw[u];
             } else {
@@ -178,7 +188,7 @@ struct Tile {
                 b16x8 w[NP];
                 dmn::la::split8<NP>(x, w);
 #pragma unroll
-                for (int k = 0; k < NP; ++k) *reinterpret_cast<b16x8 *>(q + k * C * LD) = w[k];
+                for (int k = 0; k < NP; ++k) *reinterpret_cast<b16x8 *>(q + k * C * D) = w[k];
             }
         }
     }
@@ -248,7 +258,6 @@ template <typename T, int DC, int DZ, int C, int NW, int NX, bool STATE_ONLY>
 struct Pass {
     static constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC;
     static constexpr int NT = DZ / 16 / NW, CT = C / 16, KT = DC / 16;     // tiles of 16: a wave's columns, tokens, rows of S
-    static constexpr int LC = DC + 8, LZ = DZ + 8, LP = C + 8;
     f32x4 S[KT][NT];
     f32x4 O[STATE_ONLY ? 1 : CT][NT];
 
@@ -303,56 +312,80 @@ struct Pass {
     // 2^{G_i - G_j} (x_i . y_j) scale_p for j <= i, into P[plane][i][j].  16 x 16 tiles, computed transposed: a lane holds one row
     // i and 4 adjacent j.  A diagonal tile takes the exponential of every difference; below it the decay is
     // 2^{G_i - G_e} 2^{G_e - G_j}, e the last token of j's 16, both factors at most 1: one exponential a lane.  The tiles right of
-    // a diagonal one that a product 32 wide reads are zeros.  The diagonal goes round the W waves from the first on, the rest
-    // from the last on.
+    // a diagonal one that a product 32 wide reads are zeros.
+    // Token 32 s + 16 u + 4 g + r of a row of P lies in column 32 s + 8 g + 4 u + r: in the order of the transposing reads of z.
+    static __device__ __forceinline__ void keep(__bf16 *P, int I, int J, const f32x4 &p, int lr, int lg)
+    {
+        unsigned a[NC], b[NC];
+        split2<NC>(p[0], p[1], a);
+        split2<NC>(p[2], p[3], b);
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+            *reinterpret_cast<u32x2 *>(P + k * C * C + at<C>(I * 16 + lr, 32 * (J / 2) + 8 * lg + 4 * (J % 2))) = (u32x2){a[k], b[k]};
+    }
+    // the tiles J0 .. J1 of rows I; J1 > I stands for the zeros
+    template <int I, int J0, int J1>
+    static __device__ __forceinline__ void row_tiles(const __bf16 *x, const __bf16 *y, __bf16 *P, const Decays<C> &d, float scale_p, int lr, int lg)
+    {
+        constexpr int JE = J1 < I ? J1 : I;
+        b16x8 xf[DC / 32][NP];
+        f32x4 p[JE - J0 + 1 > 0 ? JE - J0 + 1 : 1];
+#pragma unroll
+        for (int s = 0; s < DC / 32; ++s)
+#pragma unroll
+            for (int k = 0; k < NP; ++k) xf[s][k] = *reinterpret_cast<const b16x8 *>(x + k * C * DC + at<DC>(I * 16 + lr, 32 * s + 8 * lg));
+#pragma unroll
+        for (int J = J0; J <= JE; ++J) {
+            p[J - J0] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < DC / 32; ++s) {
+                b16x8 yf[NP];
+#pragma unroll
+                for (int k = 0; k < NP; ++k) yf[k] = *reinterpret_cast<const b16x8 *>(y + k * C * DC + at<DC>(J * 16 + lr, 32 * s + 8 * lg));
+                p[J - J0] = mma<NP, NP>(yf, xf[s], p[J - J0]);
+            }
+        }
+        const float gh = d.Gh[I * 16 + lr], gl = d.Gl[I * 16 + lr];
+#pragma unroll
+        for (int J = J0; J <= J1; ++J) {
+            f32x4 q = {0, 0, 0, 0};
+            if (J == I) {
+                const f32x4 jh = *reinterpret_cast<const f32x4 *>(&d.Gh[I * 16 + 4 * lg]), jl = *reinterpret_cast<const f32x4 *>(&d.Gl[I * 16 + 4 * lg]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) q[r] = 4 * lg + r > lr ? 0.0f : p[J - J0][r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
+            } else if (J < I) {
+                const f32x4 f = *reinterpret_cast<const f32x4 *>(&d.F[J * 16 + 4 * lg]);
+                const float row = fast_exp2((gh - d.Gh[J * 16 + 15]) + (gl - d.Gl[J * 16 + 15])) * scale_p;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) q[r] = p[J - J0][r] * (row * f[r]);
+            }
+            keep(P, I, J, q, lr, lg);
+        }
+    }
+    // dealt out to W waves
     template <int W>
     static __device__ __forceinline__ void scores(const __bf16 *x, const __bf16 *y, __bf16 *P, const Decays<C> &d, float scale_p, int wave, int lr, int lg)
     {
-        const auto tile = [&](int I, int J) {
-            f32x4 p = {0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < DC / 32; ++s) {
-                b16x8 xf[NP], yf[NP];
-#pragma unroll
-                for (int k = 0; k < NP; ++k) {
-                    xf[k] = *reinterpret_cast<const b16x8 *>(x + (k * C + I * 16 + lr) * LC + 32 * s + 8 * lg);
-                    yf[k] = *reinterpret_cast<const b16x8 *>(y + (k * C + J * 16 + lr) * LC + 32 * s + 8 * lg);
-                }
-                p = mma<NP, NP>(yf, xf, p);
+        if constexpr (CT == 4 && W == 4) {
+            if (wave == 0) row_tiles<0, 0, 1>(x, y, P, d, scale_p, lr, lg);
+            else if (wave == 1) row_tiles<1, 0, 1>(x, y, P, d, scale_p, lr, lg);
+            else if (wave == 2) row_tiles<2, 0, 3>(x, y, P, d, scale_p, lr, lg);
+            else row_tiles<3, 0, 3>(x, y, P, d, scale_p, lr, lg);
+        } else if constexpr (CT == 4) {
+            static_assert(W == 2, "2 or 4 waves");
+            if (wave == 0) {
+                row_tiles<0, 0, 1>(x, y, P, d, scale_p, lr, lg);
+                row_tiles<3, 0, 3>(x, y, P, d, scale_p, lr, lg);
+            } else {
+                row_tiles<1, 0, 1>(x, y, P, d, scale_p, lr, lg);
+                row_tiles<2, 0, 3>(x, y, P, d, scale_p, lr, lg);
             }
-            return p;
-        };
-        const auto keep = [&](int I, int J, const f32x4 &p) {
-            unsigned a[NC], b[NC];
-            split2<NC>(p[0], p[1], a);
-            split2<NC>(p[2], p[3], b);
-#pragma unroll
-            for (int k = 0; k < NC; ++k) *reinterpret_cast<u32x2 *>(P + (k * C + I * 16 + lr) * LP + J * 16 + 4 * lg) = (u32x2){a[k], b[k]};
-        };
-        constexpr int OFF = CT * (CT - 1) / 2, ALL = OFF + CT / 2;
-#pragma unroll
-        for (int k0 = 0; k0 < (CT + W - 1) / W; ++k0) {
-            const int I = wave + k0 * W;
-            if (CT % W && I >= CT) break;
-            f32x4 p = tile(I, I);
-            const float gh = d.Gh[I * 16 + lr], gl = d.Gl[I * 16 + lr];
-            const f32x4 jh = *reinterpret_cast<const f32x4 *>(&d.Gh[I * 16 + 4 * lg]), jl = *reinterpret_cast<const f32x4 *>(&d.Gl[I * 16 + 4 * lg]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) p[r] = 4 * lg + r > lr ? 0.0f : p[r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
-            keep(I, I, p);
-        }
-#pragma unroll
-        for (int k0 = 0; k0 < (ALL + W - 1) / W; ++k0) {
-            const int e = W - 1 - wave + k0 * W;
-            if (ALL % W && e >= ALL) break;
-            const bool below = e < OFF;
-            const int I = below ? 1 + (e >= 1) + (e >= 3) : 2 * (e - OFF), J = below ? e - I * (I - 1) / 2 : I + 1;
-            f32x4 p = tile(I, J);
-            const f32x4 f = *reinterpret_cast<const f32x4 *>(&d.F[J * 16 + 4 * lg]);
-            const float row = fast_exp2((d.Gh[I * 16 + lr] - d.Gh[J * 16 + 15]) + (d.Gl[I * 16 + lr] - d.Gl[J * 16 + 15])) * scale_p;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) p[r] = below ? p[r] * (row * f[r]) : 0.0f;
-            keep(I, J, p);
+        } else {
+            static_assert(CT == 2, "chunks of 32 or 64");
+            if (wave == 0) row_tiles<0, 0, 1>(x, y, P, d, scale_p, lr, lg);
+            else if (wave == 1 && W == 2) row_tiles<1, 0, 1>(x, y, P, d, scale_p, lr, lg);
+            else if (wave == 1) row_tiles<1, 0, 0>(x, y, P, d, scale_p, lr, lg);
+            else if (wave == 2) row_tiles<1, 1, 1>(x, y, P, d, scale_p, lr, lg);
         }
     }
 
@@ -379,8 +412,9 @@ struct Pass {
                 b16x8 xf[NP];
 #pragma unroll
                 for (int k = 0; k < NP; ++k) {
-                    const __bf16 *q = x + (k * C + I * 16 + lr) * LC + 32 * s + 4 * lg;
-                    xf[k] = join(*reinterpret_cast<const b16x4 *>(q), *reinterpret_cast<const b16x4 *>(q + 16));
+                    const __bf16 *q = x + k * C * DC;
+                    xf[k] = join(*reinterpret_cast<const b16x4 *>(q + at<DC>(I * 16 + lr, 32 * s + 4 * lg)),
+                                 *reinterpret_cast<const b16x4 *>(q + at<DC>(I * 16 + lr, 32 * s + 16 + 4 * lg)));
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) O[I][n] = mma<NX, NP>(st[n], xf, O[I][n]);
@@ -405,15 +439,15 @@ struct Pass {
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
             b16x8 zs[NT][NS];
-            const int row = 32 * s + 8 * lg;
-            const f32x4 r0 = *reinterpret_cast<const f32x4 *>(&d.R[row]), r1 = *reinterpret_cast<const f32x4 *>(&d.R[row + 4]);
+            const int row = 32 * s + 4 * lg;           // slots 4u + i of lane group g are token 32 s + 16 u + 4 g + i
+            const f32x4 r0 = *reinterpret_cast<const f32x4 *>(&d.R[row]), r1 = *reinterpret_cast<const f32x4 *>(&d.R[row + 16]);
             b16x8 zf[NT][NP];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int k = 0; k < NP; ++k) {
-                    const __bf16 *q = z + (k * C + row + lr / 4) * LZ + z0 + 16 * n + 4 * (lr % 4);
-                    zf[n][k] = join(read_tr(q), read_tr(q + 4 * LZ));
+                    const __bf16 *q = z + k * C * DZ + at<DZ>(row + lr / 4, z0 + 16 * n + 4 * (lr % 4));
+                    zf[n][k] = join(read_tr(q), read_tr(q + 16 * DZ));
                 }
             }
             if (!STATE_ONLY) {
@@ -421,7 +455,7 @@ struct Pass {
                 for (int I = 2 * s; I < CT; ++I) {
                     b16x8 pf[NC];
 #pragma unroll
-                    for (int k = 0; k < NC; ++k) pf[k] = *reinterpret_cast<const b16x8 *>(P + (k * C + I * 16 + lr) * LP + row);
+                    for (int k = 0; k < NC; ++k) pf[k] = *reinterpret_cast<const b16x8 *>(P + k * C * C + at<C>(I * 16 + lr, 32 * s + 8 * lg));
 #pragma unroll
                     for (int n = 0; n < NT; ++n) O[I][n] = mma<NP, NC>(zf[n], pf, O[I][n]);
                 }
@@ -443,8 +477,8 @@ struct Pass {
                 b16x8 yf[NP];
 #pragma unroll
                 for (int k = 0; k < NP; ++k) {
-                    const __bf16 *q = y + (k * C + row + lr / 4) * LC + 16 * t + 4 * (lr % 4);
-                    yf[k] = join(read_tr(q), read_tr(q + 4 * LC));
+                    const __bf16 *q = y + k * C * DC + at<DC>(row + lr / 4, 16 * t + 4 * (lr % 4));
+                    yf[k] = join(read_tr(q), read_tr(q + 16 * DC));
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) S[t][n] = mma<NP, NS>(yf, zs[n], S[t][n]);
@@ -588,8 +622,8 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
     constexpr int C = chunk<T>(), NW = owners<T, DZ>(), NTHR = 64 * NW, NP = Kind<T>::NP;
     typedef Pass<T, DC, DZ, C, NW, 1, true> P;
     struct Shared {
-        alignas(16) __bf16 y[NP * C * P::LC];
-        alignas(16) __bf16 z[NP * C * P::LZ];
+        alignas(16) __bf16 y[NP * C * DC];
+        alignas(16) __bf16 z[NP * C * DZ];
         Decays<C> d[2];
     };
     __shared__ Shared sm;
@@ -642,10 +676,10 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>()))) chun
     constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
     typedef Pass<T, DC, DZ, C, NO, NX, false> P;
     struct Shared {
-        alignas(16) __bf16 x[NP * C * P::LC];
-        alignas(16) __bf16 y[2][NP * C * P::LC];
-        alignas(16) __bf16 z[NP * C * P::LZ];
-        alignas(16) __bf16 p[NC * C * P::LP];
+        alignas(16) __bf16 x[NP * C * DC];
+        alignas(16) __bf16 y[2][NP * C * DC];
+        alignas(16) __bf16 z[NP * C * DZ];
+        alignas(16) __bf16 p[NC * C * C];
         Decays<C> d[2];
         float dots[NO][C];
     };
@@ -741,11 +775,11 @@ struct Pair {
     typedef Pass<T, DK, DV, C, NW0, NX, STATE_ONLY> P0;
     typedef Pass<T, DV, DK, C, NW1, NX, STATE_ONLY> P1;
     struct Shared {
-        alignas(16) __bf16 q[NP * C * P0::LC];
-        alignas(16) __bf16 k[STATE_ONLY ? 8 : NP * C * P0::LC];
-        alignas(16) __bf16 v[STATE_ONLY ? 8 : NP * C * P1::LC];
-        alignas(16) __bf16 o[NP * C * P1::LC];
-        alignas(16) __bf16 p[2][STATE_ONLY ? 8 : NC * C * P0::LP];
+        alignas(16) __bf16 q[NP * C * DK];
+        alignas(16) __bf16 k[STATE_ONLY ? 8 : NP * C * DK];
+        alignas(16) __bf16 v[STATE_ONLY ? 8 : NP * C * DV];
+        alignas(16) __bf16 o[NP * C * DV];
+        alignas(16) __bf16 p[2][STATE_ONLY ? 8 : NC * C * C];
         alignas(16) Decays<C> d[2];
         float dots[NW1][C];
     };
