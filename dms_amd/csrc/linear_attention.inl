@@ -92,6 +92,17 @@ __device__ __forceinline__ b16x4 read_tr(const __bf16 *p)
 
 __device__ __forceinline__ b16x8 join(b16x4 a, b16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
+// A wave-uniform value, kept in scalar registers from here on (left to itself the compiler loads kernel arguments again for
+// every chunk, and waits for them).
+__device__ __forceinline__ int held(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float held(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); }
+__device__ __forceinline__ long long held(long long v)
+{
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return (long long)((unsigned long long)hi << 32 | lo);
+}
+template <typename P> __device__ __forceinline__ P *held(P *p) { return reinterpret_cast<P *>(held(reinterpret_cast<long long>(p))); }
+
 // Buffer accesses: an offset of NOWHERE reads zero and writes nothing, so rows and columns that do not exist cost no branch.
 constexpr unsigned NOWHERE = 0xffffffffu;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *p)
@@ -124,8 +135,8 @@ struct Tile {
     // backwards: token t0 + r goes into row C - 1 - r
     __device__ __forceinline__ void init(const Tensor &x, int b, int h, int tid, int reverse)
     {
-        p = x.p + ((long long)b * x.sb + (long long)(h / x.group) * x.sh) * (int)sizeof(T);
-        st = x.st * (int)sizeof(T);
+        p = held(x.p + ((long long)b * x.sb + (long long)(h / x.group) * x.sh) * (int)sizeof(T));
+        st = held(x.st * (long long)sizeof(T));
         const int c = (tid % PER) * UE;
         row = tid / PER;
         off = (unsigned)row * (unsigned)st + (unsigned)(c * (int)sizeof(T));
@@ -252,6 +263,87 @@ __device__ __forceinline__ double decays(float g, int lane, float scale_x, float
     }
     return tot;
 }
+
+// Four adjacent elements of a token's row, in and out: rows lr + 16 I of a chunk, columns c0 + 16 n on.
+template <typename T, int C, int VEC>
+struct Rows {
+    char *p;                   // token 0 of the sample and head, or null
+    long long st;              // bytes from token to token
+    unsigned off, row_step;
+    int row, row16, f32, es, cols;     // cols: columns from c0 to the end
+
+    __device__ __forceinline__ Rows(const Tensor &x, int b, int h, int reverse, int lr, int c0)
+    {
+        f32 = sizeof(T) == 4 ? 0 : held(x.f32);
+        es = sizeof(T) == 4 || f32 ? 4 : 2;
+        p = held(x.p ? x.p + ((long long)b * x.sb + (long long)(h / x.group) * x.sh) * es : nullptr);
+        st = held(x.st * es);
+        row = reverse ? C - 1 - lr : lr;
+        row16 = reverse ? -16 : 16;
+        off = (unsigned)row * (unsigned)st + (unsigned)(c0 * es);
+        row_step = (unsigned)row16 * (unsigned)st;
+        cols = x.d - c0;
+    }
+    // n: tokens of the chunk
+    __device__ __forceinline__ void store4(__amdgpu_buffer_rsrc_t rs, int n_rows, int I, int n, const f32x4 &x) const
+    {
+        const bool ok = row + I * row16 < n_rows;
+        const unsigned o = off + I * row_step + 16 * n * es;
+        const int left = cols - 16 * n;
+        if (sizeof(T) == 4 || f32) {
+            if (VEC == 2 || (VEC == 1 && sizeof(T) == 2)) {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rs, ok && 0 < left ? o : NOWHERE, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = x[i];                // by value: a bit cast of a vector's element names the vector
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rs, ok && i < left ? o + 4 * i : NOWHERE, 0, 0);
+                }
+            }
+        } else if constexpr (sizeof(T) == 2) {
+            typedef T tx4 __attribute__((ext_vector_type(4)));
+            typedef unsigned short hx4 __attribute__((ext_vector_type(4)));
+            const tx4 w = __builtin_convertvector(x, tx4);
+            if (VEC >= 1) {
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, w), rs, ok && 0 < left ? o : NOWHERE, 0, 0);
+            } else {
+                const hx4 e = __builtin_bit_cast(hx4, w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_buffer_store_b16(e[i], rs, ok && i < left ? o + 2 * i : NOWHERE, 0, 0);
+            }
+        }
+    }
+    __device__ __forceinline__ f32x4 load4(__amdgpu_buffer_rsrc_t rs, int n_rows, int I, int n) const
+    {
+        const bool ok = row + I * row16 < n_rows;
+        const unsigned o = off + I * row_step + 16 * n * es;
+        const int left = cols - 16 * n;
+        f32x4 x;
+        if constexpr (sizeof(T) == 4) {
+            if (VEC == 2) {
+                x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, ok && 0 < left ? o : NOWHERE, 0, 0));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, ok && i < left ? o + 4 * i : NOWHERE, 0, 0));
+            }
+        } else {
+            typedef T tx4 __attribute__((ext_vector_type(4)));
+            typedef unsigned short hx4 __attribute__((ext_vector_type(4)));
+            tx4 y;
+            if (VEC >= 1) {
+                y = __builtin_bit_cast(tx4, __builtin_amdgcn_raw_buffer_load_b64(rs, ok && 0 < left ? o : NOWHERE, 0, 0));
+            } else {
+                hx4 e;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, ok && i < left ? o + 2 * i : NOWHERE, 0, 0);
+                y = __builtin_bit_cast(tx4, e);
+            }
+            x = __builtin_convertvector(y, f32x4);
+        }
+        return x;
+    }
+};
 
 // The part of a chunk that one pass (one Role) does, by its NW waves; x, y, z are LDS tiles of NP planes.
 template <typename T, int DC, int DZ, int C, int NW, int NX, bool STATE_ONLY>
@@ -487,91 +579,30 @@ struct Pass {
     }
 
     // rows of o: row r is token t0 + r, or t0 + C - 1 - r where time runs backwards; valid ones lie before token `len`
-    __device__ __forceinline__ void store_rows(const Role &ro, long long t0, int len, int b, int h, int z0, int lr, int lg, float *dots)
+    template <int VEC>
+    __device__ __forceinline__ void store_rows(const Rows<T, C, VEC> &o, const Rows<T, C, VEC> &w, bool dot_wanted, int t0, int len, int lg, float *dots)
     {
-        const Tensor &o = ro.O;
         if (o.p) {
-            const int es = o.f32 ? 4 : (int)sizeof(T);
-            const __amdgpu_buffer_rsrc_t rs = buffer(o.p + (t0 * o.st + (long long)b * o.sb + (long long)h * o.sh) * es);
-            const unsigned st = (unsigned)o.st * es;
+            const __amdgpu_buffer_rsrc_t rs = buffer(o.p + (long long)t0 * o.st);
 #pragma unroll
-            for (int I = 0; I < CT; ++I) {
-                const int r = I * 16 + lr, at = ro.reverse ? C - 1 - r : r;
-                const bool ok = t0 + at < len;
+            for (int I = 0; I < CT; ++I)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int c = z0 + 16 * n + 4 * lg;
-                    const unsigned off = (unsigned)at * st + (unsigned)(c * es);
-                    if (sizeof(T) == 4 || o.f32) {
-                        if (o.vec == 2) {
-                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O[I][n]), rs, ok && c < o.d ? off : NOWHERE, 0, 0);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float v = O[I][n][i];          // by value: a bit cast of a vector's element names the vector
-                                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rs, ok && c + i < o.d ? off + 4 * i : NOWHERE,
-                                                                      0, 0);
-                            }
-                        }
-                    } else if constexpr (sizeof(T) == 2) {
-                        typedef T tx4 __attribute__((ext_vector_type(4)));
-                        typedef unsigned short hx4 __attribute__((ext_vector_type(4)));
-                        const tx4 w = __builtin_convertvector(O[I][n], tx4);
-                        if (o.vec >= 1) {
-                            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, w), rs, ok && c < o.d ? off : NOWHERE, 0, 0);
-                        } else {
-                            const hx4 e = __builtin_bit_cast(hx4, w);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                __builtin_amdgcn_raw_buffer_store_b16(e[i], rs, ok && c + i < o.d ? off + 2 * i : NOWHERE, 0, 0);
-                        }
-                    }
-                }
-            }
+                for (int n = 0; n < NT; ++n) o.store4(rs, len - t0, I, n, O[I][n]);
         }
-        if (ro.dots) {
-            const Tensor &w = ro.W;
-            const __amdgpu_buffer_rsrc_t rs =
-                buffer(w.p + (t0 * w.st + (long long)b * w.sb + (long long)(h / w.group) * w.sh) * (int)sizeof(T));
-            const unsigned st = (unsigned)w.st * (unsigned)sizeof(T);
+        if (dot_wanted) {
+            const __amdgpu_buffer_rsrc_t rs = buffer(w.p + (long long)t0 * w.st);
 #pragma unroll
             for (int I = 0; I < CT; ++I) {
-                const int r = I * 16 + lr, at = ro.reverse ? C - 1 - r : r;
-                const bool ok = t0 + at < len;
                 float dot = 0.0f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const int c = z0 + 16 * n + 4 * lg;
-                    const unsigned off = (unsigned)at * st + (unsigned)(c * (int)sizeof(T));
-                    f32x4 x;
-                    if constexpr (sizeof(T) == 4) {
-                        if (w.vec == 2) {
-                            x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, ok && c < w.d ? off : NOWHERE, 0, 0));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, ok && c + i < w.d ? off + 4 * i : NOWHERE, 0, 0));
-                        }
-                    } else {
-                        typedef T tx4 __attribute__((ext_vector_type(4)));
-                        typedef unsigned short hx4 __attribute__((ext_vector_type(4)));
-                        tx4 y;
-                        if (w.vec >= 1) {
-                            y = __builtin_bit_cast(tx4, __builtin_amdgcn_raw_buffer_load_b64(rs, ok && c < w.d ? off : NOWHERE, 0, 0));
-                        } else {
-                            hx4 e;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, ok && c + i < w.d ? off + 2 * i : NOWHERE, 0, 0);
-                            y = __builtin_bit_cast(tx4, e);
-                        }
-                        x = __builtin_convertvector(y, f32x4);
-                    }
+                    const f32x4 x = w.load4(rs, len - t0, I, n);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) dot += x[i] * O[I][n][i];
                 }
                 dot += __shfl_xor(dot, 16);
                 dot += __shfl_xor(dot, 32);
-                if (lg == 0) dots[at] = dot;
+                if (lg == 0) dots[w.row + I * w.row16] = dot;
             }
         }
     }
@@ -665,21 +696,28 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
 }
 
 // One pass.  The first waves own the state's columns, the others feed them: they fetch and lay out the tiles, keep the
-// decays and compute the scores.  A chunk has two phases, a barrier behind each:
-//   1  feeders: z into its tile, scores of this chunk         owners: o from the state
-//   2  feeders: x, y of the next chunk, its decays            owners: o and the state from this chunk, rows of o out
-// so that y alone needs two tiles, and either side's waits are hidden behind the other.
+// decays and compute the scores, a chunk ahead.  A chunk has two phases, a barrier behind each:
+//   1  feeders: x, y, decays of the next chunk, z of this one   owners: o from the state
+//   2  feeders: scores of the next chunk                        owners: o and the state from this chunk, rows of o out
+// so that z alone needs one tile and the owners never wait for the feeders' loads or exponentials.
+// Waves of a SIMD that the LDS leaves room for: two workgroups of 8 where the tiles take less than half of it.
+template <typename T, int DC, int DZ> constexpr int residents()
+{
+    const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * Kind<T>::NC * chunk<T>() * chunk<T>() * 2 + 6 * 1024;
+    return (owners<T, DZ>() + feeders<DZ>()) / 4 * (tiles <= 80 * 1024 ? 2 : 1);
+}
+
 template <typename T, int DC, int DZ, int VEC, bool FINE>
-__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>()))) chunk_kernel(const Args a)
+__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>())), (residents<T, DC, DZ>())) chunk_kernel(const Args a)
 {
     constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<DZ>(), NTHR = 64 * (NO + NF);
     constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
     typedef Pass<T, DC, DZ, C, NO, NX, false> P;
     struct Shared {
-        alignas(16) __bf16 x[NP * C * DC];
+        alignas(16) __bf16 x[2][NP * C * DC];
         alignas(16) __bf16 y[2][NP * C * DC];
         alignas(16) __bf16 z[NP * C * DZ];
-        alignas(16) __bf16 p[NC * C * C];
+        alignas(16) __bf16 p[2][NC * C * C];
         Decays<C> d[2];
         float dots[NO][C];
     };
@@ -688,60 +726,71 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>()))) chun
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
     const Place<C> w(a, a.nroles);
     const Role &ro = a.role[w.ri];
-    const int c0 = w.c0, c1 = w.c1;
-    const float *pg = a.g + w.b * a.gb + w.h * a.gh;
-    const auto token0 = [&](int ci) { return (ro.reverse ? w.live - 1 - ci : ci) * C; };
+    const int c0 = held(w.c0), c1 = held(w.c1), len = w.len, live = held(w.live), reverse = held(ro.reverse);
+    const float *pg = held(a.g + w.b * a.gb + w.h * a.gh);
+    float *const dots = held(ro.dots ? ro.dots + (size_t)w.bh * a.T : nullptr);
+    const auto token0 = [&](int ci) { return (reverse ? live - 1 - ci : ci) * C; };
 
     if (wave >= NO) {
         const int fw = wave - NO, ft = tid - 64 * NO;
         Tile<T, DC, C, 64 * NF, VEC> tx, ty;
         Tile<T, DZ, C, 64 * NF, VEC> tz;
-        tx.init(ro.X, w.b, w.h, ft, ro.reverse);
-        ty.init(ro.Y, w.b, w.h, ft, ro.reverse);
-        tz.init(ro.Z, w.b, w.h, ft, ro.reverse);
+        tx.init(ro.X, w.b, w.h, ft, reverse);
+        ty.init(ro.Y, w.b, w.h, ft, reverse);
+        tz.init(ro.Z, w.b, w.h, ft, reverse);
+        const long long gt = held(a.gt);
+        const float scale_p = held(ro.scale_p), scale_x = held(ro.scale_x), scale_z = held(ro.scale_z);
         float g = 0.0f;
         const auto fetch_xy = [&](int ci) {
             const int t0 = token0(ci);
-            tx.fetch(t0, w.len - t0);
-            ty.fetch(t0, w.len - t0);
-            if (fw == 0) g = fetch_decay<C>(pg, a.gt, t0, w.len, ro.reverse, lane);
+            tx.fetch(t0, len - t0);
+            ty.fetch(t0, len - t0);
+            if (fw == 0) g = fetch_decay<C>(pg, gt, t0, len, reverse, lane);
         };
         const auto store_xy = [&](int ci) {
-            tx.store(sm.x, ft);
+            tx.store(sm.x[ci & 1], ft);
             ty.store(sm.y[ci & 1], ft);
-            if (fw == 0) decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[ci & 1]);
+            if (fw == 0) decays<C>(g, lane, scale_x, scale_z, sm.d[ci & 1]);
+        };
+        const auto scores = [&](int ci) {
+            P::template scores<NF>(sm.x[ci & 1], sm.y[ci & 1], sm.p[ci & 1], sm.d[ci & 1], scale_p, fw, lr, lg);
         };
         const auto flush_dots = [&](int ci) {
             const int t = token0(ci) + ft;
-            if (ft < C && t < w.len) {
+            if (ft < C && t < len) {
                 float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NO; ++i) s += sm.dots[i][ft];
-                ro.dots[(size_t)w.bh * a.T + t] = s;
+                dots[t] = s;
             }
         };
         if (c0 < c1) {
             fetch_xy(c0);
-            tz.fetch(token0(c0), w.len - token0(c0));
+            tz.fetch(token0(c0), len - token0(c0));
             store_xy(c0);
             if (c0 + 1 < c1) fetch_xy(c0 + 1);
+            __syncthreads();
+            scores(c0);
+        } else {
+            __syncthreads();
         }
         __syncthreads();
         for (int ci = c0; ci < c1; ++ci) {
             tz.store(sm.z, ft);
-            if (ci + 1 < c1) tz.fetch(token0(ci + 1), w.len - token0(ci + 1));
-            if (ro.dots && ci > c0) flush_dots(ci - 1);
-            P::template scores<NF>(sm.x, sm.y[ci & 1], sm.p, sm.d[ci & 1], ro.scale_p, fw, lr, lg);
-            __syncthreads();
             if (ci + 1 < c1) {
+                tz.fetch(token0(ci + 1), len - token0(ci + 1));
                 store_xy(ci + 1);
                 if (ci + 2 < c1) fetch_xy(ci + 2);
             }
+            if (dots && ci > c0) flush_dots(ci - 1);
+            __syncthreads();
+            if (ci + 1 < c1) scores(ci + 1);
             __syncthreads();
         }
-        if (ro.dots && c0 < c1) flush_dots(c1 - 1);
+        if (dots && c0 < c1) flush_dots(c1 - 1);
     } else {
         const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
+        const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(ro.W, w.b, w.h, reverse, lr, z0 + 4 * lg);
         P ps;
         ps.zero();
         if (w.seg == 0) {
@@ -751,19 +800,20 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>()))) chun
                       wave * P::KT * P::NT * 64 + lane);
         }
         __syncthreads();
+        __syncthreads();
         for (int ci = c0; ci < c1; ++ci) {
             const Decays<C> &d = sm.d[ci & 1];
-            ps.from_state(sm.x, d, lr, lg);
+            ps.from_state(sm.x[ci & 1], d, lr, lg);
             __syncthreads();
-            ps.from_chunk(sm.y[ci & 1], sm.z, sm.p, d, z0, lr, lg);
-            ps.store_rows(ro, token0(ci), w.len, w.b, w.h, z0, lr, lg, sm.dots[wave]);
+            ps.from_chunk(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
+            ps.store_rows(out, wrows, dots != nullptr, token0(ci), len, lg, sm.dots[wave]);
             __syncthreads();
         }
         if (ro.s_out && w.seg == a.nseg - 1)
             ps.store_state(ro.s_out + (size_t)w.bh * dc * dz, dc, dz, ro.out_c, ro.out_z, z0, lr, lg,
-                           ro.last_decay && w.len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f);
+                           ro.last_decay && len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f);
     }
-    zero_rows<T>(ro, w.len, c0 * C, min(a.T, (c0 + a.seg_chunks) * C), w.b, w.h, tid, NTHR);
+    zero_rows<T>(ro, len, c0 * C, min(a.T, (c0 + a.seg_chunks) * C), w.b, w.h, tid, NTHR);
 }
 
 // The two passes of the backward that run against time, dv and dk, in one workgroup: they read the same four tensors, each
@@ -800,6 +850,7 @@ struct Pair {
         const __bf16 *x = gr ? sm.v : sm.k, *y = gr ? sm.o : sm.q, *z = gr ? sm.q : sm.o;
         __bf16 *const p = sm.p[gr];
 
+        const Rows<T, C, VEC> out(ro.O, b, h, 1, lr, z0 + 4 * lg), wrows(ro.W, b, h, 1, lr, z0 + 4 * lg);
         P ps;
         ps.zero();
         const size_t slot = ((size_t)(gr * BH + bh) * a.nseg + seg) * (DK * DV);
@@ -866,7 +917,7 @@ struct Pair {
                 __syncthreads();                          // the scores are whole
             }
             ps.from_chunk(y, z, p, d, z0, lr, lg);
-            if (!STATE_ONLY) ps.store_rows(ro, token0(ci), len, b, h, z0, lr, lg, sm.dots[gr ? wave : 0]);
+            if (!STATE_ONLY) ps.store_rows(out, wrows, gr && r1.dots, token0(ci), len, lg, sm.dots[gr ? wave : 0]);
             if (clock && ci + 1 < c1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[(ci + 1) & 1]);
         }
         if (STATE_ONLY) {
@@ -938,12 +989,15 @@ static int launch_width(const Args &a, int DC, int DZ, int kind, hipStream_t str
 template <typename T>
 int launch_chunks(const Args &a, int DC, int DZ, int kind, hipStream_t stream)
 {
-    int vec = 2;                                     // of the tensors that go through tiles
+    int vec = 2;                                     // of all rows that the kernel touches
+    const auto touch = [&vec](const Tensor &t) { vec = t.p && t.vec < vec ? t.vec : vec; };
     for (int r = 0; r < a.nroles; ++r) {
-        const int y = a.role[r].Y.vec, z = a.role[r].Z.vec, x = kind & STATES ? 2 : a.role[r].X.vec;
-        vec = vec < x ? vec : x;
-        vec = vec < y ? vec : y;
-        vec = vec < z ? vec : z;
+        touch(a.role[r].Y);
+        touch(a.role[r].Z);
+        if (kind & STATES) continue;
+        touch(a.role[r].X);
+        if (a.role[r].dots) touch(a.role[r].W);
+        touch(a.role[r].O);
     }
     if (vec == 2) return launch_width<T, 2>(a, DC, DZ, kind, stream);
     if (vec == 1) return launch_width<T, 1>(a, DC, DZ, kind, stream);
