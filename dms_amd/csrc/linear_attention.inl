@@ -69,18 +69,20 @@ __device__ __forceinline__ void split8(const float (&x)[8], b16x8 (&p)[N])
     for (int k = 0; k < N; ++k) p[k] = __builtin_bit_cast(b16x8, w[k]);
 }
 
-// acc += sum of a[i] b[j] over the pairs that reach the precision of the finer operand
-template <int NA, int NB>
-__device__ __forceinline__ f32x4 mma(const b16x8 (&a)[NA], const b16x8 (&b)[NB], f32x4 acc)
+// The products of planes a[i] b[j] that reach the precision of the finer operand, smallest first: f(i, j) does one of them, for
+// all tiles in turn (a matrix instruction that waits for the one before it costs as much as four that do not).
+template <int NA, int NB, typename F>
+__device__ __forceinline__ void plane_products(F f)
 {
     constexpr int M = NA > NB ? NA : NB;
 #pragma unroll
     for (int s = M - 1; s >= 0; --s)
 #pragma unroll
         for (int i = 0; i < NA; ++i)
-            if (s - i >= 0 && s - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], acc, 0, 0, 0);
-    return acc;
+            if (s - i >= 0 && s - i < NB) f(i, s - i);
 }
+
+__device__ __forceinline__ f32x4 mfma(const b16x8 &a, const b16x8 &b, const f32x4 &c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 // The transposing read: in a group of 16 lanes, lane 4j + c names 4 adjacent elements of row j; lane l receives
 // element l%4 of the lanes 4j + l/4, j = 0..3.
@@ -105,6 +107,7 @@ template <typename P> __device__ __forceinline__ P *held(P *p) { return reinterp
 
 // Buffer accesses: an offset of NOWHERE reads zero and writes nothing, so rows and columns that do not exist cost no branch.
 constexpr unsigned NOWHERE = 0xffffffffu;
+constexpr int STREAM = 2;                // non-temporal: whole lines that nobody here reads again do not sit dirty in the L2 at the kernel's end
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *p)
 {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, 0xfffffff0u, 0x00027000);
@@ -126,11 +129,11 @@ template <typename T, int D, int C, int NTHR, int VEC>
 struct Tile {
     static constexpr int UE = 16 / (int)sizeof(T), PER = D / UE, N = C * PER, U = (N + NTHR - 1) / NTHR;
     static constexpr int NP = Kind<T>::NP;
-    u32x4 raw[U];
+    struct Flight { u32x4 raw[U]; };
     const char *p;             // token 0 of the sample and head
     long long st;              // bytes from token to token
     unsigned off, step;
-    int row, dcol, lds, lds_step;      // lds: of unit 0; the others lie whole multiples of 8 rows from it, so in the same permutation
+    int row, dcol, ocol, lds, lds_step;      // ocol: columns of o from the thread's first to the end (drain); lds: of unit 0; the others lie whole multiples of 8 rows from it, so in the same permutation
 
     // backwards: token t0 + r goes into row C - 1 - r
     __device__ __forceinline__ void init(const Tensor &x, int b, int h, int tid, int reverse)
@@ -148,8 +151,9 @@ struct Tile {
         if (dcol <= 0 || row >= C) row = 1 << 20;
     }
     // tokens t0 .. t0 + n - 1, zeros behind them
-    __device__ __forceinline__ void fetch(long long t0, int n)
+    __device__ __forceinline__ void fetch(Flight &f, long long t0, int n) const
     {
+        u32x4 (&raw)[U] = f.raw;
         const __amdgpu_buffer_rsrc_t rs = buffer(p + t0 * st);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -174,9 +178,45 @@ struct Tile {
             }
         }
     }
-    // into LDS planes of C rows of D elements; the last thread's units may lie behind the tile
-    __device__ __forceinline__ void store(__bf16 *tile, int tid) const
+    // rows of o out of LDS, where they lie as a tile does: the 16 bytes that unit u would be stored from (of fp32: 8 in plane 0, 8 in
+    // plane 1).  A thread takes what its own next store() overwrites, so nobody has to wait in between.  `o` is o's row base.
+    __device__ __forceinline__ void drain(const __bf16 *tile, int tid, const char *o, long long o_st, int n) const
     {
+        const __amdgpu_buffer_rsrc_t rs = buffer(o);
+        const int row0 = tid / PER;
+        const unsigned first = (unsigned)row0 * (unsigned)o_st + (unsigned)((tid % PER) * 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (U * NTHR > N && tid + u * NTHR >= N) break;
+            const __bf16 *q = tile + lds + u * lds_step;
+            u32x4 w;
+            if constexpr (sizeof(T) == 4) {
+                const u32x2 a = *reinterpret_cast<const u32x2 *>(q), b = *reinterpret_cast<const u32x2 *>(q + C * D);
+                w = (u32x4){a.x, a.y, b.x, b.y};
+            } else {
+                w = *reinterpret_cast<const u32x4 *>(q);
+            }
+            const bool ok = row0 + u * (NTHR / PER) < n && 0 < ocol;
+            const unsigned at = first + u * (NTHR / PER) * (unsigned)o_st;
+            if (VEC == 2) {
+                __builtin_amdgcn_raw_buffer_store_b128(w, rs, ok ? at : NOWHERE, 0, STREAM);
+            } else if (VEC == 1) {
+                __builtin_amdgcn_raw_buffer_store_b64((u32x2){w.x, w.y}, rs, ok ? at : NOWHERE, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b64((u32x2){w.z, w.w}, rs, ok && UE / 2 < ocol ? at + 8 : NOWHERE, 0, 0);
+            } else if (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_buffer_store_b32((unsigned)w[i], rs, ok && i < ocol ? at + 4 * i : NOWHERE, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[i / 2] >> (16 * (i % 2))), rs, ok && i < ocol ? at + 2 * i : NOWHERE, 0, 0);
+            }
+        }
+    }
+    // into LDS planes of C rows of D elements; the last thread's units may lie behind the tile
+    __device__ __forceinline__ void store(const Flight &f, __bf16 *tile, int tid) const
+    {
+        const u32x4 (&raw)[U] = f.raw;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (U * NTHR > N && tid + u * NTHR >= N) break;
@@ -419,23 +459,23 @@ struct Pass {
     template <int I, int J0, int J1>
     static __device__ __forceinline__ void row_tiles(const __bf16 *x, const __bf16 *y, __bf16 *P, const Decays<C> &d, float scale_p, int lr, int lg)
     {
-        constexpr int JE = J1 < I ? J1 : I;
-        b16x8 xf[DC / 32][NP];
-        f32x4 p[JE - J0 + 1 > 0 ? JE - J0 + 1 : 1];
+        constexpr int JE = J1 < I ? J1 : I, NJ = JE - J0 + 1;
+        f32x4 p[NJ];
 #pragma unroll
-        for (int s = 0; s < DC / 32; ++s)
+        for (int J = 0; J < NJ; ++J) p[J] = (f32x4){0, 0, 0, 0};
 #pragma unroll
-            for (int k = 0; k < NP; ++k) xf[s][k] = *reinterpret_cast<const b16x8 *>(x + k * C * DC + at<DC>(I * 16 + lr, 32 * s + 8 * lg));
+        for (int s = 0; s < DC / 32; ++s) {
+            b16x8 xf[NP], yf[NJ][NP];
 #pragma unroll
-        for (int J = J0; J <= JE; ++J) {
-            p[J - J0] = (f32x4){0, 0, 0, 0};
+            for (int k = 0; k < NP; ++k) {
+                xf[k] = *reinterpret_cast<const b16x8 *>(x + k * C * DC + at<DC>(I * 16 + lr, 32 * s + 8 * lg));
 #pragma unroll
-            for (int s = 0; s < DC / 32; ++s) {
-                b16x8 yf[NP];
-#pragma unroll
-                for (int k = 0; k < NP; ++k) yf[k] = *reinterpret_cast<const b16x8 *>(y + k * C * DC + at<DC>(J * 16 + lr, 32 * s + 8 * lg));
-                p[J - J0] = mma<NP, NP>(yf, xf[s], p[J - J0]);
+                for (int J = 0; J < NJ; ++J) yf[J][k] = *reinterpret_cast<const b16x8 *>(y + k * C * DC + at<DC>((J0 + J) * 16 + lr, 32 * s + 8 * lg));
             }
+            plane_products<NP, NP>([&](int i, int j) __attribute__((always_inline)) {
+#pragma unroll
+                for (int J = 0; J < NJ; ++J) p[J] = mfma(yf[J][i], xf[j], p[J]);
+            });
         }
         const float gh = d.Gh[I * 16 + lr], gl = d.Gl[I * 16 + lr];
 #pragma unroll
@@ -444,12 +484,12 @@ struct Pass {
             if (J == I) {
                 const f32x4 jh = *reinterpret_cast<const f32x4 *>(&d.Gh[I * 16 + 4 * lg]), jl = *reinterpret_cast<const f32x4 *>(&d.Gl[I * 16 + 4 * lg]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) q[r] = 4 * lg + r > lr ? 0.0f : p[J - J0][r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
+                for (int r = 0; r < 4; ++r) q[r] = 4 * lg + r > lr ? 0.0f : p[J < NJ + J0 ? J - J0 : 0][r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
             } else if (J < I) {
                 const f32x4 f = *reinterpret_cast<const f32x4 *>(&d.F[J * 16 + 4 * lg]);
                 const float row = fast_exp2((gh - d.Gh[J * 16 + 15]) + (gl - d.Gl[J * 16 + 15])) * scale_p;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) q[r] = p[J - J0][r] * (row * f[r]);
+                for (int r = 0; r < 4; ++r) q[r] = p[J < NJ + J0 ? J - J0 : 0][r] * (row * f[r]);
             }
             keep(P, I, J, q, lr, lg);
         }
@@ -499,18 +539,21 @@ struct Pass {
                 for (int j = 0; j < 8; ++j) w[j] = S[2 * s + j / 4][n][j % 4];
                 split8<NX>(w, st[n]);
             }
+            b16x8 xf[CT][NP];
 #pragma unroll
-            for (int I = 0; I < CT; ++I) {
-                b16x8 xf[NP];
+            for (int I = 0; I < CT; ++I)
 #pragma unroll
                 for (int k = 0; k < NP; ++k) {
                     const __bf16 *q = x + k * C * DC;
-                    xf[k] = join(*reinterpret_cast<const b16x4 *>(q + at<DC>(I * 16 + lr, 32 * s + 4 * lg)),
-                                 *reinterpret_cast<const b16x4 *>(q + at<DC>(I * 16 + lr, 32 * s + 16 + 4 * lg)));
+                    xf[I][k] = join(*reinterpret_cast<const b16x4 *>(q + at<DC>(I * 16 + lr, 32 * s + 4 * lg)),
+                                    *reinterpret_cast<const b16x4 *>(q + at<DC>(I * 16 + lr, 32 * s + 16 + 4 * lg)));
                 }
+            plane_products<NX, NP>([&](int i, int j) __attribute__((always_inline)) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) O[I][n] = mma<NX, NP>(st[n], xf, O[I][n]);
-            }
+                for (int I = 0; I < CT; ++I)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) O[I][n] = mfma(st[n][i], xf[I][j], O[I][n]);
+            });
         }
 #pragma unroll
         for (int I = 0; I < CT; ++I) {
@@ -543,14 +586,17 @@ struct Pass {
                 }
             }
             if (!STATE_ONLY) {
+                b16x8 pf[CT][NC];
 #pragma unroll
-                for (int I = 2 * s; I < CT; ++I) {
-                    b16x8 pf[NC];
+                for (int I = 2 * s; I < CT; ++I)
 #pragma unroll
-                    for (int k = 0; k < NC; ++k) pf[k] = *reinterpret_cast<const b16x8 *>(P + k * C * C + at<C>(I * 16 + lr, 32 * s + 8 * lg));
+                    for (int k = 0; k < NC; ++k) pf[I][k] = *reinterpret_cast<const b16x8 *>(P + k * C * C + at<C>(I * 16 + lr, 32 * s + 8 * lg));
+                plane_products<NP, NC>([&](int i, int j) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) O[I][n] = mma<NP, NC>(zf[n], pf, O[I][n]);
-                }
+                    for (int I = 2 * s; I < CT; ++I)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) O[I][n] = mfma(zf[n][i], pf[I][j], O[I][n]);
+                });
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -564,25 +610,51 @@ struct Pass {
                 }
                 split8<NS>(w, zs[n]);
             }
+            constexpr int TG = KT < 4 ? KT : 4;          // rows of S at a time
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                b16x8 yf[NP];
+            for (int t0 = 0; t0 < KT; t0 += TG) {
+                b16x8 yf[TG][NP];
 #pragma unroll
-                for (int k = 0; k < NP; ++k) {
-                    const __bf16 *q = y + k * C * DC + at<DC>(row + lr / 4, 16 * t + 4 * (lr % 4));
-                    yf[k] = join(read_tr(q), read_tr(q + 16 * DC));
-                }
+                for (int t = 0; t < TG; ++t)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) S[t][n] = mma<NP, NS>(yf, zs[n], S[t][n]);
+                    for (int k = 0; k < NP; ++k) {
+                        const __bf16 *q = y + k * C * DC + at<DC>(row + lr / 4, 16 * (t0 + t) + 4 * (lr % 4));
+                        yf[t][k] = join(read_tr(q), read_tr(q + 16 * DC));
+                    }
+                plane_products<NP, NS>([&](int i, int j) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int t = 0; t < TG; ++t)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) S[t0 + t][n] = mfma(yf[t][i], zs[n][j], S[t0 + t][n]);
+                });
             }
         }
     }
 
+    // rows of o into a tile of x's shape, in the call's type (fp32: 8 bytes of 4 elements in plane 0, 8 in plane 1)
+    __device__ __forceinline__ void lay_rows(__bf16 *tile, int z0, int lr, int lg) const
+    {
+#pragma unroll
+        for (int I = 0; I < CT; ++I)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                __bf16 *q = tile + at<DZ>(I * 16 + lr, z0 + 16 * n + 4 * lg);
+                if constexpr (sizeof(T) == 4) {
+                    const u32x4 w = __builtin_bit_cast(u32x4, O[I][n]);
+                    *reinterpret_cast<u32x2 *>(q) = (u32x2){w.x, w.y};
+                    *reinterpret_cast<u32x2 *>(q + C * DZ) = (u32x2){w.z, w.w};
+                } else {
+                    typedef T tx4 __attribute__((ext_vector_type(4)));
+                    *reinterpret_cast<u32x2 *>(q) = __builtin_bit_cast(u32x2, __builtin_convertvector(O[I][n], tx4));
+                }
+            }
+    }
+
     // rows of o: row r is token t0 + r, or t0 + C - 1 - r where time runs backwards; valid ones lie before token `len`
     template <int VEC>
-    __device__ __forceinline__ void store_rows(const Rows<T, C, VEC> &o, const Rows<T, C, VEC> &w, bool dot_wanted, int t0, int len, int lg, float *dots)
+    __device__ __forceinline__ void store_rows(const Rows<T, C, VEC> &o, const Rows<T, C, VEC> &w, bool rows_wanted, bool dot_wanted, int t0, int len, int lg, float *dots)
     {
-        if (o.p) {
+        if (rows_wanted) {
             const __amdgpu_buffer_rsrc_t rs = buffer(o.p + (long long)t0 * o.st);
 #pragma unroll
             for (int I = 0; I < CT; ++I)
@@ -672,20 +744,22 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
     Tile<T, DZ, C, NTHR, VEC> tz;
     ty.init(ro.Y, w.b, w.h, tid, ro.reverse);
     tz.init(ro.Z, w.b, w.h, tid, ro.reverse);
+    typename decltype(ty)::Flight fy;
+    typename decltype(tz)::Flight fz;
     float g = 0.0f;
     double gsum = 0.0;
     const auto fetch = [&](int ci) {
         const int t0 = token0(ci);
-        ty.fetch(t0, w.len - t0);
-        tz.fetch(t0, w.len - t0);
+        ty.fetch(fy, t0, w.len - t0);
+        tz.fetch(fz, t0, w.len - t0);
         if (wave == NW - 1) g = fetch_decay<C>(pg, a.gt, t0, w.len, ro.reverse, lane);
     };
     if (w.c0 < w.c1) fetch(w.c0);
     for (int ci = w.c0; ci < w.c1; ++ci) {
         if (wave == NW - 1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[ci & 1]);
         __syncthreads();                              // nobody reads the last chunk's tiles any more
-        ty.store(sm.y, tid);
-        tz.store(sm.z, tid);
+        ty.store(fy, sm.y, tid);
+        tz.store(fz, sm.z, tid);
         __syncthreads();
         if (ci + 1 < w.c1) fetch(ci + 1);
         ps.from_chunk(sm.y, sm.z, nullptr, sm.d[ci & 1], z0, lr, lg);
@@ -696,15 +770,18 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
 }
 
 // One pass.  The first waves own the state's columns, the others feed them: they fetch and lay out the tiles, keep the
-// decays and compute the scores, a chunk ahead.  A chunk has two phases, a barrier behind each:
-//   1  feeders: x, y, decays of the next chunk, z of this one   owners: o from the state
-//   2  feeders: scores of the next chunk                        owners: o and the state from this chunk, rows of o out
-// so that z alone needs one tile and the owners never wait for the feeders' loads or exponentials.
+// decays, compute the scores, a chunk ahead, and write the rows of o.  A chunk has two phases, a barrier behind each:
+//   1  feeders: o of the last chunk out; x, y, decays of the next one, z of this one    owners: o from the state
+//   2  feeders: scores of the next chunk                                               owners: o and the state from this chunk
+// so that z alone needs one tile and the owners never wait for the feeders' loads or exponentials.  In phase 2 the owners leave o in the
+// x tile that nobody reads any more, and the feeders write whole rows of it (the owners' own columns are 32-byte pieces,
+// and cost the memory twice as much).
 // Waves of a SIMD that the LDS leaves room for: two workgroups of 8 where the tiles take less than half of it.
 template <typename T, int DC, int DZ> constexpr int residents()
 {
     const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * Kind<T>::NC * chunk<T>() * chunk<T>() * 2 + 6 * 1024;
-    return (owners<T, DZ>() + feeders<DZ>()) / 4 * (tiles <= 80 * 1024 ? 2 : 1);
+    const int waves = owners<T, DZ>() + feeders<DZ>();
+    return waves / 4 * (waves == 8 && tiles <= 80 * 1024 ? 2 : 1);
 }
 
 template <typename T, int DC, int DZ, int VEC, bool FINE>
@@ -712,6 +789,8 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>())), (res
 {
     constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<DZ>(), NTHR = 64 * (NO + NF);
     constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
+    constexpr bool WHOLE = DC == DZ;                 // rows of o fit x's tile
+    constexpr int AHEAD = DC <= 64 && DZ <= 64 ? 2 : 1;   // chunks of rows in flight: with 128 columns one is as many bytes, and registers are short
     typedef Pass<T, DC, DZ, C, NO, NX, false> P;
     struct Shared {
         alignas(16) __bf16 x[2][NP * C * DC];
@@ -738,56 +817,66 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>())), (res
         tx.init(ro.X, w.b, w.h, ft, reverse);
         ty.init(ro.Y, w.b, w.h, ft, reverse);
         tz.init(ro.Z, w.b, w.h, ft, reverse);
-        const long long gt = held(a.gt);
+        struct Chunk {
+            typename decltype(tx)::Flight x, y;
+            typename decltype(tz)::Flight z;
+            float g;
+        } even, odd;                                     // the chunks of either parity from c0 on
+        const long long gt = held(a.gt), o_st = held(ro.O.st * (long long)sizeof(T));
+        const char *const o = held(WHOLE && ro.O.p && !ro.O.f32 ? ro.O.p + ((long long)w.b * ro.O.sb + (long long)w.h * ro.O.sh) * (long long)sizeof(T) : nullptr);
+        tx.ocol = ro.O.d - (ft % tx.PER) * tx.UE;
         const float scale_p = held(ro.scale_p), scale_x = held(ro.scale_x), scale_z = held(ro.scale_z);
-        float g = 0.0f;
-        const auto fetch_xy = [&](int ci) {
+        const auto fetch_xy = [&](int ci, Chunk &f) __attribute__((always_inline)) {
+            if (ci >= c1) return;
             const int t0 = token0(ci);
-            tx.fetch(t0, len - t0);
-            ty.fetch(t0, len - t0);
-            if (fw == 0) g = fetch_decay<C>(pg, gt, t0, len, reverse, lane);
+            tx.fetch(f.x, t0, len - t0);
+            ty.fetch(f.y, t0, len - t0);
+            if (fw == 0) f.g = fetch_decay<C>(pg, gt, t0, len, reverse, lane);
         };
-        const auto store_xy = [&](int ci) {
-            tx.store(sm.x[ci & 1], ft);
-            ty.store(sm.y[ci & 1], ft);
-            if (fw == 0) decays<C>(g, lane, scale_x, scale_z, sm.d[ci & 1]);
+        const auto fetch_z = [&](int ci, Chunk &f) __attribute__((always_inline)) {
+            if (ci < c1) tz.fetch(f.z, token0(ci), len - token0(ci));
         };
-        const auto scores = [&](int ci) {
-            P::template scores<NF>(sm.x[ci & 1], sm.y[ci & 1], sm.p[ci & 1], sm.d[ci & 1], scale_p, fw, lr, lg);
+        const auto store_xy = [&](int ci, const Chunk &f) __attribute__((always_inline)) {
+            tx.store(f.x, sm.x[ci & 1], ft);
+            ty.store(f.y, sm.y[ci & 1], ft);
+            if (fw == 0) decays<C>(f.g, lane, scale_x, scale_z, sm.d[ci & 1]);
         };
-        const auto flush_dots = [&](int ci) {
+        const auto flush = [&](int ci) __attribute__((always_inline)) {
+            if (o) tx.drain(sm.x[ci & 1], ft, o + token0(ci) * o_st, o_st, len - token0(ci));
             const int t = token0(ci) + ft;
-            if (ft < C && t < len) {
+            if (dots && ft < C && t < len) {
                 float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NO; ++i) s += sm.dots[i][ft];
                 dots[t] = s;
             }
         };
-        if (c0 < c1) {
-            fetch_xy(c0);
-            tz.fetch(token0(c0), len - token0(c0));
-            store_xy(c0);
-            if (c0 + 1 < c1) fetch_xy(c0 + 1);
-            __syncthreads();
-            scores(c0);
-        } else {
-            __syncthreads();
-        }
-        __syncthreads();
-        for (int ci = c0; ci < c1; ++ci) {
-            tz.store(sm.z, ft);
-            if (ci + 1 < c1) {
-                tz.fetch(token0(ci + 1), len - token0(ci + 1));
-                store_xy(ci + 1);
-                if (ci + 2 < c1) fetch_xy(ci + 2);
+        const auto lay = [&](int ci, Chunk &mine, Chunk &other) __attribute__((always_inline)) {
+            if (ci >= c0) {
+                tz.store(mine.z, sm.z, ft);
+                fetch_z(ci + AHEAD, mine);
             }
-            if (dots && ci > c0) flush_dots(ci - 1);
+            if (ci + 1 < c1) {
+                store_xy(ci + 1, other);
+                fetch_xy(ci + 1 + AHEAD, other);
+            }
+        };
+        fetch_xy(c0, even);
+        fetch_z(c0, even);
+        if (AHEAD == 2) {
+            fetch_xy(c0 + 1, odd);
+            fetch_z(c0 + 1, odd);
+        }
+        for (int ci = c0 - 1; ci < c1; ++ci) {           // the first turn lays out chunk c0 only
+            if (ci > c0) flush(ci - 1);
+            if (AHEAD == 1) lay(ci, even, even);
+            else if ((ci - c0) & 1) lay(ci, odd, even);
+            else lay(ci, even, odd);
             __syncthreads();
-            if (ci + 1 < c1) scores(ci + 1);
+            if (ci + 1 < c1) P::template scores<NF>(sm.x[(ci + 1) & 1], sm.y[(ci + 1) & 1], sm.p[(ci + 1) & 1], sm.d[(ci + 1) & 1], scale_p, fw, lr, lg);
             __syncthreads();
         }
-        if (dots && c0 < c1) flush_dots(c1 - 1);
+        if (c0 < c1) flush(c1 - 1);
     } else {
         const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
         const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(ro.W, w.b, w.h, reverse, lr, z0 + 4 * lg);
@@ -799,14 +888,17 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>())), (res
             ps.resume(reinterpret_cast<const f32x4 *>(a.states + ((size_t)(w.ri * a.B * a.H + w.bh) * a.nseg + w.seg - 1) * (DC * DZ)) +
                       wave * P::KT * P::NT * 64 + lane);
         }
-        __syncthreads();
-        __syncthreads();
+        if (c0 <= c1) {                                  // the feeders' first turn
+            __syncthreads();
+            __syncthreads();
+        }
         for (int ci = c0; ci < c1; ++ci) {
             const Decays<C> &d = sm.d[ci & 1];
             ps.from_state(sm.x[ci & 1], d, lr, lg);
             __syncthreads();
             ps.from_chunk(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
-            ps.store_rows(out, wrows, dots != nullptr, token0(ci), len, lg, sm.dots[wave]);
+            if (WHOLE && !out.f32) ps.lay_rows(sm.x[ci & 1], z0, lr, lg);
+            ps.store_rows(out, wrows, out.p && !(WHOLE && !out.f32), dots != nullptr, token0(ci), len, lg, sm.dots[wave]);
             __syncthreads();
         }
         if (ro.s_out && w.seg == a.nseg - 1)
@@ -862,6 +954,8 @@ struct Pair {
         }
         Tile<T, DK, C, NTHR, VEC> tq, tk;
         Tile<T, DV, C, NTHR, VEC> tv, to;
+        typename decltype(tq)::Flight fq, fk;
+        typename decltype(tv)::Flight fv, fo;
         tq.init(r0.Y, b, h, tid, 1);
         to.init(r0.Z, b, h, tid, 1);
         if (!STATE_ONLY) {
@@ -872,11 +966,11 @@ struct Pair {
         double gsum = 0.0;
         const auto fetch = [&](int ci) {
             const int t0 = token0(ci), n = len - t0;
-            tq.fetch(t0, n);
-            to.fetch(t0, n);
+            tq.fetch(fq, t0, n);
+            to.fetch(fo, t0, n);
             if (!STATE_ONLY) {
-                tk.fetch(t0, n);
-                tv.fetch(t0, n);
+                tk.fetch(fk, t0, n);
+                tv.fetch(fv, t0, n);
             }
         };
         const auto fetch_g = [&](int ci) { g = fetch_decay<C>(pg, a.gt, token0(ci), len, 1, lane); };
@@ -900,11 +994,11 @@ struct Pair {
             const Decays<C> &d = sm.d[ci & 1];
             __syncthreads();                              // nobody reads the last chunk's tiles any more
             if (!STATE_ONLY && r1.dots && ci > c0) flush_dots(ci - 1);
-            tq.store(sm.q, tid);
-            to.store(sm.o, tid);
+            tq.store(fq, sm.q, tid);
+            to.store(fo, sm.o, tid);
             if (!STATE_ONLY) {
-                tk.store(sm.k, tid);
-                tv.store(sm.v, tid);
+                tk.store(fk, sm.k, tid);
+                tv.store(fv, sm.v, tid);
             }
             __syncthreads();
             if (ci + 1 < c1) {
@@ -917,7 +1011,7 @@ struct Pair {
                 __syncthreads();                          // the scores are whole
             }
             ps.from_chunk(y, z, p, d, z0, lr, lg);
-            if (!STATE_ONLY) ps.store_rows(out, wrows, gr && r1.dots, token0(ci), len, lg, sm.dots[gr ? wave : 0]);
+            if (!STATE_ONLY) ps.store_rows(out, wrows, out.p, gr && r1.dots, token0(ci), len, lg, sm.dots[gr ? wave : 0]);
             if (clock && ci + 1 < c1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[(ci + 1) & 1]);
         }
         if (STATE_ONLY) {
