@@ -682,7 +682,8 @@ struct Pass {
 
 template <typename T> constexpr int chunk() { return Kind<T>::NP == 1 ? 64 : 32; }       // chunk_tokens()
 // waves that own columns of the state, a 16-column tile each (two of them where 128 columns leave the registers for it)
-template <int DZ> constexpr int feeders() { return DZ == 32 ? 2 : 4; }
+// waves that feed them: as many as own where splitting fp32 rows into planes is most of their work
+template <typename T, int DZ> constexpr int feeders() { return DZ == 32 ? 2 : (DZ == 128 && Kind<T>::NP == 3 ? 8 : 4); }
 template <typename T, int DZ> constexpr int owners() { return DZ / 16 < 4 ? DZ / 16 : (DZ == 128 ? 8 : 4); }
 
 // rows first .. behind - 1 of o that lie behind the sample's length: zeros
@@ -780,14 +781,14 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
 template <typename T, int DC, int DZ> constexpr int residents()
 {
     const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * Kind<T>::NC * chunk<T>() * chunk<T>() * 2 + 6 * 1024;
-    const int waves = owners<T, DZ>() + feeders<DZ>();
+    const int waves = owners<T, DZ>() + feeders<T, DZ>();
     return waves / 4 * (waves == 8 && tiles <= 80 * 1024 ? 2 : 1);
 }
 
 template <typename T, int DC, int DZ, int VEC, bool FINE>
-__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<DZ>())), (residents<T, DC, DZ>())) chunk_kernel(const Args a)
+__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ>())) chunk_kernel(const Args a)
 {
-    constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<DZ>(), NTHR = 64 * (NO + NF);
+    constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<T, DZ>(), NTHR = 64 * (NO + NF);
     constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
     constexpr bool WHOLE = DC == DZ;                 // rows of o fit x's tile
     constexpr int AHEAD = DC <= 64 && DZ <= 64 ? 2 : 1;   // chunks of rows in flight: with 128 columns one is as many bytes, and registers are short
@@ -1062,7 +1063,7 @@ static int launch_one(const Args &a, int kind, hipStream_t stream)
         else if (fine) pair_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3, false><<<grid, n, 0, stream>>>(a);
         else pair_kernel<T, DC, DZ, VEC, false, false><<<grid, n, 0, stream>>>(a);
     } else {
-        constexpr int n = 64 * (owners<T, DZ>() + feeders<DZ>());
+        constexpr int n = 64 * (owners<T, DZ>() + feeders<T, DZ>());
         if (kind & STATES) state_kernel<T, DC, DZ, VEC><<<grid, 64 * owners<T, DZ>(), 0, stream>>>(a);
         else if (fine) chunk_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3><<<grid, n, 0, stream>>>(a);
         else chunk_kernel<T, DC, DZ, VEC, false><<<grid, n, 0, stream>>>(a);
