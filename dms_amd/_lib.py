@@ -15,7 +15,6 @@ ABI_VERSION = 4
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
-_d = ctypes.c_double
 _ll = ctypes.c_longlong
 
 # name -> argtypes, mirrors include/dmn_hip.h one to one
@@ -60,9 +59,9 @@ SIGNATURES = {
     "dmn_linear_attention_fwd": [_i] + [_p] * 6 + [_i] + [_p] * 4 + [_i] * 8 + [_f, _p],
     "dmn_linear_attention_bwd": [_i] + [_p] * 6 + [_i] + [_p] * 6 + [_i] + [_p] * 3 + [_i] * 8 + [_f, _p],
     "dmn_linear_attention_step": [_i] + [_p] * 7 + [_i] * 7 + [_f, _p],
-    "dmn_head_norm_rotary_fwd": [_i] + [_p] * 4 + [_i, _p, _i, _p, _i, _d, _f] + [_p] * 3 + [_i] * 5 + [_p],
+    "dmn_head_norm_rotary_fwd": [_i] + [_p] * 4 + [_i, _p, _i, _p, _i, _p, _f] + [_p] * 3 + [_i] * 5 + [_p],
     "dmn_head_norm_rotary_workspace_floats": [_i] * 3,
-    "dmn_head_norm_rotary_bwd": [_i] + [_p] * 4 + [_i, _p, _i, _p, _i, _d, _f] + [_p] * 8 + [_i] * 5 + [_p],
+    "dmn_head_norm_rotary_bwd": [_i] + [_p] * 4 + [_i, _p, _i, _p, _i, _p, _f] + [_p] * 8 + [_i] * 5 + [_p],
 }
 
 # entry points whose return VALUE is not a C int
@@ -101,7 +100,7 @@ def load():
 
 def call(name, *args):
     """Invoke an entry point; non-zero status -> RuntimeError(dmn_last_error())."""
-    lib = load()
+    lib = _lib or load()
     timer = TIMER
     token = timer.begin(name, args) if timer is not None else None
     rc = getattr(lib, name)(*args)

@@ -1,8 +1,8 @@
 // dms_amd/csrc/head_norm_rotary.hip -- RMS norm of every query and key head and its rotation by positions on several
 // axes, in one pass, and the gradients of both.
 //
-//   y = x rsqrt(mean(x^2) + eps) w;   pair (2i, 2i + 1) of y turns by pos[axis(i)] * base^(-j/n), j the pair's number in its
-//   axis' section of n pairs; the pairs behind all sections stay as they are.
+//   y = x rsqrt(mean(x^2) + eps) w;   pair (2i, 2i + 1) of y turns by pos[axis(i)] * rate(i); the pairs behind all axes' sections
+//   stay as they are.
 // Backward, with u = dy turned back:  dw = sum u x r,  dx = r u w - x r^3 mean(x u w),  r = rsqrt(mean(x^2) + eps).
 //
 // Bound by memory: x is read and y written once (backward: x and dy read, dx written), in 16-byte pieces where the rows
@@ -10,8 +10,6 @@
 // them: a lane keeps those of its own E/2 pairs.  The angle is formed in turns and in 64 bits (a position of 2^20 radians
 // has lost 4 digits in 32), reduced there, and only the rest of the turn goes on in 32.
 #include "common.h"
-
-#include <cmath>
 
 namespace dmn {
 namespace hnr {
@@ -349,7 +347,7 @@ static int run(const char *who, int dtype, Args &a, bool backward, hipStream_t s
     return launch_status(who);
 }
 
-static int check(const char *who, int dtype, int T, int B, int Hq, int Hk, int D, const int *sections, int axes, double base)
+static int check(const char *who, int dtype, int T, int B, int Hq, int Hk, int D, const int *sections, int axes, const double *rates)
 {
     if (dtype < 0 || dtype > 2) return fail(-2, "%s: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16), got %d", who, dtype);
     if (T < 0 || B < 0 || Hq < 1 || Hk < 0) return fail(-3, "%s: bad sizes T=%d B=%d Hq=%d Hk=%d", who, T, B, Hq, Hk);
@@ -361,12 +359,12 @@ static int check(const char *who, int dtype, int T, int B, int Hq, int Hk, int D
         sum += sections[i];
     }
     if (sum > D / 2) return fail(-4, "%s: %d pairs turn, a head of width %d has %d", who, sum, D, D / 2);
-    if (!(base > 0.0)) return fail(-4, "%s: base must be positive", who);
+    if (sum > 0 && !rates) return fail(-1, "%s: null pointer", who);
     return 0;
 }
 
 static void fill(Args &a, const void *q, const void *k, const void *wq, const void *wk, int w32, const void *pos, int pos64, const int *sections,
-                 int axes, double base, float eps, const long long *s, int T, int B, int Hq, int Hk, int D)
+                 int axes, const double *rates, float eps, const long long *s, int T, int B, int Hq, int Hk, int D)
 {
     a.x[0] = rows(q, T, B, Hq, s);
     a.x[1] = rows(k, T, B, Hk, s + 3);
@@ -389,7 +387,7 @@ static void fill(Args &a, const void *q, const void *k, const void *wq, const vo
     a.table.pairs = 0;
     for (int i = 0; i < axes; ++i)
         for (int j = 0; j < sections[i]; ++j) {
-            a.table.turns[a.table.pairs] = pow(base, -(double)j / sections[i]) / 6.283185307179586476925286766559;
+            a.table.turns[a.table.pairs] = rates[a.table.pairs] * 0.15915494309189533576888376337251;      // 1 / 2 pi
             a.table.axis[a.table.pairs++] = i;
         }
 }
@@ -401,16 +399,16 @@ using namespace dmn;
 using namespace dmn::hnr;
 
 extern "C" int dmn_head_norm_rotary_fwd(int dtype, const void *q, const void *k, const void *wq, const void *wk, int w32, const void *positions,
-                                        int positions64, const int *sections, int axes, double base, float eps, void *yq, void *yk,
+                                        int positions64, const int *sections, int axes, const double *rates, float eps, void *yq, void *yk,
                                         const long long *strides, int T, int B, int Hq, int Hk, int D, void *stream)
 {
     const char *who = "dmn_head_norm_rotary_fwd";
-    const int rc = check(who, dtype, T, B, Hq, Hk, D, sections, axes, base);
+    const int rc = check(who, dtype, T, B, Hq, Hk, D, sections, axes, rates);
     if (rc) return rc;
     if (!strides || (T > 0 && B > 0 && (!q || !yq || (Hk && (!k || !yk)) || (axes > 0 && !positions)))) return fail(-1, "%s: null pointer", who);
     if ((long long)T * B == 0) return 0;
     Args a;
-    fill(a, q, k, wq, wk, w32, positions, positions64, sections, axes, base, eps, strides, T, B, Hq, Hk, D);
+    fill(a, q, k, wq, wk, w32, positions, positions64, sections, axes, rates, eps, strides, T, B, Hq, Hk, D);
     a.out[0] = dense(yq, T, B, Hq, D);
     a.out[1] = dense(yk, T, B, Hk, D);
     return run(who, dtype, a, false, (hipStream_t)stream);
@@ -423,12 +421,12 @@ extern "C" int dmn_head_norm_rotary_workspace_floats(int Hq, int Hk, int D)
 }
 
 extern "C" int dmn_head_norm_rotary_bwd(int dtype, const void *q, const void *k, const void *wq, const void *wk, int w32, const void *positions,
-                                        int positions64, const int *sections, int axes, double base, float eps, const void *grad_yq,
+                                        int positions64, const int *sections, int axes, const double *rates, float eps, const void *grad_yq,
                                         const void *grad_yk, void *grad_q, void *grad_k, void *grad_wq, void *grad_wk, const long long *strides,
                                         float *workspace, int T, int B, int Hq, int Hk, int D, void *stream)
 {
     const char *who = "dmn_head_norm_rotary_bwd";
-    int rc = check(who, dtype, T, B, Hq, Hk, D, sections, axes, base);
+    int rc = check(who, dtype, T, B, Hq, Hk, D, sections, axes, rates);
     if (rc) return rc;
     if (!strides || (T > 0 && B > 0 && (!q || !grad_yq || !grad_q || (Hk && (!k || !grad_yk || !grad_k)) || (axes > 0 && !positions))))
         return fail(-1, "%s: null pointer", who);
@@ -439,7 +437,7 @@ extern "C" int dmn_head_norm_rotary_bwd(int dtype, const void *q, const void *k,
     a.nslice = 0;
     long long blocks = 0;
     if ((long long)T * B > 0) {
-        fill(a, q, k, wq, wk, w32, positions, positions64, sections, axes, base, eps, strides, T, B, Hq, Hk, D);
+        fill(a, q, k, wq, wk, w32, positions, positions64, sections, axes, rates, eps, strides, T, B, Hq, Hk, D);
         a.dy[0] = rows(grad_yq, T, B, Hq, strides + 9);
         a.dy[1] = rows(grad_yk, T, B, Hk, strides + 12);
         a.out[0] = dense(grad_q, T, B, Hq, D);

@@ -7,6 +7,7 @@ fp32, bf16 or fp16) and on a ROCm device -- anything else raises (there is no CP
 """
 import contextlib
 import ctypes
+import functools
 import os
 import tempfile
 
@@ -790,6 +791,15 @@ _DTYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 LINEAR_ATTENTION_MAX_WIDTH = 128
 
 
+def _on(device):
+    """torch.cuda.device(device), without its cost where that is the current one already."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream_of(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _chk_rows(name, what, t, shape, dtype, device):
     """A tensor with unit stride along its last axis and any other strides."""
     if not torch.is_tensor(t) or not t.is_cuda:
@@ -806,6 +816,13 @@ def _chk_rows(name, what, t, shape, dtype, device):
 
 def _chk_heads(name, q, k, v, H):
     """Type and widths of q, k, v (..., heads, width) beside a state of H heads."""
+    if isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor):          # all well: one look
+        sq, sk, sv, dev, dt, most = q.shape, k.shape, v.shape, q.device, q.dtype, LINEAR_ATTENTION_MAX_WIDTH
+        if (q.is_cuda and dt in _DTYPE_IDS and k.dtype is dt and v.dtype is dt and k.device == dev and v.device == dev
+                and len(sk) == len(sq) == len(sv) and sk[:-2] == sq[:-2] == sv[:-2] and 0 < sk[-1] == sq[-1] <= most
+                and 0 < sv[-1] <= most and q.stride(-1) == k.stride(-1) == v.stride(-1) == 1
+                and sq[-2] and sk[-2] and sv[-2] and not (H % sq[-2] or H % sk[-2] or H % sv[-2])):
+            return
     if not torch.is_tensor(q) or q.dtype not in _DTYPE_IDS:
         raise RuntimeError("dms_amd.%s: q, k and v must be float32, bfloat16 or float16 tensors" % name)
     lead = q.shape[:-2]
@@ -828,6 +845,12 @@ def _strides(*groups):
     return (ctypes.c_longlong * len(flat))(*flat)
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace(name, *sizes):
+    """Floats of workspace, by the sizes alone."""
+    return _lib.query(name, *sizes)
+
+
 def _linear_attention_sizes(q, k, v, H):
     T, B, Hq, dk = q.shape
     return T, B, H, Hq, k.shape[2], v.shape[2], dk, v.shape[3]
@@ -840,14 +863,14 @@ def _decay_strides(g):
 def _linear_attention_raw(q, k, v, g, state0, lengths, scale):
     T, B, H, Hq, Hk, Hv, dk, dv = sizes = _linear_attention_sizes(q, k, v, g.shape[-1])
     dt = _DTYPE_IDS[q.dtype]
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         o = torch.empty((T, B, H, dv), device=q.device, dtype=q.dtype)
         state = torch.empty((B, H, dk, dv), device=q.device, dtype=torch.float32)
-        n = _lib.query("dmn_linear_attention_workspace_floats", dt, 0, *sizes)
+        n = _workspace("dmn_linear_attention_workspace_floats", dt, 0, *sizes)
         ws = torch.empty(n, device=q.device, dtype=torch.float32) if n > 0 else None
         _lib.call("dmn_linear_attention_fwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state0), _ptr(lengths),
                   int(lengths is not None and lengths.dtype == torch.int64), _ptr(o), _ptr(state),
-                  _strides(q.stride()[:3], k.stride()[:3], v.stride()[:3], _decay_strides(g)), _ptr(ws), *sizes, scale, _stream())
+                  _strides(q.stride()[:3], k.stride()[:3], v.stride()[:3], _decay_strides(g)), _ptr(ws), *sizes, scale, _stream_of(q.device))
     return o, state
 
 
@@ -868,7 +891,7 @@ class _LinearAttention(torch.autograd.Function):
         T, B, H, Hq, Hk, Hv, dk, dv = sizes = _linear_attention_sizes(q, k, v, g.shape[-1])
         dt, dev = _DTYPE_IDS[q.dtype], q.device
         need = ctx.needs_input_grad
-        with torch.cuda.device(dev):
+        with _on(dev):
             if grad_o is None:
                 grad_o = torch.zeros(dv, device=dev, dtype=q.dtype).expand(T, B, H, dv)
             elif dv > 1 and grad_o.stride(3) != 1:
@@ -880,13 +903,13 @@ class _LinearAttention(torch.autograd.Function):
             gv = torch.empty((T, B, Hv, dv), device=dev, dtype=q.dtype) if need[2] else None
             gg = torch.empty(g.shape, device=dev, dtype=torch.float32) if need[3] else None
             gs = torch.empty((B, H, dk, dv), device=dev, dtype=torch.float32) if state0 is not None and need[4] else None
-            ws = torch.empty(max(_lib.query("dmn_linear_attention_workspace_floats", dt, 1, *sizes), 4), device=dev,
+            ws = torch.empty(max(_workspace("dmn_linear_attention_workspace_floats", dt, 1, *sizes), 4), device=dev,
                              dtype=torch.float32)
             _lib.call("dmn_linear_attention_bwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state0), _ptr(lengths),
                       int(lengths is not None and lengths.dtype == torch.int64), _ptr(grad_o), _ptr(grad_state), _ptr(gq),
                       _ptr(gk), _ptr(gv), _ptr(gg), int(g.dim() == 1), _ptr(gs),
                       _strides(q.stride()[:3], k.stride()[:3], v.stride()[:3], _decay_strides(g), grad_o.stride()[:3]),
-                      _ptr(ws), *sizes, ctx.scale, _stream())
+                      _ptr(ws), *sizes, ctx.scale, _stream_of(q.device))
         return gq, gk, gv, gg, gs, None, None
 
 
@@ -950,11 +973,11 @@ def linear_attention_step(q, k, v, g, state, scale=None):
         raise RuntimeError("dms_amd.%s: inference only (the state is updated in place): call it under no_grad, or use "
                            "linear_attention" % name)
     scale = float(dk) ** -0.5 if scale is None else float(scale)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         o = torch.empty((B, H, dv), device=q.device, dtype=q.dtype)
         _lib.call("dmn_linear_attention_step", _DTYPE_IDS[q.dtype], _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state), _ptr(o),
                   _strides(q.stride()[:2], k.stride()[:2], v.stride()[:2], (0, g.stride(0)) if g.dim() == 1 else g.stride(),
-                           state.stride()[:1]), B, H, q.shape[1], k.shape[1], v.shape[1], dk, dv, scale, _stream())
+                           state.stride()[:1]), B, H, q.shape[1], k.shape[1], v.shape[1], dk, dv, scale, _stream_of(q.device))
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)      # a graph that saved the state must notice
     return o
@@ -966,23 +989,30 @@ def linear_attention_step(q, k, v, g, state, scale=None):
 HEAD_NORM_ROTARY_MAX_WIDTH = 256
 
 
+@functools.lru_cache(maxsize=256)
+def _rotation(sections, base):
+    """Host arrays of the sections and of every turning pair's radians for a position step."""
+    rates = [base ** (-j / n) for n in sections for j in range(n)]
+    return (ctypes.c_int * max(len(sections), 1))(*sections), (ctypes.c_double * max(len(rates), 1))(*rates)
+
+
 def _head_norm_rotary_args(q, k, wq, wk, positions, sections, base, eps):
-    T, B = q.shape[:2]
+    T, B, Hq, D = q.shape
     pos = (0, 0, 0) if positions is None else ((positions.stride(0), 0, positions.stride(1)) if positions.dim() == 2
                                                else positions.stride())
     weight = wq if wq is not None else wk
+    counts, rates = _rotation(sections, base)
     return (_ptr(q), _ptr(k), _ptr(wq), _ptr(wk), int(weight is not None and weight.dtype == torch.float32), _ptr(positions),
-            int(positions is not None and positions.dtype == torch.int64), (ctypes.c_int * max(len(sections), 1))(*sections),
-            len(sections), base, eps), pos, (T, B, q.shape[2], k.shape[2], q.shape[3])
+            int(positions is not None and positions.dtype == torch.int64), counts, len(sections), rates, eps), pos, (T, B, Hq, k.shape[2], D)
 
 
 def _head_norm_rotary_raw(q, k, wq, wk, positions, sections, base, eps):
     args, pos, sizes = _head_norm_rotary_args(q, k, wq, wk, positions, sections, base, eps)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         yk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
         _lib.call("dmn_head_norm_rotary_fwd", _DTYPE_IDS[q.dtype], *args, _ptr(yq), _ptr(yk),
-                  _strides(q.stride()[:3], k.stride()[:3], pos), *sizes, _stream())
+                  _strides(q.stride()[:3], k.stride()[:3], pos), *sizes, _stream_of(q.device))
     return yq, yk
 
 
@@ -1000,17 +1030,17 @@ class _HeadNormRotary(torch.autograd.Function):
         need, dev = ctx.needs_input_grad, q.device
         args, pos, sizes = _head_norm_rotary_args(q, k, wq, wk, positions, *ctx.consts)
         gyq, gyk = (x if x.shape[3] == 1 or x.stride(3) == 1 else x.contiguous() for x in (gyq, gyk))
-        with torch.cuda.device(dev):
+        with _on(dev):
             gq = torch.empty(q.shape, device=dev, dtype=q.dtype)
             gk = torch.empty(k.shape, device=dev, dtype=q.dtype)
             gwq = torch.empty(wq.shape, device=dev, dtype=wq.dtype) if wq is not None and need[2] else None
             gwk = torch.empty(wk.shape, device=dev, dtype=wk.dtype) if wk is not None and need[3] else None
             ws = None
             if gwq is not None or gwk is not None:
-                ws = torch.empty(_lib.query("dmn_head_norm_rotary_workspace_floats", *sizes[2:]), device=dev, dtype=torch.float32)
+                ws = torch.empty(_workspace("dmn_head_norm_rotary_workspace_floats", *sizes[2:]), device=dev, dtype=torch.float32)
             _lib.call("dmn_head_norm_rotary_bwd", _DTYPE_IDS[q.dtype], *args, _ptr(gyq), _ptr(gyk), _ptr(gq), _ptr(gk), _ptr(gwq),
                       _ptr(gwk), _strides(q.stride()[:3], k.stride()[:3], pos, gyq.stride()[:3], gyk.stride()[:3]), _ptr(ws),
-                      *sizes, _stream())
+                      *sizes, _stream_of(q.device))
         return gq if need[0] else None, gk if need[1] else None, gwq, gwk, None, None, None, None
 
 
@@ -1026,12 +1056,13 @@ def head_norm_rotary(q, k, q_weight, k_weight, positions, sections, base=10000.0
     name = "head_norm_rotary"
     if not torch.is_tensor(q) or q.dim() != 4 or q.dtype not in _DTYPE_IDS:
         raise RuntimeError("dms_amd.%s: q must be a float32, bfloat16 or float16 tensor (T, B, heads, width)" % name)
-    T, B, _, D = q.shape
+    T, B, Hq, D = q.shape
     _chk_rows(name, "q", q, q.shape, q.dtype, q.device)
     if not torch.is_tensor(k) or k.dim() != 4:
         raise RuntimeError("dms_amd.%s: k must have 4 axes like q" % name)
-    _chk_rows(name, "k", k, (T, B, k.shape[2], D), q.dtype, q.device)
-    if q.shape[2] < 1 or k.shape[2] < 1 or not 1 <= D <= HEAD_NORM_ROTARY_MAX_WIDTH:
+    Hk = k.shape[2]
+    _chk_rows(name, "k", k, (T, B, Hk, D), q.dtype, q.device)
+    if Hq < 1 or Hk < 1 or not 1 <= D <= HEAD_NORM_ROTARY_MAX_WIDTH:
         raise RuntimeError("dms_amd.%s: at least one head each, of width 1 .. %d, got %s and %s"
                            % (name, HEAD_NORM_ROTARY_MAX_WIDTH, tuple(q.shape), tuple(k.shape)))
     for what, w in (("q_weight", q_weight), ("k_weight", k_weight)):
@@ -1042,8 +1073,8 @@ def head_norm_rotary(q, k, q_weight, k_weight, positions, sections, base=10000.0
         _chk_rows(name, what, w, (D,), w.dtype, q.device)
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise RuntimeError("dms_amd.%s: q_weight and k_weight must have the same type" % name)
-    sections = tuple(int(n) for n in sections)
-    if len(sections) > 4 or any(n < 0 for n in sections) or sum(sections) > D // 2:
+    sections = tuple(map(int, sections))
+    if len(sections) > 4 or sum(sections) > D // 2 or (sections and min(sections) < 0):
         raise RuntimeError("dms_amd.%s: up to 4 sections of together at most %d pairs, got %s" % (name, D // 2, sections))
     if sections:
         if (not torch.is_tensor(positions) or not positions.is_cuda or positions.device != q.device

@@ -451,24 +451,24 @@ int dmn_linear_attention_step(int dtype, const void *q, const void *k, const voi
  * reference: what stands before linear attention over its (pixel, word) sequence, whose tokens have a word, a row and a
  * column).  For every head of q (T,B,Hq,D) and k (T,B,Hk,D):
  *     y = x * rsqrt(mean(x^2) + eps) * w
- *     pair (2i, 2i+1) of y is turned by positions[t, b, axis] * base^(-j / n): the pairs 0, 1, .. go to axis 0's section of n =
- *     sections[0] pairs (j = 0 .. n-1), then to axis 1's, and so on; pairs behind all sections, and the last element of an odd
- *     D, are not turned.  Angles are formed and reduced in 64 bits.
+ *     pair (2i, 2i+1) of y is turned by the angle positions[t, b, axis] * rates[i]: the pairs 0, 1, .. go to axis 0's section of
+ *     sections[0] pairs, then to axis 1's, and so on; pairs behind all sections, and the last element of an odd D, are not
+ *     turned.  Angles are formed and reduced in 64 bits.
  *   dtype    0: fp32, 1: bf16, 2: fp16 -- of q, k, yq, yk.  1 <= D <= 256, at most 4 axes, sum of the sections <= D/2.
  *   q, k     unit stride along the last axis, any other strides; yq, yk contiguous.  Hk = 0: q alone.
  *   wq, wk   (D) in fp32 (w32 = 1) or in the type of q (0), or NULL = ones
  *   positions (T,B,axes) int64 (positions64 = 1) or int32 (0), any strides (0 over b: one for all samples)
- *   sections HOST array of `axes` ints;  strides  HOST array of 9, in elements: t, b, h of q, of k, then t, b, axis of positions
+ *   sections HOST array of `axes` ints;  rates  HOST array of their sum doubles, radians for a position step;  strides  HOST array of 9, in elements: t, b, h of q, of k, then t, b, axis of positions
  * Gradients: grad_q, grad_k contiguous; grad_wq, grad_wk (D), in the type of the weights, or NULL: summed over tokens and heads in a
  *   fixed order; strides has 6 more: t, b, h of grad_yq, of grad_yk (unit stride along the last axis);
  *   workspace: dmn_head_norm_rotary_workspace_floats(Hq, Hk, D) floats, NULL if neither weight gradient is wanted.
  */
 int dmn_head_norm_rotary_fwd(int dtype, const void *q, const void *k, const void *wq, const void *wk, int w32, const void *positions,
-                             int positions64, const int *sections, int axes, double base, float eps, void *yq, void *yk,
+                             int positions64, const int *sections, int axes, const double *rates, float eps, void *yq, void *yk,
                              const long long *strides, int T, int B, int Hq, int Hk, int D, void *stream);
 int dmn_head_norm_rotary_workspace_floats(int Hq, int Hk, int D);
 int dmn_head_norm_rotary_bwd(int dtype, const void *q, const void *k, const void *wq, const void *wk, int w32, const void *positions,
-                             int positions64, const int *sections, int axes, double base, float eps, const void *grad_yq,
+                             int positions64, const int *sections, int axes, const double *rates, float eps, const void *grad_yq,
                              const void *grad_yk, void *grad_q, void *grad_k, void *grad_wq, void *grad_wk, const long long *strides,
                              float *workspace, int T, int B, int Hq, int Hk, int D, void *stream);
 

@@ -252,18 +252,20 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     st = ops._strides([64, 64, 8] * 5)
     sec = lambda *n: (ctypes.c_int * max(len(n), 1))(*n)  # noqa: E731
 
-    def fwd(dtype=0, q=16, sections=(2,), base=100.0, T=1, B=1, Hq=1, Hk=1, D=8, pos=16, strides=st):
-        _lib.call("dmn_head_norm_rotary_fwd", dtype, q, 16, None, None, 1, pos, 1, sec(*sections), len(sections), base, 1e-6, 16, 16,
+    rates = (ctypes.c_double * 2)(1.0, 0.5)
+
+    def fwd(dtype=0, q=16, sections=(2,), rates=rates, T=1, B=1, Hq=1, Hk=1, D=8, pos=16, strides=st):
+        _lib.call("dmn_head_norm_rotary_fwd", dtype, q, 16, None, None, 1, pos, 1, sec(*sections), len(sections), rates, 1e-6, 16, 16,
                   strides, T, B, Hq, Hk, D, None)
 
     for bad, word in ((dict(dtype=3), "dtype"), (dict(T=-1), "bad sizes"), (dict(Hq=0), "bad sizes"), (dict(D=0), "widths"),
                       (dict(D=257), "widths"), (dict(sections=(3, 2)), "pairs turn"), (dict(sections=(-1, 2)), "bad section"),
-                      (dict(sections=(0,) * 5), "axes"), (dict(base=0.0), "base"), (dict(base=math.nan), "base"), (dict(q=None), "null"),
+                      (dict(sections=(0,) * 5), "axes"), (dict(rates=None), "null"), (dict(q=None), "null"),
                       (dict(pos=None), "null"), (dict(strides=None), "null")):
         with pytest.raises(RuntimeError, match=word):
             fwd(**bad)
     with pytest.raises(RuntimeError, match="workspace"):
-        _lib.call("dmn_head_norm_rotary_bwd", 0, 16, 16, 16, 16, 1, 16, 1, sec(2), 1, 100.0, 1e-6, 16, 16, 16, 16, 16, 16, st, None,
+        _lib.call("dmn_head_norm_rotary_bwd", 0, 16, 16, 16, 16, 1, 16, 1, sec(2), 1, rates, 1e-6, 16, 16, 16, 16, 16, 16, st, None,
                   1, 1, 1, 1, 8, None)
     assert lib.dmn_head_norm_rotary_workspace_floats(0, 1, 8) == -1 and lib.dmn_head_norm_rotary_workspace_floats(4, 1, 64) > 0
     x = torch.zeros(2, 1, 1, 8)
@@ -293,6 +295,7 @@ def test_refusals():
             (lambda: call(x, x, w, w, p.cpu(), (4,)), "positions must be"),
             (lambda: call(x, x, w, w, None, (4,)), "positions must be"),
             (lambda: call(x, x, w, w, p, (4,), base=0.0), "base"),
+            (lambda: call(x, x, w, w, p, (4,), base=math.nan), "base"),
             (lambda: call(x[:, :, :0], x, w, w, p, (4,)), "at least one head"),
             (lambda: call(torch.zeros(1, 1, 1, 300, device=DEV), torch.zeros(1, 1, 1, 300, device=DEV), None, None, None, ()), "width")):
         with pytest.raises(RuntimeError, match=word):
