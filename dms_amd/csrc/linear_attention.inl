@@ -915,6 +915,8 @@ template <typename T, int DK, int DV, int VEC, bool FINE, bool STATE_ONLY>
 struct Pair {
     static constexpr int C = chunk<T>(), NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
     static constexpr int NW0 = DV / 16 < 4 ? DV / 16 : 4, NW1 = DK / 16 < 4 ? DK / 16 : 4, NTHR = 64 * (NW0 + NW1);
+    // waves of a SIMD: two workgroups of 8 where tiles and scores take less than half of the LDS
+    static constexpr int RESIDENT = DK == 64 && DV == 64 ? 4 : 1;
     typedef Pass<T, DK, DV, C, NW0, NX, STATE_ONLY> P0;
     typedef Pass<T, DV, DK, C, NW1, NX, STATE_ONLY> P1;
     struct Shared {
@@ -1038,7 +1040,7 @@ struct Pair {
 };
 
 template <typename T, int DK, int DV, int VEC, bool FINE, bool STATE_ONLY>
-__global__ void __launch_bounds__((Pair<T, DK, DV, VEC, FINE, STATE_ONLY>::NTHR)) pair_kernel(const Args a)
+__global__ void __launch_bounds__((Pair<T, DK, DV, VEC, FINE, STATE_ONLY>::NTHR), (Pair<T, DK, DV, VEC, FINE, STATE_ONLY>::RESIDENT)) pair_kernel(const Args a)
 {
     typedef Pair<T, DK, DV, VEC, FINE, STATE_ONLY> K;
     __shared__ typename K::Shared sm;
