@@ -455,7 +455,7 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         t.f32 = 1;
         return t;
     };
-    const int fine = grad_g ? FINE_PASS : 0;
+    const int dots_too = grad_g ? DOTS_PASS : 0;
     Args a;
     fill_common(a, g, strides + 9, lengths, lengths64, T, B, H);
     a.nseg = p.nseg;
@@ -473,7 +473,7 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         r.scale_p = r.scale_x = scale;
         r.scale_z = 1.0f;
         r.reverse = r.last_decay = 0;
-        rc = run_passes(dtype, a, p.DV, p.DK, fine, workspace + p.one, st);
+        rc = run_passes(dtype, a, p.DV, p.DK, dots_too, workspace + p.one, st);
         if (rc) return rc;
     }
     if (grad_k || grad_v || grad_g || grad_state0) {
@@ -496,7 +496,7 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         rk.in_c = rk.out_c = 1;
         rk.in_z = rk.out_z = dv;
         rk.dots = grad_g ? dots + (size_t)T * B * H : nullptr;
-        rc = run_passes(dtype, a, p.DK, p.DV, fine | PAIR, workspace + p.pair, st);
+        rc = run_passes(dtype, a, p.DK, p.DV, dots_too | PAIR, workspace + p.pair, st);
         if (rc) return rc;
     }
     if (grad_g) {

@@ -21,6 +21,8 @@
 #pragma once
 #include "linear_attention.h"
 
+#include <type_traits>
+
 namespace dmn {
 namespace la {
 
@@ -245,6 +247,17 @@ struct Tile {
     }
 };
 
+// four adjacent elements of an LDS tile
+template <typename T, int D, int C>
+__device__ __forceinline__ f32x4 tile_value(const __bf16 *tile, int row, int col)
+{
+    f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = Kind<T>::NP - 1; k >= 0; --k)
+        x += __builtin_convertvector(*reinterpret_cast<const b16x4 *>(tile + k * C * D + at<D>(row, col)), f32x4);
+    return x;
+}
+
 // The decays of a chunk, in the order in which its rows are walked (row r is token r, or C - 1 - r where time runs backwards)
 template <int C>
 struct alignas(16) Decays {
@@ -353,35 +366,39 @@ struct Rows {
             }
         }
     }
-    __device__ __forceinline__ f32x4 load4(__amdgpu_buffer_rsrc_t rs, int n_rows, int I, int n) const
+    // as it lies in memory; value() makes numbers of it, later
+    typedef typename std::conditional<sizeof(T) == 4, u32x4, u32x2>::type Raw;
+    __device__ __forceinline__ Raw load4(__amdgpu_buffer_rsrc_t rs, int n_rows, int I, int n) const
     {
         const bool ok = row + I * row16 < n_rows;
         const unsigned o = off + I * row_step + 16 * n * es;
         const int left = cols - 16 * n;
-        f32x4 x;
         if constexpr (sizeof(T) == 4) {
-            if (VEC == 2) {
-                x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, ok && 0 < left ? o : NOWHERE, 0, 0));
-            } else {
+            if (VEC == 2) return __builtin_amdgcn_raw_buffer_load_b128(rs, ok && 0 < left ? o : NOWHERE, 0, 0);
+            Raw x;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, ok && i < left ? o + 4 * i : NOWHERE, 0, 0));
+            for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, ok && i < left ? o + 4 * i : NOWHERE, 0, 0);
+            return x;
+        } else {
+            if (VEC >= 1) return __builtin_amdgcn_raw_buffer_load_b64(rs, ok && 0 < left ? o : NOWHERE, 0, 0);
+            Raw x;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const unsigned lo = __builtin_amdgcn_raw_buffer_load_b16(rs, ok && 2 * i < left ? o + 4 * i : NOWHERE, 0, 0);
+                const unsigned hi = __builtin_amdgcn_raw_buffer_load_b16(rs, ok && 2 * i + 1 < left ? o + 4 * i + 2 : NOWHERE, 0, 0);
+                x[i] = lo | hi << 16;
             }
+            return x;
+        }
+    }
+    static __device__ __forceinline__ f32x4 value(const Raw &x)
+    {
+        if constexpr (sizeof(T) == 4) {
+            return __builtin_bit_cast(f32x4, x);
         } else {
             typedef T tx4 __attribute__((ext_vector_type(4)));
-            typedef unsigned short hx4 __attribute__((ext_vector_type(4)));
-            tx4 y;
-            if (VEC >= 1) {
-                y = __builtin_bit_cast(tx4, __builtin_amdgcn_raw_buffer_load_b64(rs, ok && 0 < left ? o : NOWHERE, 0, 0));
-            } else {
-                hx4 e;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, ok && i < left ? o + 2 * i : NOWHERE, 0, 0);
-                y = __builtin_bit_cast(tx4, e);
-            }
-            x = __builtin_convertvector(y, f32x4);
+            return __builtin_convertvector(__builtin_bit_cast(tx4, x), f32x4);
         }
-        return x;
     }
 };
 
@@ -389,7 +406,7 @@ struct Rows {
 template <typename T, int DC, int DZ, int C, int NW, int NX, bool STATE_ONLY>
 struct Pass {
     static constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC;
-    static constexpr int NT = DZ / 16 / NW, CT = C / 16, KT = DC / 16;     // tiles of 16: a wave's columns, tokens, rows of S
+    static constexpr int DZ_ = DZ, NT = DZ / 16 / NW, CT = C / 16, KT = DC / 16;     // tiles of 16: a wave's columns, tokens, rows of S
     f32x4 S[KT][NT];
     f32x4 O[STATE_ONLY ? 1 : CT][NT];
 
@@ -650,32 +667,33 @@ struct Pass {
             }
     }
 
-    // rows of o: row r is token t0 + r, or t0 + C - 1 - r where time runs backwards; valid ones lie before token `len`
+    // rows of o to memory from the owners' registers: row r is token t0 + r, or t0 + C - 1 - r where time runs backwards
     template <int VEC>
-    __device__ __forceinline__ void store_rows(const Rows<T, C, VEC> &o, const Rows<T, C, VEC> &w, bool rows_wanted, bool dot_wanted, int t0, int len, int lg, float *dots)
+    __device__ __forceinline__ void store_rows(const Rows<T, C, VEC> &o, int t0, int len) const
     {
-        if (rows_wanted) {
-            const __amdgpu_buffer_rsrc_t rs = buffer(o.p + (long long)t0 * o.st);
+        const __amdgpu_buffer_rsrc_t rs = buffer(o.p + (long long)t0 * o.st);
 #pragma unroll
-            for (int I = 0; I < CT; ++I)
+        for (int I = 0; I < CT; ++I)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) o.store4(rs, len - t0, I, n, O[I][n]);
-        }
-        if (dot_wanted) {
-            const __amdgpu_buffer_rsrc_t rs = buffer(w.p + (long long)t0 * w.st);
+            for (int n = 0; n < NT; ++n) o.store4(rs, len - t0, I, n, O[I][n]);
+    }
+
+    // a wave's share of sum_c W[t, c] o[t, c]: f(I, n) gives W's four numbers; dots[] goes by the token
+    template <typename F>
+    __device__ __forceinline__ void dot_rows(float *dots, int reverse, int lr, int lg, F f) const
+    {
 #pragma unroll
-            for (int I = 0; I < CT; ++I) {
-                float dot = 0.0f;
+        for (int I = 0; I < CT; ++I) {
+            float dot = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const f32x4 x = w.load4(rs, len - t0, I, n);
+            for (int n = 0; n < NT; ++n) {
+                const f32x4 x = f(I, n);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) dot += x[i] * O[I][n][i];
-                }
-                dot += __shfl_xor(dot, 16);
-                dot += __shfl_xor(dot, 32);
-                if (lg == 0) dots[w.row + I * w.row16] = dot;
+                for (int i = 0; i < 4; ++i) dot += x[i] * O[I][n][i];
             }
+            dot += __shfl_xor(dot, 16);
+            dot += __shfl_xor(dot, 32);
+            if (lg == 0) dots[reverse ? C - 1 - I * 16 - lr : I * 16 + lr] = dot;
         }
     }
 };
@@ -785,11 +803,12 @@ template <typename T, int DC, int DZ> constexpr int residents()
     return waves / 4 * (waves == 8 && tiles <= 80 * 1024 ? 2 : 1);
 }
 
-template <typename T, int DC, int DZ, int VEC, bool FINE>
+// DOTS: the sums of W o as well, and x S to 24 bits for them.
+template <typename T, int DC, int DZ, int VEC, bool DOTS>
 __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ>())) chunk_kernel(const Args a)
 {
     constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<T, DZ>(), NTHR = 64 * (NO + NF);
-    constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
+    constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = DOTS ? 3 : NC;
     constexpr bool WHOLE = DC == DZ;                 // rows of o fit x's tile
     constexpr int AHEAD = DC <= 64 && DZ <= 64 ? 2 : 1;   // chunks of rows in flight: with 128 columns one is as many bytes, and registers are short
     typedef Pass<T, DC, DZ, C, NO, NX, false> P;
@@ -824,7 +843,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
             float g;
         } even, odd;                                     // the chunks of either parity from c0 on
         const long long gt = held(a.gt), o_st = held(ro.O.st * (long long)sizeof(T));
-        const char *const o = held(WHOLE && ro.O.p && !ro.O.f32 ? ro.O.p + ((long long)w.b * ro.O.sb + (long long)w.h * ro.O.sh) * (long long)sizeof(T) : nullptr);
+        const char *const o = held(WHOLE && ro.O.p && (sizeof(T) == 4 || !ro.O.f32) ? ro.O.p + ((long long)w.b * ro.O.sb + (long long)w.h * ro.O.sh) * (long long)sizeof(T) : nullptr);
         tx.ocol = ro.O.d - (ft % tx.PER) * tx.UE;
         const float scale_p = held(ro.scale_p), scale_x = held(ro.scale_x), scale_z = held(ro.scale_z);
         const auto fetch_xy = [&](int ci, Chunk &f) __attribute__((always_inline)) {
@@ -845,7 +864,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         const auto flush = [&](int ci) __attribute__((always_inline)) {
             if (o) tx.drain(sm.x[ci & 1], ft, o + token0(ci) * o_st, o_st, len - token0(ci));
             const int t = token0(ci) + ft;
-            if (dots && ft < C && t < len) {
+            if (DOTS && ft < C && t < len) {
                 float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NO; ++i) s += sm.dots[i][ft];
@@ -880,7 +899,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         if (c0 < c1) flush(c1 - 1);
     } else {
         const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
-        const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(ro.W, w.b, w.h, reverse, lr, z0 + 4 * lg);
+        const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(DOTS ? ro.W : ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg);
         P ps;
         ps.zero();
         if (w.seg == 0) {
@@ -895,11 +914,22 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         }
         for (int ci = c0; ci < c1; ++ci) {
             const Decays<C> &d = sm.d[ci & 1];
+            const int t0 = token0(ci);
+            typename Rows<T, C, VEC>::Raw wf[DOTS ? P::CT : 1][P::NT];
+            if constexpr (DOTS) {                            // on their way while o is computed
+                const __amdgpu_buffer_rsrc_t rs = buffer(wrows.p + (long long)t0 * wrows.st);
+#pragma unroll
+                for (int I = 0; I < P::CT; ++I)
+#pragma unroll
+                    for (int n = 0; n < P::NT; ++n) wf[I][n] = wrows.load4(rs, len - t0, I, n);
+            }
             ps.from_state(sm.x[ci & 1], d, lr, lg);
             __syncthreads();
             ps.from_chunk(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
             if (WHOLE && !out.f32) ps.lay_rows(sm.x[ci & 1], z0, lr, lg);
-            ps.store_rows(out, wrows, out.p && !(WHOLE && !out.f32), dots != nullptr, token0(ci), len, lg, sm.dots[wave]);
+            else if (out.p) ps.store_rows(out, t0, len);
+            if constexpr (DOTS)
+                ps.dot_rows(sm.dots[wave], reverse, lr, lg, [&](int I, int n) __attribute__((always_inline)) { return Rows<T, C, VEC>::value(wf[I][n]); });
             __syncthreads();
         }
         if (ro.s_out && w.seg == a.nseg - 1)
@@ -911,9 +941,9 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
 
 // The two passes of the backward that run against time, dv and dk, in one workgroup: they read the same four tensors, each
 // into one tile, and walk the same decays.  Waves 0 .. do dv (x = k, y = q, z = dO), the others dk (x = v, y = dO, z = q).
-template <typename T, int DK, int DV, int VEC, bool FINE, bool STATE_ONLY>
+template <typename T, int DK, int DV, int VEC, bool DOTS, bool STATE_ONLY>
 struct Pair {
-    static constexpr int C = chunk<T>(), NP = Kind<T>::NP, NC = Kind<T>::NC, NX = FINE ? 3 : NC;
+    static constexpr int C = chunk<T>(), NP = Kind<T>::NP, NC = Kind<T>::NC, NX = DOTS ? 3 : NC;
     static constexpr int NW0 = DV / 16 < 4 ? DV / 16 : 4, NW1 = DK / 16 < 4 ? DK / 16 : 4, NTHR = 64 * (NW0 + NW1);
     // waves of a SIMD: two workgroups of 8 where tiles and scores take less than half of the LDS
     static constexpr int RESIDENT = DK == 64 && DV == 64 ? 4 : 1;
@@ -945,7 +975,12 @@ struct Pair {
         const __bf16 *x = gr ? sm.v : sm.k, *y = gr ? sm.o : sm.q, *z = gr ? sm.q : sm.o;
         __bf16 *const p = sm.p[gr];
 
-        const Rows<T, C, VEC> out(ro.O, b, h, 1, lr, z0 + 4 * lg), wrows(ro.W, b, h, 1, lr, z0 + 4 * lg);
+        const Rows<T, C, VEC> out(ro.O, b, h, 1, lr, z0 + 4 * lg);
+        const auto row_base = [&](const Tensor &t) {
+            return held(t.p && (sizeof(T) == 4 || !t.f32) ? t.p + ((long long)b * t.sb + (long long)h * t.sh) * (long long)sizeof(T) : nullptr);
+        };
+        const char *const ov = row_base(r0.O), *const ok = row_base(r1.O);
+        const long long ov_st = held(r0.O.st * (long long)sizeof(T)), ok_st = held(r1.O.st * (long long)sizeof(T));
         P ps;
         ps.zero();
         const size_t slot = ((size_t)(gr * BH + bh) * a.nseg + seg) * (DK * DV);
@@ -964,6 +999,8 @@ struct Pair {
         if (!STATE_ONLY) {
             tk.init(r0.X, b, h, tid, 1);
             tv.init(r1.X, b, h, tid, 1);
+            tk.ocol = r1.O.d - (tid % tk.PER) * tk.UE;
+            tv.ocol = r0.O.d - (tid % tv.PER) * tv.UE;
         }
         float g = 0.0f;
         double gsum = 0.0;
@@ -977,9 +1014,11 @@ struct Pair {
             }
         };
         const auto fetch_g = [&](int ci) { g = fetch_decay<C>(pg, a.gt, token0(ci), len, 1, lane); };
-        const auto flush_dots = [&](int ci) {
-            const int t = token0(ci) + tid;
-            if (tid < C && t < len) {
+        const auto flush = [&](int ci) {
+            const int t0 = token0(ci), t = t0 + tid;
+            if (ov) tv.drain(sm.v, tid, ov + t0 * ov_st, ov_st, len - t0);
+            if (ok) tk.drain(sm.k, tid, ok + t0 * ok_st, ok_st, len - t0);
+            if (DOTS && tid < C && t < len) {
                 float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NW1; ++i) s += sm.dots[i][tid];
@@ -996,7 +1035,7 @@ struct Pair {
         for (int ci = c0; ci < c1; ++ci) {
             const Decays<C> &d = sm.d[ci & 1];
             __syncthreads();                              // nobody reads the last chunk's tiles any more
-            if (!STATE_ONLY && r1.dots && ci > c0) flush_dots(ci - 1);
+            if (!STATE_ONLY && ci > c0) flush(ci - 1);
             tq.store(fq, sm.q, tid);
             to.store(fo, sm.o, tid);
             if (!STATE_ONLY) {
@@ -1014,7 +1053,15 @@ struct Pair {
                 __syncthreads();                          // the scores are whole
             }
             ps.from_chunk(y, z, p, d, z0, lr, lg);
-            if (!STATE_ONLY) ps.store_rows(out, wrows, out.p, gr && r1.dots, token0(ci), len, lg, sm.dots[gr ? wave : 0]);
+            if constexpr (!STATE_ONLY) {
+                // k's tile and v's are read no more: dk and dv into them, for whole rows to memory.  A lane reads k, for its dots, where it
+                // puts dk.
+                if constexpr (DOTS && GROUP != 0) {
+                    if (gr) ps.dot_rows(sm.dots[wave], 1, lr, lg, [&](int I, int n) __attribute__((always_inline)) { return tile_value<T, P::DZ_, C>(sm.k, I * 16 + lr, z0 + 16 * n + 4 * lg); });
+                }
+                if (!out.f32) ps.lay_rows(gr ? sm.k : sm.v, z0, lr, lg);
+                else if (out.p) ps.store_rows(out, token0(ci), len);
+            }
             if (clock && ci + 1 < c1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[(ci + 1) & 1]);
         }
         if (STATE_ONLY) {
@@ -1026,9 +1073,9 @@ struct Pair {
             }
             return;
         }
-        if (r1.dots && c0 < c1) {
+        if (c0 < c1) {
             __syncthreads();
-            flush_dots(c1 - 1);
+            flush(c1 - 1);
         }
         const int first = c0 * C, behind = min(a.T, (c0 + a.seg_chunks) * C);
         zero_rows<T>(r0, len, first, behind, b, h, tid, NTHR);
@@ -1039,10 +1086,10 @@ struct Pair {
     }
 };
 
-template <typename T, int DK, int DV, int VEC, bool FINE, bool STATE_ONLY>
-__global__ void __launch_bounds__((Pair<T, DK, DV, VEC, FINE, STATE_ONLY>::NTHR), (Pair<T, DK, DV, VEC, FINE, STATE_ONLY>::RESIDENT)) pair_kernel(const Args a)
+template <typename T, int DK, int DV, int VEC, bool DOTS, bool STATE_ONLY>
+__global__ void __launch_bounds__((Pair<T, DK, DV, VEC, DOTS, STATE_ONLY>::NTHR), (Pair<T, DK, DV, VEC, DOTS, STATE_ONLY>::RESIDENT)) pair_kernel(const Args a)
 {
-    typedef Pair<T, DK, DV, VEC, FINE, STATE_ONLY> K;
+    typedef Pair<T, DK, DV, VEC, DOTS, STATE_ONLY> K;
     __shared__ typename K::Shared sm;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wave >= K::NW0, w = group ? wave - K::NW0 : wave;
@@ -1058,16 +1105,15 @@ template <typename T, int DC, int DZ, int VEC>
 static int launch_one(const Args &a, int kind, hipStream_t stream)
 {
     const unsigned grid = (unsigned)((size_t)a.B * a.H * a.nseg * (kind & PAIR ? 1 : a.nroles));
-    const bool fine = Kind<T>::NC < 3 && (kind & FINE_PASS);
     if (kind & PAIR) {
         constexpr int n = Pair<T, DC, DZ, VEC, false, true>::NTHR;
         if (kind & STATES) pair_kernel<T, DC, DZ, VEC, false, true><<<grid, n, 0, stream>>>(a);
-        else if (fine) pair_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3, false><<<grid, n, 0, stream>>>(a);
+        else if (kind & DOTS_PASS) pair_kernel<T, DC, DZ, VEC, true, false><<<grid, n, 0, stream>>>(a);
         else pair_kernel<T, DC, DZ, VEC, false, false><<<grid, n, 0, stream>>>(a);
     } else {
         constexpr int n = 64 * (owners<T, DZ>() + feeders<T, DZ>());
         if (kind & STATES) state_kernel<T, DC, DZ, VEC><<<grid, 64 * owners<T, DZ>(), 0, stream>>>(a);
-        else if (fine) chunk_kernel<T, DC, DZ, VEC, Kind<T>::NC < 3><<<grid, n, 0, stream>>>(a);
+        else if (kind & DOTS_PASS) chunk_kernel<T, DC, DZ, VEC, true><<<grid, n, 0, stream>>>(a);
         else chunk_kernel<T, DC, DZ, VEC, false><<<grid, n, 0, stream>>>(a);
     }
     return launch_status("linear_attention");

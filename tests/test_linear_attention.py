@@ -113,6 +113,8 @@ CASES = [
     ("bf16", 257, 3, 1, 70, 40, dict(Hq=1, ragged=True, fixed=True)),
     ("fp32", 320, 1, 2, 100, 100, dict(state=True)),
     ("fp16", 200, 2, 2, 32, 17, dict(ragged=True, state=True, resets=(7,))),
+    ("fp32", 70, 2, 4, 64, 64, dict(Hq=2, Hk=1, Hv=2)),
+    ("bf16", 140, 1, 4, 64, 100, dict(Hq=1, Hv=2, state=True)),
 ]
 
 
