@@ -53,6 +53,34 @@ __device__ __forceinline__ double log2_decay(float g)
     return v < -160.0 ? -160.0 : v;
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double shifted(double v)
+{
+    const unsigned long long x = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+__device__ __forceinline__ double lane_value(double v, int lane)
+{
+    const unsigned long long x = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+// inclusive sums over the 64 lanes
+__device__ __forceinline__ double lane_sums(double v)
+{
+    v += shifted<0x111, 0xf>(v);                   // row_shr 1, 2, 4, 8: of 16 lanes
+    v += shifted<0x112, 0xf>(v);
+    v += shifted<0x114, 0xf>(v);
+    v += shifted<0x118, 0xf>(v);
+    v += shifted<0x142, 0xa>(v);                   // row_bcast 15, 31: of 64
+    v += shifted<0x143, 0xc>(v);
+    return v;
+}
+
 constexpr int DTYPE_F32 = 0, DTYPE_BF16 = 1, DTYPE_F16 = 2;
 inline int elem_size(int dtype) { return dtype == DTYPE_F32 ? 4 : 2; }
 // tokens of a chunk: see linear_attention.inl

@@ -267,22 +267,6 @@ struct alignas(16) Decays {
     float tot;                 // 2^{G_C}
 };
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double shifted(double v)
-{
-    const unsigned long long x = __builtin_bit_cast(unsigned long long, v);
-    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
-    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
-    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
-}
-
-__device__ __forceinline__ double lane_value(double v, int lane)
-{
-    const unsigned long long x = __builtin_bit_cast(unsigned long long, v);
-    const unsigned lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
-    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
-}
-
 // the log decay of a lane's step: of its token, or backwards of the token after it
 template <int C>
 __device__ __forceinline__ float fetch_decay(const float *pg, long long gt, int t0, int len, int reverse, int lane)
@@ -295,13 +279,7 @@ __device__ __forceinline__ float fetch_decay(const float *pg, long long gt, int 
 template <int C>
 __device__ __forceinline__ double decays(float g, int lane, float scale_x, float scale_z, Decays<C> &d)
 {
-    double G = log2_decay(g);
-    G += shifted<0x111, 0xf>(G);                   // row_shr 1, 2, 4, 8: inclusive sums of 16 lanes
-    G += shifted<0x112, 0xf>(G);
-    G += shifted<0x114, 0xf>(G);
-    G += shifted<0x118, 0xf>(G);
-    G += shifted<0x142, 0xa>(G);                   // row_bcast 15, 31: of 64
-    if (C > 32) G += shifted<0x143, 0xc>(G);
+    const double G = lane_sums(log2_decay(g));
     const double tot = lane_value(G, C - 1);
     const double ends[4] = {lane_value(G, 15), lane_value(G, 31), lane_value(G, C > 32 ? 47 : 15), lane_value(G, C > 32 ? 63 : 15)};
     const double end = lane < 16 ? ends[0] : lane < 32 ? ends[1] : lane < 48 ? ends[2] : ends[3];
