@@ -28,7 +28,7 @@ struct Role {
 };
 
 struct Args {
-    Role role[2];
+    Role role[3];
     const float *g;
     long long gt, gb, gh;
     const void *lengths;
@@ -88,8 +88,7 @@ inline int chunk_tokens(int dtype) { return dtype == DTYPE_BF16 ? 64 : 32; }
 
 // kind, bits:
 constexpr int STATES = 1;      // the states after each segment (from s_in for segment 0, from zero for the others), nothing else
-constexpr int PAIR = 2;        // role[0] and role[1] are dv and dk: one workgroup does both
-constexpr int DOTS_PASS = 4;   // the dots of W and o as well (of a pair: of role[1]), and x S to 24 bits, as they are summed over the sequence
+constexpr int DOTS_PASS = 2;   // the dots of W and o as well where a role wants them, and x S to 24 bits, as they are summed over the sequence
 // DC, DZ (of role[0]) in {32/32, 64/64, 64/128, 128/64, 128/128}.  Returns launch_status.
 template <typename T> int launch_chunks(const Args &a, int DC, int DZ, int kind, hipStream_t stream);
 extern template int launch_chunks<float>(const Args &, int, int, int, hipStream_t);

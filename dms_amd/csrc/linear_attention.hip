@@ -331,8 +331,8 @@ static void fill_common(Args &a, const float *g, const long long *gs, const void
 
 // the backward's passes: where each one's piece of the workspace begins
 struct BwdPlan {
-    int DK, DV, nseg, seg_chunks;
-    long long one, pair, dots, dq, dk, dv, ds0, part, total;
+    int DK, DV;
+    long long passes, dots, dq, dk, dv, ds0, part, total;
 };
 
 static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)
@@ -340,11 +340,15 @@ static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, 
     BwdPlan p;
     pad_pair(dk, dv, &p.DK, &p.DV);
     const long long BH = (long long)B * H, rows = (long long)T * BH;
-    plan_segments(dtype, T, BH, &p.nseg, &p.seg_chunks);
-    long long at = 0;
+    long long at = 0, most = 0;
+    for (int n = 1; n <= 3; ++n) {                         // roles of a launch: fewer are cut into more segments
+        int nseg, seg_chunks;
+        plan_segments(dtype, T, n * BH, &nseg, &seg_chunks);
+        const long long f = passes_floats(n, BH, nseg, p.DK, p.DV);
+        most = f > most ? f : most;
+    }
     const auto take = [&at](long long n) { const long long o = at; at += up4(n); return o; };
-    p.one = take(passes_floats(1, BH, p.nseg, p.DK, p.DV));
-    p.pair = take(passes_floats(2, BH, p.nseg, p.DK, p.DV));
+    p.passes = take(most);                                 // of two launches the second begins when the first is done with it
     p.dots = take(2 * rows);
     p.dq = take(Hq < H ? rows * dk : 0);
     p.dk = take(Hk < H ? rows * dk : 0);
@@ -477,14 +481,10 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         t.f32 = 1;
         return t;
     };
-    const int dots_too = grad_g ? DOTS_PASS : 0;
-    Args a;
-    fill_common(a, g, strides + 9, lengths, lengths64, T, B, H);
-    a.nseg = p.nseg;
-    a.seg_chunks = p.seg_chunks;
+    Role role[3];
+    int n = 0;
     if (grad_q || grad_g) {                               // dq: the operator on (dO, v, k)
-        a.nroles = 1;
-        Role &r = a.role[0];
+        Role &r = role[n++];
         r.X = D; r.Y = V; r.Z = K; r.W = Q;
         r.O = output(grad_q, workspace + p.dq, Hq, dk);
         r.s_in = state0;
@@ -495,30 +495,51 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         r.scale_p = r.scale_x = scale;
         r.scale_z = 1.0f;
         r.reverse = r.last_decay = 0;
-        rc = run_passes(dtype, a, p.DV, p.DK, dots_too, workspace + p.one, st);
-        if (rc) return rc;
     }
-    if (grad_k || grad_v || grad_g || grad_state0) {
-        a.nroles = 2;
-        Role &rv = a.role[0], &rk = a.role[1];
-        rv.X = K; rv.Y = Q; rv.Z = D; rv.W = V;           // dv and dS_0: backwards in time, on (k, q, dO)
-        rv.O = output(grad_v, workspace + p.dv, Hv, dv);
-        rv.s_in = grad_state;
-        rv.s_out = need_ds0 ? ds0 : nullptr;
-        rv.in_c = rv.out_c = dv;
-        rv.in_z = rv.out_z = 1;
-        rv.dots = nullptr;
-        rv.scale_p = rv.scale_z = scale;
-        rv.scale_x = 1.0f;
-        rv.reverse = rv.last_decay = 1;
-        rk = rv;
-        rk.X = V; rk.Y = D; rk.Z = Q; rk.W = K;           // dk: the same on (v, dO, q), with the states transposed
-        rk.O = output(grad_k, workspace + p.dk, Hk, dk);
-        rk.s_out = nullptr;
-        rk.in_c = rk.out_c = 1;
-        rk.in_z = rk.out_z = dv;
-        rk.dots = grad_g ? dots + (size_t)T * B * H : nullptr;
-        rc = run_passes(dtype, a, p.DK, p.DV, dots_too | PAIR, workspace + p.pair, st);
+    if (grad_k || grad_g) {                               // dk: backwards in time, on (v, dO, q)
+        Role &r = role[n++];
+        r.X = V; r.Y = D; r.Z = Q; r.W = K;
+        r.O = output(grad_k, workspace + p.dk, Hk, dk);
+        r.s_in = grad_state;
+        r.s_out = nullptr;
+        r.in_c = r.out_c = 1;
+        r.in_z = r.out_z = dv;
+        r.dots = grad_g ? dots + (size_t)T * B * H : nullptr;
+        r.scale_p = r.scale_z = scale;
+        r.scale_x = 1.0f;
+        r.reverse = 1;
+        r.last_decay = 0;
+    }
+    const int first = n;
+    if (grad_v || need_ds0) {                             // dv and dS_0: backwards in time, on (k, q, dO)
+        Role &r = role[n++];
+        r.X = K; r.Y = Q; r.Z = D; r.W = V;
+        r.O = output(grad_v, workspace + p.dv, Hv, dv);
+        r.s_in = grad_state;
+        r.s_out = need_ds0 ? ds0 : nullptr;
+        r.in_c = r.out_c = dv;
+        r.in_z = r.out_z = 1;
+        r.dots = nullptr;
+        r.scale_p = r.scale_z = scale;
+        r.scale_x = 1.0f;
+        r.reverse = r.last_decay = 1;
+    }
+    Args a;
+    fill_common(a, g, strides + 9, lengths, lengths64, T, B, H);
+    const auto passes = [&](int from, int to, int DC, int DZ, int kind) {
+        a.nroles = to - from;
+        for (int i = from; i < to; ++i) a.role[i - from] = role[i];
+        plan_segments(dtype, T, (long long)a.nroles * B * H, &a.nseg, &a.seg_chunks);
+        return from < to ? run_passes(dtype, a, DC, DZ, kind, workspace + p.passes, st) : 0;
+    };
+    const int dots_too = grad_g ? DOTS_PASS : 0;
+    if (p.DK == p.DV) {                                   // all in one launch where keys and values are padded alike
+        rc = passes(0, n, p.DV, p.DK, dots_too);
+        if (rc) return rc;
+    } else {
+        rc = passes(0, first, p.DV, p.DK, dots_too);
+        if (rc) return rc;
+        rc = passes(first, n, p.DK, p.DV, 0);
         if (rc) return rc;
     }
     if (grad_g) {

@@ -247,17 +247,6 @@ struct Tile {
     }
 };
 
-// four adjacent elements of an LDS tile
-template <typename T, int D, int C>
-__device__ __forceinline__ f32x4 tile_value(const __bf16 *tile, int row, int col)
-{
-    f32x4 x = {0, 0, 0, 0};
-#pragma unroll
-    for (int k = Kind<T>::NP - 1; k >= 0; --k)
-        x += __builtin_convertvector(*reinterpret_cast<const b16x4 *>(tile + k * C * D + at<D>(row, col)), f32x4);
-    return x;
-}
-
 // The decays of a chunk, in the order in which its rows are walked (row r is token r, or C - 1 - r where time runs backwards)
 template <int C>
 struct alignas(16) Decays {
@@ -384,7 +373,7 @@ struct Rows {
 template <typename T, int DC, int DZ, int C, int NW, int NX, bool STATE_ONLY>
 struct Pass {
     static constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC;
-    static constexpr int DZ_ = DZ, NT = DZ / 16 / NW, CT = C / 16, KT = DC / 16;     // tiles of 16: a wave's columns, tokens, rows of S
+    static constexpr int NT = DZ / 16 / NW, CT = C / 16, KT = DC / 16;     // tiles of 16: a wave's columns, tokens, rows of S
     f32x4 S[KT][NT];
     f32x4 O[STATE_ONLY ? 1 : CT][NT];
 
@@ -700,12 +689,14 @@ template <int C>
 struct Place {
     int bh, seg, ri, b, h, len, live, c0, c1;
 
-    __device__ __forceinline__ Place(const Args &a, int passes)
+    // The roles of a head sit 8 blocks apart: on the same XCD and started together, so that what they all read comes once from memory.
+    __device__ __forceinline__ Place(const Args &a)
     {
-        const int BH = a.B * a.H, rest = blockIdx.x / BH;
-        bh = blockIdx.x % BH;
-        seg = rest % a.nseg;
-        ri = passes > 1 ? rest / a.nseg : 0;
+        const int BH = a.B * a.H, per = BH * a.nroles, in = blockIdx.x % per;
+        seg = blockIdx.x / per;
+        const int eight = in / (8 * a.nroles), left = in % (8 * a.nroles), wide = min(8, BH - 8 * eight);
+        ri = left / wide;
+        bh = 8 * eight + left % wide;
         b = bh / a.H;
         h = bh % a.H;
         len = __builtin_amdgcn_readfirstlane(valid_length(a.lengths, a.lengths64, b, a.T));
@@ -728,7 +719,7 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
     };
     __shared__ Shared sm;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-    const Place<C> w(a, a.nroles);
+    const Place<C> w(a);
     if (w.seg == a.nseg - 1) return;
     const Role &ro = a.role[w.ri];
     const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT, BH = a.B * a.H;
@@ -773,17 +764,18 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
 // so that z alone needs one tile and the owners never wait for the feeders' loads or exponentials.  In phase 2 the owners leave o in the
 // x tile that nobody reads any more, and the feeders write whole rows of it (the owners' own columns are 32-byte pieces,
 // and cost the memory twice as much).
-// Waves of a SIMD that the LDS leaves room for: two workgroups of 8 where the tiles take less than half of it.
-template <typename T, int DC, int DZ> constexpr int residents()
+// Waves of a SIMD that the LDS leaves room for: two workgroups of 8 where the tiles take less than half of it (rows that are
+// fetched element by element need the registers more).
+template <typename T, int DC, int DZ, int VEC> constexpr int residents()
 {
     const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * Kind<T>::NC * chunk<T>() * chunk<T>() * 2 + 6 * 1024;
     const int waves = owners<T, DZ>() + feeders<T, DZ>();
-    return waves / 4 * (waves == 8 && tiles <= 80 * 1024 ? 2 : 1);
+    return waves / 4 * (VEC && waves == 8 && tiles <= 80 * 1024 ? 2 : 1);
 }
 
 // DOTS: the sums of W o as well, and x S to 24 bits for them.
 template <typename T, int DC, int DZ, int VEC, bool DOTS>
-__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ>())) chunk_kernel(const Args a)
+__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ, VEC>())) chunk_kernel(const Args a)
 {
     constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<T, DZ>(), NTHR = 64 * (NO + NF);
     constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = DOTS ? 3 : NC;
@@ -801,7 +793,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
     __shared__ Shared sm;
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-    const Place<C> w(a, a.nroles);
+    const Place<C> w(a);
     const Role &ro = a.role[w.ri];
     const int c0 = held(w.c0), c1 = held(w.c1), len = w.len, live = held(w.live), reverse = held(ro.reverse);
     const float *pg = held(a.g + w.b * a.gb + w.h * a.gh);
@@ -842,7 +834,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         const auto flush = [&](int ci) __attribute__((always_inline)) {
             if (o) tx.drain(sm.x[ci & 1], ft, o + token0(ci) * o_st, o_st, len - token0(ci));
             const int t = token0(ci) + ft;
-            if (DOTS && ft < C && t < len) {
+            if (DOTS && dots && ft < C && t < len) {
                 float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NO; ++i) s += sm.dots[i][ft];
@@ -877,7 +869,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         if (c0 < c1) flush(c1 - 1);
     } else {
         const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
-        const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(DOTS ? ro.W : ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg);
+        const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(DOTS && dots ? ro.W : ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg);
         P ps;
         ps.zero();
         if (w.seg == 0) {
@@ -894,19 +886,19 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
             const Decays<C> &d = sm.d[ci & 1];
             const int t0 = token0(ci);
             typename Rows<T, C, VEC>::Raw wf[DOTS ? P::CT : 1][P::NT];
-            if constexpr (DOTS) {                            // on their way while o is computed
+            if (DOTS && dots) {                              // on their way while o is computed
                 const __amdgpu_buffer_rsrc_t rs = buffer(wrows.p + (long long)t0 * wrows.st);
 #pragma unroll
                 for (int I = 0; I < P::CT; ++I)
 #pragma unroll
                     for (int n = 0; n < P::NT; ++n) wf[I][n] = wrows.load4(rs, len - t0, I, n);
             }
-            ps.from_state(sm.x[ci & 1], d, lr, lg);
+            if (z0 < dz) ps.from_state(sm.x[ci & 1], d, lr, lg);
             __syncthreads();
-            ps.from_chunk(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
+            if (z0 < dz) ps.from_chunk(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
             if (WHOLE && !out.f32) ps.lay_rows(sm.x[ci & 1], z0, lr, lg);
             else if (out.p) ps.store_rows(out, t0, len);
-            if constexpr (DOTS)
+            if (DOTS && dots)
                 ps.dot_rows(sm.dots[wave], reverse, lr, lg, [&](int I, int n) __attribute__((always_inline)) { return Rows<T, C, VEC>::value(wf[I][n]); });
             __syncthreads();
         }
@@ -917,183 +909,14 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
     zero_rows<T>(ro, len, c0 * C, min(a.T, (c0 + a.seg_chunks) * C), w.b, w.h, tid, NTHR);
 }
 
-// The two passes of the backward that run against time, dv and dk, in one workgroup: they read the same four tensors, each
-// into one tile, and walk the same decays.  Waves 0 .. do dv (x = k, y = q, z = dO), the others dk (x = v, y = dO, z = q).
-template <typename T, int DK, int DV, int VEC, bool DOTS, bool STATE_ONLY>
-struct Pair {
-    static constexpr int C = chunk<T>(), NP = Kind<T>::NP, NC = Kind<T>::NC, NX = DOTS ? 3 : NC;
-    static constexpr int NW0 = DV / 16 < 4 ? DV / 16 : 4, NW1 = DK / 16 < 4 ? DK / 16 : 4, NTHR = 64 * (NW0 + NW1);
-    // waves of a SIMD: two workgroups of 8 where tiles and scores take less than half of the LDS
-    static constexpr int RESIDENT = DK == 64 && DV == 64 ? 4 : 1;
-    typedef Pass<T, DK, DV, C, NW0, NX, STATE_ONLY> P0;
-    typedef Pass<T, DV, DK, C, NW1, NX, STATE_ONLY> P1;
-    struct Shared {
-        alignas(16) __bf16 q[NP * C * DK];
-        alignas(16) __bf16 k[STATE_ONLY ? 8 : NP * C * DK];
-        alignas(16) __bf16 v[STATE_ONLY ? 8 : NP * C * DV];
-        alignas(16) __bf16 o[NP * C * DV];
-        alignas(16) __bf16 p[2][STATE_ONLY ? 8 : NC * C * C];
-        alignas(16) Decays<C> d[2];
-        float dots[NW1][C];
-    };
-
-    template <typename P, int GROUP, int NW>
-    static __device__ __forceinline__ void walk(const Args &a, Shared &sm, int group, int wave, int tid)
-    {
-        const int lane = tid & 63, lr = lane & 15, lg = lane >> 4;
-        const Place<C> w(a, 1);
-        const int BH = a.B * a.H, bh = w.bh, seg = w.seg, b = w.b, h = w.h, len = w.len, live = w.live, c0 = w.c0, c1 = w.c1;
-        if (STATE_ONLY && seg == a.nseg - 1) return;
-        const int gr = GROUP < 0 ? group : GROUP;
-        const Role &ro = a.role[gr], &r0 = a.role[0], &r1 = a.role[1];
-        const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
-        const bool clock = gr == 1 && wave == NW - 1;        // the wave that keeps the decays
-        const float *pg = a.g + b * a.gb + h * a.gh;
-        const auto token0 = [&](int ci) { return (live - 1 - ci) * C; };
-        const __bf16 *x = gr ? sm.v : sm.k, *y = gr ? sm.o : sm.q, *z = gr ? sm.q : sm.o;
-        __bf16 *const p = sm.p[gr];
-
-        const Rows<T, C, VEC> out(ro.O, b, h, 1, lr, z0 + 4 * lg);
-        const auto row_base = [&](const Tensor &t) {
-            return held(t.p && (sizeof(T) == 4 || !t.f32) ? t.p + ((long long)b * t.sb + (long long)h * t.sh) * (long long)sizeof(T) : nullptr);
-        };
-        const char *const ov = row_base(r0.O), *const ok = row_base(r1.O);
-        const long long ov_st = held(r0.O.st * (long long)sizeof(T)), ok_st = held(r1.O.st * (long long)sizeof(T));
-        P ps;
-        ps.zero();
-        const size_t slot = ((size_t)(gr * BH + bh) * a.nseg + seg) * (DK * DV);
-        f32x4 *const states = reinterpret_cast<f32x4 *>(a.states + (STATE_ONLY ? slot : slot - DK * DV)) + wave * P::KT * P::NT * 64 + lane;
-        if (seg == 0) {
-            if (ro.s_in) ps.load_state(ro.s_in + (size_t)bh * dc * dz, dc, dz, ro.in_c, ro.in_z, z0, lr, lg);
-        } else if (!STATE_ONLY) {
-            ps.resume(states);
-        }
-        Tile<T, DK, C, NTHR, VEC> tq, tk;
-        Tile<T, DV, C, NTHR, VEC> tv, to;
-        typename decltype(tq)::Flight fq, fk;
-        typename decltype(tv)::Flight fv, fo;
-        tq.init(r0.Y, b, h, tid, 1);
-        to.init(r0.Z, b, h, tid, 1);
-        if (!STATE_ONLY) {
-            tk.init(r0.X, b, h, tid, 1);
-            tv.init(r1.X, b, h, tid, 1);
-            tk.ocol = r1.O.d - (tid % tk.PER) * tk.UE;
-            tv.ocol = r0.O.d - (tid % tv.PER) * tv.UE;
-        }
-        float g = 0.0f;
-        double gsum = 0.0;
-        const auto fetch = [&](int ci) {
-            const int t0 = token0(ci), n = len - t0;
-            tq.fetch(fq, t0, n);
-            to.fetch(fo, t0, n);
-            if (!STATE_ONLY) {
-                tk.fetch(fk, t0, n);
-                tv.fetch(fv, t0, n);
-            }
-        };
-        const auto fetch_g = [&](int ci) { g = fetch_decay<C>(pg, a.gt, token0(ci), len, 1, lane); };
-        const auto flush = [&](int ci) {
-            const int t0 = token0(ci), t = t0 + tid;
-            if (ov) tv.drain(sm.v, tid, ov + t0 * ov_st, ov_st, len - t0);
-            if (ok) tk.drain(sm.k, tid, ok + t0 * ok_st, ok_st, len - t0);
-            if (DOTS && tid < C && t < len) {
-                float s = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NW1; ++i) s += sm.dots[i][tid];
-                r1.dots[(size_t)bh * a.T + t] = s;
-            }
-        };
-        if (c0 < c1) {
-            fetch(c0);
-            if (clock) {
-                fetch_g(c0);
-                gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[c0 & 1]);
-            }
-        }
-        for (int ci = c0; ci < c1; ++ci) {
-            const Decays<C> &d = sm.d[ci & 1];
-            __syncthreads();                              // nobody reads the last chunk's tiles any more
-            if (!STATE_ONLY && ci > c0) flush(ci - 1);
-            tq.store(fq, sm.q, tid);
-            to.store(fo, sm.o, tid);
-            if (!STATE_ONLY) {
-                tk.store(fk, sm.k, tid);
-                tv.store(fv, sm.v, tid);
-            }
-            __syncthreads();
-            if (ci + 1 < c1) {
-                fetch(ci + 1);
-                if (clock) fetch_g(ci + 1);
-            }
-            if (!STATE_ONLY) {
-                P::template scores<NW>(x, y, p, d, ro.scale_p, wave, lr, lg);
-                ps.from_state(x, d, lr, lg);
-                __syncthreads();                          // the scores are whole
-            }
-            ps.from_chunk(y, z, p, d, z0, lr, lg);
-            if constexpr (!STATE_ONLY) {
-                // k's tile and v's are read no more: dk and dv into them, for whole rows to memory.  A lane reads k, for its dots, where it
-                // puts dk.
-                if constexpr (DOTS && GROUP != 0) {
-                    if (gr) ps.dot_rows(sm.dots[wave], 1, lr, lg, [&](int I, int n) __attribute__((always_inline)) { return tile_value<T, P::DZ_, C>(sm.k, I * 16 + lr, z0 + 16 * n + 4 * lg); });
-                }
-                if (!out.f32) ps.lay_rows(gr ? sm.k : sm.v, z0, lr, lg);
-                else if (out.p) ps.store_rows(out, token0(ci), len);
-            }
-            if (clock && ci + 1 < c1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[(ci + 1) & 1]);
-        }
-        if (STATE_ONLY) {
-            ps.save(states);
-            if (clock && lane == 0) {
-                const float e = fast_exp2((float)gsum);
-                a.decays[(size_t)bh * a.nseg + seg] = e;
-                a.decays[(size_t)(BH + bh) * a.nseg + seg] = e;
-            }
-            return;
-        }
-        if (c0 < c1) {
-            __syncthreads();
-            flush(c1 - 1);
-        }
-        const int first = c0 * C, behind = min(a.T, (c0 + a.seg_chunks) * C);
-        zero_rows<T>(r0, len, first, behind, b, h, tid, NTHR);
-        zero_rows<T>(r1, len, first, behind, b, h, tid, NTHR);
-        if (ro.s_out && seg == a.nseg - 1)
-            ps.store_state(ro.s_out + (size_t)bh * dc * dz, dc, dz, ro.out_c, ro.out_z, z0, lr, lg,
-                           ro.last_decay && len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f);
-    }
-};
-
-template <typename T, int DK, int DV, int VEC, bool DOTS, bool STATE_ONLY>
-__global__ void __launch_bounds__((Pair<T, DK, DV, VEC, DOTS, STATE_ONLY>::NTHR), (Pair<T, DK, DV, VEC, DOTS, STATE_ONLY>::RESIDENT)) pair_kernel(const Args a)
-{
-    typedef Pair<T, DK, DV, VEC, DOTS, STATE_ONLY> K;
-    __shared__ typename K::Shared sm;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int group = wave >= K::NW0, w = group ? wave - K::NW0 : wave;
-    if constexpr (DK == DV) {
-        K::template walk<typename K::P0, -1, K::NW0>(a, sm, group, w, tid);
-    } else {
-        if (group == 0) K::template walk<typename K::P0, 0, K::NW0>(a, sm, 0, w, tid);
-        else K::template walk<typename K::P1, 1, K::NW1>(a, sm, 1, w, tid);
-    }
-}
-
 template <typename T, int DC, int DZ, int VEC>
 static int launch_one(const Args &a, int kind, hipStream_t stream)
 {
-    const unsigned grid = (unsigned)((size_t)a.B * a.H * a.nseg * (kind & PAIR ? 1 : a.nroles));
-    if (kind & PAIR) {
-        constexpr int n = Pair<T, DC, DZ, VEC, false, true>::NTHR;
-        if (kind & STATES) pair_kernel<T, DC, DZ, VEC, false, true><<<grid, n, 0, stream>>>(a);
-        else if (kind & DOTS_PASS) pair_kernel<T, DC, DZ, VEC, true, false><<<grid, n, 0, stream>>>(a);
-        else pair_kernel<T, DC, DZ, VEC, false, false><<<grid, n, 0, stream>>>(a);
-    } else {
-        constexpr int n = 64 * (owners<T, DZ>() + feeders<T, DZ>());
-        if (kind & STATES) state_kernel<T, DC, DZ, VEC><<<grid, 64 * owners<T, DZ>(), 0, stream>>>(a);
-        else if (kind & DOTS_PASS) chunk_kernel<T, DC, DZ, VEC, true><<<grid, n, 0, stream>>>(a);
-        else chunk_kernel<T, DC, DZ, VEC, false><<<grid, n, 0, stream>>>(a);
-    }
+    const unsigned grid = (unsigned)((size_t)a.B * a.H * a.nseg * a.nroles);
+    constexpr int n = 64 * (owners<T, DZ>() + feeders<T, DZ>());
+    if (kind & STATES) state_kernel<T, DC, DZ, VEC><<<grid, 64 * owners<T, DZ>(), 0, stream>>>(a);
+    else if (kind & DOTS_PASS) chunk_kernel<T, DC, DZ, VEC, true><<<grid, n, 0, stream>>>(a);
+    else chunk_kernel<T, DC, DZ, VEC, false><<<grid, n, 0, stream>>>(a);
     return launch_status("linear_attention");
 }
 
