@@ -384,6 +384,13 @@ struct Pass {
 #pragma unroll
             for (int n = 0; n < NT; ++n) S[t][n] = (f32x4){0, 0, 0, 0};
     }
+    __device__ __forceinline__ void zero_rows()
+    {
+#pragma unroll
+        for (int I = 0; I < CT; ++I)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) O[I][n] = (f32x4){0, 0, 0, 0};
+    }
     // between kernels: in the order of the registers
     __device__ __forceinline__ void save(f32x4 *p) const
     {
@@ -547,19 +554,21 @@ struct Pass {
         }
     }
 
-    // by 32 tokens: O^T += z^T P^T;  S = 2^{G_C} S + y^T (2^{G_C - G_j} z_j)
+    // by 32 tokens: O^T += z^T P^T, and where the state is wanted S = 2^{G_C} S + y^T (2^{G_C - G_j} z_j)
+    template <bool UPDATE>
     __device__ __forceinline__ void from_chunk(const __bf16 *y, const __bf16 *z, const __bf16 *P, const Decays<C> &d, int z0, int lr, int lg)
     {
-        const float tot = d.tot;
+        if (UPDATE) {
+            const float tot = d.tot;
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+            for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) S[t][n] *= tot;
+                for (int n = 0; n < NT; ++n) S[t][n] *= tot;
+        }
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
             b16x8 zs[NT][NS];
             const int row = 32 * s + 4 * lg;           // slots 4u + i of lane group g are token 32 s + 16 u + 4 g + i
-            const f32x4 r0 = *reinterpret_cast<const f32x4 *>(&d.R[row]), r1 = *reinterpret_cast<const f32x4 *>(&d.R[row + 16]);
             b16x8 zf[NT][NP];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -582,6 +591,8 @@ struct Pass {
                         for (int n = 0; n < NT; ++n) O[I][n] = mfma(zf[n][i], pf[I][j], O[I][n]);
                 });
             }
+            if (!UPDATE) continue;
+            const f32x4 r0 = *reinterpret_cast<const f32x4 *>(&d.R[row]), r1 = *reinterpret_cast<const f32x4 *>(&d.R[row + 16]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float w[8];
@@ -750,7 +761,7 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
         tz.store(fz, sm.z, tid);
         __syncthreads();
         if (ci + 1 < w.c1) fetch(ci + 1);
-        ps.from_chunk(sm.y, sm.z, nullptr, sm.d[ci & 1], z0, lr, lg);
+        ps.template from_chunk<true>(sm.y, sm.z, nullptr, sm.d[ci & 1], z0, lr, lg);
     }
     f32x4 *const states = reinterpret_cast<f32x4 *>(a.states + ((size_t)(w.ri * BH + w.bh) * a.nseg + w.seg) * (DC * DZ)) + wave * P::KT * P::NT * 64 + lane;
     ps.save(states);
@@ -870,8 +881,10 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
     } else {
         const int dc = ro.Y.d, dz = ro.Z.d, z0 = wave * 16 * P::NT;
         const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(DOTS && dots ? ro.W : ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg);
+        const bool fresh = w.seg == 0 && !ro.s_in, leaves = ro.s_out && w.seg == a.nseg - 1;
         P ps;
         ps.zero();
+        ps.zero_rows();                                  // for good where the owner has no columns: its dots are 0
         if (w.seg == 0) {
             if (ro.s_in) ps.load_state(ro.s_in + (size_t)w.bh * dc * dz, dc, dz, ro.in_c, ro.in_z, z0, lr, lg);
         } else {
@@ -893,16 +906,19 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
 #pragma unroll
                     for (int n = 0; n < P::NT; ++n) wf[I][n] = wrows.load4(rs, len - t0, I, n);
             }
-            if (z0 < dz) ps.from_state(sm.x[ci & 1], d, lr, lg);
+            // an owner without columns has nothing to do, the first chunk of a sequence no state to read, the last none to leave
+            if (z0 < dz && ci == c0 && fresh) ps.zero_rows();
+            else if (z0 < dz) ps.from_state(sm.x[ci & 1], d, lr, lg);
             __syncthreads();
-            if (z0 < dz) ps.from_chunk(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
+            if (z0 < dz && (ci + 1 < c1 || leaves)) ps.template from_chunk<true>(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
+            else if (z0 < dz) ps.template from_chunk<false>(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
             if (WHOLE && !out.f32) ps.lay_rows(sm.x[ci & 1], z0, lr, lg);
             else if (out.p) ps.store_rows(out, t0, len);
             if (DOTS && dots)
                 ps.dot_rows(sm.dots[wave], reverse, lr, lg, [&](int I, int n) __attribute__((always_inline)) { return Rows<T, C, VEC>::value(wf[I][n]); });
             __syncthreads();
         }
-        if (ro.s_out && w.seg == a.nseg - 1)
+        if (leaves)
             ps.store_state(ro.s_out + (size_t)w.bh * dc * dz, dc, dz, ro.out_c, ro.out_z, z0, lr, lg,
                            ro.last_decay && len > 0 ? fast_exp2((float)log2_decay(pg[0])) : 1.0f);
     }
