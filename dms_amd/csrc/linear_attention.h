@@ -22,10 +22,15 @@ struct Role {
     float *s_out;                 // state after the last step, the same with out_c / out_z, or null
     int in_c, in_z, out_c, out_z;
     float *dots;                  // (B, H, T) or null
+    float *keep;                  // with dots: the states that meet another role's at the tokens ANCHOR, 2 ANCHOR, .., or null
     float scale_p, scale_x, scale_z;   // of the products inside a chunk, of x S, and of z in the state
     int reverse;                  // 1: time runs backwards; step s decays by the g of the token after it
     int last_decay;               // 1: s_out is decayed by g of token 0 as well
 };
+
+// tokens at which the gradient of the decays is known from the two states that meet there: a multiple of both chunks
+constexpr int ANCHOR = 256;
+__host__ __device__ inline int anchors(int T) { return T > 0 ? (T - 1) / ANCHOR : 0; }
 
 struct Args {
     Role role[3];

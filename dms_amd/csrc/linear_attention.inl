@@ -369,10 +369,18 @@ struct Rows {
     }
 };
 
-// The part of a chunk that one pass (one Role) does, by its NW waves; x, y, z are LDS tiles of NP planes.
-template <typename T, int DC, int DZ, int C, int NW, int NX, bool STATE_ONLY>
+// A plane of the scores P: 32 tokens see nothing behind themselves, so that the first 32 rows of 64 are half as long (with three
+// planes two workgroups of 64 x 64 bf16 still share a compute unit).  Row lr of tile row I.
+template <int C> constexpr int scores_plane() { return C == 64 ? 32 * (32 + 64) : 32 * 32; }
+template <int C> __device__ __forceinline__ int score(int I, int lr, int col)
+{
+    return I < 2 ? at<32>(I * 16 + lr, col) : 32 * 32 + at<C>((I - 2) * 16 + lr, col);
+}
+
+// The part of a chunk that one pass (one Role) does, by its NW waves; x, y, z are LDS tiles of NP planes, what is computed has NC.
+template <typename T, int DC, int DZ, int C, int NW, int NC, bool STATE_ONLY>
 struct Pass {
-    static constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC;
+    static constexpr int NP = Kind<T>::NP;
     static constexpr int NT = DZ / 16 / NW, CT = C / 16, KT = DC / 16;     // tiles of 16: a wave's columns, tokens, rows of S
     f32x4 S[KT][NT];
     f32x4 O[STATE_ONLY ? 1 : CT][NT];
@@ -444,7 +452,7 @@ struct Pass {
         split2<NC>(p[2], p[3], b);
 #pragma unroll
         for (int k = 0; k < NC; ++k)
-            *reinterpret_cast<u32x2 *>(P + k * C * C + at<C>(I * 16 + lr, 32 * (J / 2) + 8 * lg + 4 * (J % 2))) = (u32x2){a[k], b[k]};
+            *reinterpret_cast<u32x2 *>(P + k * scores_plane<C>() + score<C>(I, lr, 32 * (J / 2) + 8 * lg + 4 * (J % 2))) = (u32x2){a[k], b[k]};
     }
     // the tiles J0 .. J1 of rows I; J1 > I stands for the zeros
     template <int I, int J0, int J1>
@@ -522,13 +530,13 @@ struct Pass {
             for (int n = 0; n < NT; ++n) O[I][n] = (f32x4){0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < DC / 32; ++s) {
-            b16x8 st[NT][NX];
+            b16x8 st[NT][NC];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float w[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) w[j] = S[2 * s + j / 4][n][j % 4];
-                split8<NX>(w, st[n]);
+                split8<NC>(w, st[n]);
             }
             b16x8 xf[CT][NP];
 #pragma unroll
@@ -539,7 +547,7 @@ struct Pass {
                     xf[I][k] = join(*reinterpret_cast<const b16x4 *>(q + at<DC>(I * 16 + lr, 32 * s + 4 * lg)),
                                     *reinterpret_cast<const b16x4 *>(q + at<DC>(I * 16 + lr, 32 * s + 16 + 4 * lg)));
                 }
-            plane_products<NX, NP>([&](int i, int j) __attribute__((always_inline)) {
+            plane_products<NC, NP>([&](int i, int j) __attribute__((always_inline)) {
 #pragma unroll
                 for (int I = 0; I < CT; ++I)
 #pragma unroll
@@ -583,7 +591,7 @@ struct Pass {
 #pragma unroll
                 for (int I = 2 * s; I < CT; ++I)
 #pragma unroll
-                    for (int k = 0; k < NC; ++k) pf[I][k] = *reinterpret_cast<const b16x8 *>(P + k * C * C + at<C>(I * 16 + lr, 32 * s + 8 * lg));
+                    for (int k = 0; k < NC; ++k) pf[I][k] = *reinterpret_cast<const b16x8 *>(P + k * scores_plane<C>() + score<C>(I, lr, 32 * s + 8 * lg));
                 plane_products<NP, NC>([&](int i, int j) __attribute__((always_inline)) {
 #pragma unroll
                     for (int I = 2 * s; I < CT; ++I)
@@ -777,27 +785,28 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
 // and cost the memory twice as much).
 // Waves of a SIMD that the LDS leaves room for: two workgroups of 8 where the tiles take less than half of it (rows that are
 // fetched element by element need the registers more).
-template <typename T, int DC, int DZ, int VEC> constexpr int residents()
+template <typename T, int DC, int DZ, int VEC, bool DOTS> constexpr int residents()
 {
-    const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * Kind<T>::NC * chunk<T>() * chunk<T>() * 2 + 6 * 1024;
+    const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * (DOTS ? 3 : Kind<T>::NC) * scores_plane<chunk<T>()>() * 2 + 4 * 1024;
     const int waves = owners<T, DZ>() + feeders<T, DZ>();
     return waves / 4 * (VEC && waves == 8 && tiles <= 80 * 1024 ? 2 : 1);
 }
 
-// DOTS: the sums of W o as well, and x S to 24 bits for them.
+// DOTS: the sums of W o as well, x S and the scores to 24 bits for them: with 16 the decays' gradient, an fp32 output, is off by 2.3e-6
+// of its norm for 2000 tokens in bf16 (3.3e-7 with 24), by 6.5e-6 for 11 in fp16 (1.1e-6), at 1025 against 1131 us for 512 heads of 64.
 template <typename T, int DC, int DZ, int VEC, bool DOTS>
-__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ, VEC>())) chunk_kernel(const Args a)
+__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ, VEC, DOTS>())) chunk_kernel(const Args a)
 {
     constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<T, DZ>(), NTHR = 64 * (NO + NF);
-    constexpr int NP = Kind<T>::NP, NC = Kind<T>::NC, NX = DOTS ? 3 : NC;
+    constexpr int NP = Kind<T>::NP, NC = DOTS ? 3 : Kind<T>::NC;
     constexpr bool WHOLE = DC == DZ;                 // rows of o fit x's tile
     constexpr int AHEAD = DC <= 64 && DZ <= 64 ? 2 : 1;   // chunks of rows in flight: with 128 columns one is as many bytes, and registers are short
-    typedef Pass<T, DC, DZ, C, NO, NX, false> P;
+    typedef Pass<T, DC, DZ, C, NO, NC, false> P;
     struct Shared {
         alignas(16) __bf16 x[2][NP * C * DC];
         alignas(16) __bf16 y[2][NP * C * DC];
         alignas(16) __bf16 z[NP * C * DZ];
-        alignas(16) __bf16 p[2][NC * C * C];
+        alignas(16) __bf16 p[2][NC * scores_plane<C>()];
         Decays<C> d[2];
         float dots[NO][C];
     };
@@ -883,6 +892,10 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(DOTS && dots ? ro.W : ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg);
         const bool fresh = w.seg == 0 && !ro.s_in, leaves = ro.s_out && w.seg == a.nseg - 1;
         P ps;
+        f32x4 *const keep = reinterpret_cast<f32x4 *>(held(DOTS && ro.keep ? ro.keep + (size_t)w.bh * anchors(a.T) * (DC * DZ) : nullptr));
+        const auto save = [&](int t0) {                  // the state that meets the other role's before token t0
+            ps.save(keep + (t0 / ANCHOR - 1) * (DC * DZ / 4) + wave * P::KT * P::NT * 64 + lane);
+        };
         ps.zero();
         ps.zero_rows();                                  // for good where the owner has no columns: its dots are 0
         if (w.seg == 0) {
@@ -898,6 +911,8 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         for (int ci = c0; ci < c1; ++ci) {
             const Decays<C> &d = sm.d[ci & 1];
             const int t0 = token0(ci);
+            const bool anchor = DOTS && keep && t0 > 0 && t0 % ANCHOR == 0;
+            if (anchor && !reverse) save(t0);
             typename Rows<T, C, VEC>::Raw wf[DOTS ? P::CT : 1][P::NT];
             if (DOTS && dots) {                              // on their way while o is computed
                 const __amdgpu_buffer_rsrc_t rs = buffer(wrows.p + (long long)t0 * wrows.st);
@@ -910,10 +925,11 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
             if (z0 < dz && ci == c0 && fresh) ps.zero_rows();
             else if (z0 < dz) ps.from_state(sm.x[ci & 1], d, lr, lg);
             __syncthreads();
-            if (z0 < dz && (ci + 1 < c1 || leaves)) ps.template from_chunk<true>(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
+            if (z0 < dz && (ci + 1 < c1 || leaves || anchor)) ps.template from_chunk<true>(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
             else if (z0 < dz) ps.template from_chunk<false>(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
             if (WHOLE && !out.f32) ps.lay_rows(sm.x[ci & 1], z0, lr, lg);
             else if (out.p) ps.store_rows(out, t0, len);
+            if (anchor && reverse) save(t0);
             if (DOTS && dots)
                 ps.dot_rows(sm.dots[wave], reverse, lr, lg, [&](int I, int n) __attribute__((always_inline)) { return Rows<T, C, VEC>::value(wf[I][n]); });
             __syncthreads();

@@ -157,6 +157,36 @@ def test_backward(case):
         bounded(x, y, m, x.dtype, DELTA[dtype] * (2 if n == "g" else 1))       # g: two operands carry the error
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,T,dk,dv,end", [("fp32", 1100, 16, 16, True), ("bf16", 1100, 16, 24, True), ("fp16", 513, 24, 16, False),
+                                               ("bf16", 257, 64, 64, False), ("fp32", 512, 33, 16, True)])
+def test_gradient_of_the_decays_far_from_either_end(dtype, T, dk, dv, end):
+    """Lengths on both sides of every 256th token, where the gradient is known from the states that meet there.  In between it is
+    a sum of at most 256 dots that starts at one of them and is corrected at the next, so that its error stays below that of the two
+    and twice that of the dots: 24 bits of each operand beside every type (2 * 2^-26), 2^-20 for the exponents, and 7 roundings of
+    2^-24 in at most 35 chunks with 64 for the dot and its chunk, 2^-15.7: 2^-15."""
+    lengths = [n for n in (0, 1, 255, 256, 257, 511, 512, 513, 1024, 1025, 1100) if n <= T]
+    a, do, ds, scale = make(dtype, T, len(lengths), 1, dk, dv, state=True, resets=(128, 256), seed=T + 5)
+    a["g"] = a["g"] * 0.1                                  # states that live for a while
+    a["lengths"] = torch.tensor(lengths)
+    ds = ds if end else torch.zeros_like(ds)
+    dev = {n: x.to(DEV) for n, x in a.items()}
+    dev["g"].requires_grad_()
+    o, s = ops.linear_attention(**dev)
+    got, = torch.autograd.grad([o, s] if end else [o], [dev["g"]], [do.to(DEV), ds.to(DEV)][:2 if end else 1])
+    args = [f64(a[n]) for n in ("q", "k", "v", "g", "state0")]
+    want = plain_grads(*args, a["lengths"], scale, f64(do), f64(ds))[5]
+    size = [x.abs() if i != 3 else x for i, x in enumerate(args)]
+    mag = plain_grads(*size, a["lengths"], scale, f64(do).abs(), f64(ds).abs())
+    ends = (mag[1] * f64(ds).abs()).sum((-1, -2))          # what meets behind the last token
+    flow = (size[0] * mag[2] + size[1] * mag[3]).sum(-1)
+    bound = torch.zeros_like(want)
+    for t in range(0, T, 256):
+        far = torch.where((torch.tensor(lengths) > t + 256)[:, None], mag[5][min(t + 256, T - 1)], ends)
+        bound[t:t + 256] = mag[5][t] + far + 2 * flow[t:t + 256].sum(0)
+    bounded(got, want, bound, torch.float32, 2.0 ** -15)
+
+
 def test_plain_gradients_are_differences():
     """The 64-bit gradients that the kernels are held to, against central differences."""
     a, do, ds, scale = make("fp32", 5, 2, 2, 3, 2, Hk=1, state=True, ragged=True, seed=4)
@@ -459,6 +489,11 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
         _lib.call("dmn_linear_attention_fwd", 0, 16, 16, 16, 16, None, None, 0, 16, None, strides, None, *long[1:], 1.0, None)
     with pytest.raises(RuntimeError, match="workspace"):
         _lib.call("dmn_linear_attention_bwd", 0, 16, 16, 16, 16, None, None, 0, 16, None, 16, 16, 16, None, 0, None, strides, 8, *ok[1:], 1.0, None)
+    for at, value in ((0, (1 << 24) + (1 << 20) + 1), (3, -8), (6, 1 << 40)):
+        far = [16, 16, 8] * 5
+        far[at] = value
+        with pytest.raises(RuntimeError, match="stride"):
+            _lib.call("dmn_linear_attention_fwd", 0, 16, 16, 16, 16, None, None, 0, 16, None, ops._strides(far), None, *ok[1:], 1.0, None)
     with pytest.raises(RuntimeError, match="null pointer"):
         _lib.call("dmn_linear_attention_step", 0, 16, 16, 16, 16, None, 16, strides, 1, 2, 2, 2, 2, 8, 8, 1.0, None)
 
