@@ -334,7 +334,7 @@ static int run(const char *who, int dtype, Args &a, bool backward, hipStream_t s
     const int groups = 256 >> s.lg, all = a.heads[0] + a.heads[1];
     long long blocks = (a.tokens + groups - 1) / groups;
     if (backward && blocks > MAX_BLOCKS) blocks = MAX_BLOCKS;
-    if (blocks > 0x7fffffffLL) return fail(-6, "%s: %lld tokens exceed one grid", who, a.tokens);
+    if (blocks > 0xffffffLL) return fail(-6, "%s: %lld tokens exceed one grid", who, a.tokens);
     // few tokens: the heads go over the grid as well, at the price of the angles once more for each slice
     a.nslice = 1;
     while (a.nslice < all && blocks * a.nslice < 2 * NUM_CU) a.nslice *= 2;

@@ -40,13 +40,13 @@ __global__ void __launch_bounds__(64) combine_kernel(float *states, const float 
 template <typename T>
 __global__ void __launch_bounds__(256) group_sum_kernel(const float *in, T *out, int heads, int group, int d, long long total)
 {
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (e >= total) return;
-    const long long row = e / d;                          // (token, sample, head)
-    const float *p = in + row * group * d + e % d;
-    float s = 0.0f;
-    for (int u = 0; u < group; ++u) s += p[(long long)u * d];
-    out[e] = (T)s;
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
+        const long long row = e / d;                      // (token, sample, head)
+        const float *p = in + row * group * d + e % d;
+        float s = 0.0f;
+        for (int u = 0; u < group; ++u) s += p[(long long)u * d];
+        out[e] = (T)s;
+    }
 }
 
 template <int N>
@@ -333,7 +333,8 @@ static int check(const char *who, int dtype, int T, int B, int H, int Hq, int Hk
     if (H % Hq || H % Hk || H % Hv) return fail(-4, "%s: the %d heads of the state must be a multiple of Hq=%d, Hk=%d and Hv=%d", who, H, Hq, Hk, Hv);
     if (dk < 1 || dk > 128 || dv < 1 || dv > 128) return fail(-5, "%s: head widths must be 1 .. 128, got dk=%d dv=%d", who, dk, dv);
     if ((long long)B * H > (1 << 17)) return fail(-6, "%s: B * H = %lld exceeds 2^17", who, (long long)B * H);
-    if (T > 0x3fffffff) return fail(-6, "%s: T = %d exceeds 2^30", who, T);
+    if (T > 1 << 29 || (long long)T * B * H > 0xffffffffLL)   // threads of a grid
+        return fail(-6, "%s: T = %d exceeds 2^29, or T * B * H = %lld 2^32", who, T, (long long)T * B * H);
     return 0;
 }
 
@@ -388,14 +389,14 @@ static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, 
 template <typename T>
 static void group_sum(const float *in, void *out, int heads, int H, int d, long long total, hipStream_t stream)
 {
-    group_sum_kernel<T><<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(in, static_cast<T *>(out), heads, H / heads, d, total);
+    const long long blocks = (total + 255) / 256;
+    group_sum_kernel<T><<<(unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), 256, 0, stream>>>(in, static_cast<T *>(out), heads, H / heads, d, total);
 }
 
 static int group_sum(int dtype, const float *in, void *out, int T, int B, int heads, int H, int d, hipStream_t stream)
 {
     const long long total = (long long)T * B * heads * d;
     if (total == 0) return 0;
-    if ((total + 255) / 256 > 0x7fffffffLL) return fail(-6, "linear_attention: %lld gradients exceed one grid", total);
     if (dtype == DTYPE_BF16) group_sum<__bf16>(in, out, heads, H, d, total, stream);
     else if (dtype == DTYPE_F16) group_sum<_Float16>(in, out, heads, H, d, total, stream);
     else group_sum<float>(in, out, heads, H, d, total, stream);

@@ -919,7 +919,7 @@ def linear_attention(q, k, v, g, state0=None, lengths=None, scale=None):
     q (T, B, Hq, dk), k (T, B, Hk, dk), v (T, B, Hv, dv) in float32, bfloat16 or float16, with unit stride along the last
     axis and any other strides; g (T, B, H) or (H,) float32 log decays (<= 0; -inf empties the state before that token, so
     sequences can be packed one behind the other).  H, the heads of the state, is a multiple of Hq, Hk and Hv: head h
-    reads head h // (H // Hq) of q, and so on.  Head widths up to 128.  state0 (B, H, dk, dv) float32 or None (zeros);
+    reads head h // (H // Hq) of q, and so on.  Head widths up to 128, B * H up to 2^17, tokens up to 2^24 elements apart.  state0 (B, H, dk, dv) float32 or None (zeros);
     lengths (B,) int32 or int64 on the device, or None: tokens of each sample, rows behind them are neither read nor do
     they change the state, and their outputs and gradients are zero.  scale: dk ** -0.5 if None.
     Returns o (T, B, H, dv) and the state (B, H, dk, dv) after the last token, both under autograd (once)."""
@@ -938,7 +938,7 @@ def linear_attention(q, k, v, g, state0=None, lengths=None, scale=None):
         if state0.device != q.device:
             raise RuntimeError("dms_amd.%s: state0 is on %s, q on %s" % (name, state0.device, q.device))
     if lengths is not None:
-        if (not lengths.is_cuda or lengths.device != q.device or lengths.dtype not in (torch.int32, torch.int64)
+        if (not torch.is_tensor(lengths) or not lengths.is_cuda or lengths.device != q.device or lengths.dtype not in (torch.int32, torch.int64)
                 or lengths.shape != (B,) or not lengths.is_contiguous()):
             raise RuntimeError("dms_amd.%s: lengths must be a contiguous int32 or int64 tensor of shape (%d,) on %s"
                                % (name, B, q.device))

@@ -405,8 +405,8 @@ int dmn_dpn_stage_pass(float *buf, float *act, float *out,
  *     o[t,b,h] = scale * q[t,b,h] S_t
  *   dtype    0: fp32, 1: bf16, 2: fp16 -- of q, k, v, o and their gradients.  g, the states and grad_g are fp32.
  *   q (T,B,Hq,dk), k (T,B,Hk,dk), v (T,B,Hv,dv): unit stride along the last axis, any other strides (a slice of a fused
- *            projection, an expanded tensor).  Head h of the H heads of the state reads head h / (H/Hq) of q, and so on: H
- *            is a multiple of Hq, Hk and Hv.  1 <= dk, dv <= 128.
+ *            projection, an expanded tensor), that over t from 0 to 2^24 + 2^20 where T > 1.  Head h of the H heads of the state reads head h / (H/Hq) of q, and so on: H
+ *            is a multiple of Hq, Hk and Hv.  1 <= dk, dv <= 128; B*H <= 2^17, T <= 2^29, T*B*H < 2^32.
  *   g        log decay, <= 0 in any sensible use; -inf empties the state before the token (sequences packed one behind the
  *            other).  strides of 0 over t and b: one decay for each head.
  *   state0, state (B,H,dk,dv) contiguous or NULL; they may not overlap.
@@ -428,8 +428,9 @@ int dmn_linear_attention_fwd(int dtype, const void *q, const void *k, const void
  *   strides  HOST array of 15: the 12 above, then t, b, h of grad_o.
  *   grad_q (T,B,Hq,dk), grad_k (T,B,Hk,dk), grad_v (T,B,Hv,dv), grad_state0 (B,H,dk,dv): contiguous, or NULL if not wanted;
  *            of shared heads: the sum over the heads that read them, in head order.
- *   grad_g   (T,B,H) contiguous, or (H) with grad_g_per_head = 1 (summed over t and b, in that order), or NULL.  Zero where exp(g)
- *            is zero in 32 bits.
+ *   grad_g   (T,B,H) contiguous, or (H) with grad_g_per_head = 1 (summed over t and b, always in the same order), or NULL.  Zero
+ *            where exp(g) is zero in 32 bits.  It is the difference of what queries and keys give back, so that its error goes by
+ *            the sizes of q . grad_q and k . grad_k, summed from the 256th token before it on, where it is known from two states.
  *   workspace  dmn_linear_attention_workspace_floats(dtype, 1, ...) floats, 16-byte aligned.
  * No atomics: the same inputs give the same bits.
  */

@@ -224,6 +224,37 @@ def test_backward_is_a_difference_of_the_kernel_itself():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dk,dv", [("bf16", 64, 64), ("fp32", 64, 100), ("fp16", 32, 20)])
+def test_one_gradient_at_a_time(dtype, dk, dv):
+    """Each leaf alone, and each output alone: other launches than all together, each within the bound of its own."""
+    a, do, ds, scale = make(dtype, 300, 2, 4, dk, dv, Hq=2, Hv=1, state=True, ragged=True, seed=21)
+    names = ("q", "k", "v", "g", "state0")
+    do, ds = do.to(DEV), ds.to(DEV)
+
+    def run(wanted, outs=(0, 1)):
+        dev = {n: x.to(DEV) for n, x in a.items()}
+        leaves = [dev[n].requires_grad_() for n in wanted]
+        out = ops.linear_attention(**dev)
+        return torch.autograd.grad([out[i] for i in outs], leaves, [(do, ds)[i] for i in outs], allow_unused=True)
+
+    full = run(names)
+    want = plain_grads(*[f64(a[n]) for n in names], a["lengths"], scale, f64(do), f64(ds))[2:]
+    size = [f64(a[n]).abs() if n != "g" else f64(a[n]) for n in names]
+    mag = plain_grads(*size, a["lengths"], scale, f64(do).abs(), f64(ds).abs())[2:]
+    for n, x, y, m, all_of_them in zip(names, [run((n,))[0] for n in names], want, mag, full):
+        if n == "g":                                       # its own bound is that of test_backward; here only the same sums differ
+            assert (f64(x) - f64(all_of_them)).abs().max() <= DELTA[dtype] * m.max()
+        else:
+            bounded(x, y, m, x.dtype, DELTA[dtype])
+    parts = [run(names, (i,)) for i in (0, 1)]
+    assert parts[1][0] is None or not parts[1][0].any()    # the state does not depend on q
+    for n, x, y, z, m in zip(names[1:], parts[0][1:], parts[1][1:], full[1:], mag[1:]):
+        half = 2 * torch.finfo(z.dtype).eps * (f64(x).abs() + f64(y).abs())
+        slack = 4 * DELTA[dtype] * (m if n != "g" else m.max())
+        assert ((f64(x) + f64(y) - f64(z)).abs() <= half + slack).all(), n
+
+
+@pytest.mark.gpu
 def test_rows_behind_the_lengths_are_neither_read_nor_counted():
     a, do, ds, scale = make("bf16", 150, 4, 2, 64, 64, state=True, seed=3)
     a["lengths"] = torch.tensor([0, 1, 64, 150], dtype=torch.int64)
@@ -473,10 +504,11 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     assert size(*ok) == 0
     assert int(lib.dmn_linear_attention_workspace_floats(ok[0], 1, *ok[1:])) > 0
     for at, value, word in ((0, 3, b"dtype"), (1, -1, b"bad sizes"), (2, -1, b"bad sizes"), (3, 0, b"bad sizes"), (4, 3, b"multiple"),
-                            (7, 0, b"widths"), (7, 129, b"widths"), (8, 200, b"widths"), (2, 1 << 17, b"2^17")):
+                            (7, 0, b"widths"), (7, 129, b"widths"), (8, 200, b"widths"), (2, 1 << 17, b"2^17"), (1, (1 << 29) + 1, b"2^29")):
         bad = list(ok)
         bad[at] = value
         assert size(*bad) == -1 and word in lib.dmn_last_error(), (at, value)
+    assert size(0, 1 << 20, 1 << 12, 1, 1, 1, 1, 8, 8) == -1 and b"2^32" in lib.dmn_last_error()
     strides = ops._strides([16, 16, 8] * 5)
     for args, word in (((1, 1, 1, 1, None, None, 0, None, None, strides, None), "null pointer"),
                        ((1, 1, 1, 1, None, None, 0, 1, None, None, None), "null pointer"),
@@ -528,6 +560,7 @@ def test_refusals():
             (lambda: call(x, x, x, g, s.bfloat16()), "expected float32"),
             (lambda: call(x, x, x, g, lengths=torch.zeros(2, dtype=torch.int32, device=DEV)), "lengths"),
             (lambda: call(x, x, x, g, lengths=torch.zeros(1, device=DEV)), "lengths"),
+            (lambda: call(x, x, x, g, lengths=[3]), "lengths"),
             (lambda: call(x, x, x, g, lengths=torch.zeros(1, dtype=torch.int32)), "lengths"),
             (lambda: call(x, x.cpu(), x, g), "no CPU fallback"),
             (lambda: ops.linear_attention_step(x[0], x[0], x[0], g[0], s.transpose(2, 3)), "contiguous"),
