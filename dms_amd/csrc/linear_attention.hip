@@ -68,10 +68,12 @@ __device__ __forceinline__ double block_sum(double v, double *sh)
 //   dg_t = dg_s - sum_{s <= i < t} (q_i . dq_i - k_i . dk_i)
 // The dots are right to fp32, and their running sum walks away from the truth with the root of the distance.  So dg is known
 // directly at every ANCHOR-th token, from the two states that meet there, at the first (<S_0, dS_0>) and behind the last
-// (<S_T, dS_T>): a sum starts at each and what it misses at the next is spread over the way (2046 tokens: an error of 2.2e-6 of the
-// norm without, 4.4e-7 with).
+// (<S_T, dS_T>; not without anchors: 512 heads of 125 x 125 would pay 20 us for 20 tokens): a sum starts at each and what it
+// misses at the next is spread over the way (2046 tokens: an error of 2.2e-6 of the norm without, 4.4e-7 with).
 //
-// flow[bh][i] = <S, dS> between the tokens before and from (i + 1) ANCHOR on; n of either state, in the same order
+// flow[bh][i] = <S, dS> between the tokens before and from (i + 1) ANCHOR on, n4 fours of either state in the same order.  Bound by
+// reading them: 42 us, 5.6 TB/s, for 1024 heads of 64 x 64 and 2000 tokens; every 512th token would halve that, and leave 1.4 times
+// the error.
 __global__ void __launch_bounds__(256) meet_kernel(const f32x4 *before, const f32x4 *behind, double *flow, int n4)
 {
     __shared__ double sh[4];
@@ -90,8 +92,8 @@ __global__ void __launch_bounds__(256) meet_kernel(const f32x4 *before, const f3
 __host__ __device__ static inline int stretches(int T) { return (T + 4 * ANCHOR - 1) / (4 * ANCHOR); }
 
 // A wave for each stretch between anchors, four a workgroup, in 64 bits; the result takes the dots' place, or its sum goes to
-// `part`: g and dg have the heads together, and 4 bytes of every line would be written from here (44 us for 512 heads of 2000
-// tokens; this takes 20, the turn below 17).
+// `part`: g and dg have the heads together, and 4 bytes of every line would be written from here (44 us for 1024 heads of 2000
+// tokens; this takes 16, the turn below 17).
 __global__ void __launch_bounds__(256)
 decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const float *s0, const float *ds0, const float *s_end, const float *ds_end,
                   const float *g, long long gt, long long gb, long long gh, const void *lengths, int lengths64, float *part, int T, int B, int H, int n)
@@ -103,13 +105,14 @@ decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const 
     const float *pg = g + b * gb + h * gh;
     const auto meet = [&](const float *x, const float *y) {
         double v = 0.0;
+#pragma unroll 8
         for (int i = tid; i < n; i += 256) v += (double)x[(size_t)bh * n + i] * (double)y[(size_t)bh * n + i];
         v = block_sum<256>(v, sh);
         __syncthreads();
         return v;
     };
     const double first = at == 0 && s0 ? meet(s0, ds0) : 0.0;
-    const double end = at == (len - 1) / (4 * ANCHOR) && ds_end ? meet(s_end, ds_end) : 0.0;
+    const double end = at == (len - 1) / (4 * ANCHOR) && s_end ? meet(s_end, ds_end) : 0.0;
     const int a = 4 * at + (tid >> 6), t_a = a * ANCHOR;   // this stretch begins at anchor a
     const auto known = [&](int i) {                        // dg at anchor i, or behind the last token
         if (i * ANCHOR >= len) return end;
@@ -127,7 +130,8 @@ decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const 
             mine += d[i];
         }
         const double upto = lane_sums(mine), from = t_a < len ? known(a) : 0.0;
-        const double off = t_a < len ? (from - __shfl(upto, 63) - known(a + 1)) / (double)min(ANCHOR, len - t_a) : 0.0;
+        const bool tied = t_a < len && (s_end || !ds_end || t_a + ANCHOR < len);
+        const double off = tied ? (from - __shfl(upto, 63) - known(a + 1)) / (double)min(ANCHOR, len - t_a) : 0.0;
         double v = from - (upto - mine);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -380,7 +384,7 @@ static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, 
     p.dk = take(Hk < H ? rows * dk : 0);
     p.dv = take(Hv < H ? rows * dv : 0);
     p.ds0 = take(BH * dk * dv);
-    p.end = take(BH * dk * dv);
+    p.end = take(anchors(T) > 0 ? BH * dk * dv : 0);
     p.part = take(BH * stretches(T));
     p.total = at;
     return p;
@@ -510,7 +514,7 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         return t;
     };
     const bool meet = grad_g && anchors(T) > 0;           // states of dq and dk between the first and the last
-    float *const end = grad_g && grad_state ? workspace + p.end : nullptr;
+    float *const end = meet && grad_state ? workspace + p.end : nullptr;
     Role role[3] = {};
     int n = 0;
     if (grad_q || grad_g) {                               // dq: the operator on (dO, v, k)

@@ -9,15 +9,24 @@
 // is summed in 64 bits and kept as two floats: the difference of two far sums keeps its low bits.
 //
 // All four products run on the bf16 matrix instruction (16x16x32).  An operand of t bits is the sum of bf16 planes
-// (bf16: 1, fp16: 2, fp32: 3; a number that the kernel itself computed: 2, and 3 beside fp32), and a product of two is
-// the sum of the plane products that matter, smallest first, in fp32: 16 bits and more in bf16 and fp16 calls, 24 in
-// fp32 ones.  Six bf16 products take 96 cycles where the fp32 instruction takes 256 for the same product.
+// (bf16: 1, fp16: 2, fp32: 3; a number that the kernel itself computed: 2, and 3 beside fp32 and wherever the result is an
+// fp32 output or goes into one: the state, the dots W o of the decays' gradient), and a product of two is the sum of the plane
+// products that matter, smallest first, in fp32: 16 bits and more in o of bf16 and fp16 calls, 24 elsewhere.  Six bf16
+// products take 96 cycles where the fp32 instruction takes 256 for the same product.
 //
-// A workgroup takes one (sample, head, segment) and walks its chunks; a wave owns 16 * NT columns of z, and with them
-// that part of S, which stays in its accumulators from the first chunk to the last: converted, they are the operand of the
-// next chunk's x S without any exchange, because the order of a product's inner index is free.
-// x, y, z planes are staged in LDS, the next chunk's rows are in flight meanwhile.  Transposed fragments come from the
-// transposing LDS read.
+// A workgroup takes one (sample, head, segment) and walks its chunks with two kinds of waves.  Owners have 16 columns of z each,
+// and with them that part of S, which stays in their accumulators from the first chunk to the last: converted, they are the
+// operand of the next chunk's x S without any exchange, because the order of a product's inner index is free.  Feeders fetch
+// the rows of the chunks to come, lay them into LDS as planes, form decays and scores, and write whole rows of o; transposed
+// fragments come from the transposing LDS read.  bf16 chunks have 64 tokens, the others 32 (the planes' room in LDS).
+//
+// The gradients are the same kernel in other roles: dq on (dO, v, k) forward, dk on (v, dO, q) and dv on (k, q, dO) backward.
+//
+// Measured (copies here reach 5.1 TB/s): bf16, 512 heads of 64 x 64, 5120 tokens: 315 us, 1.36 GB of inputs and outputs, 4.3 TB/s
+// (566 us with one kind of wave that does all); bf16, 1024 heads, 2000 tokens, all gradients: 1110 us for three roles that
+// read 11 and write 3 tensors of 262 MB, 3.3 TB/s; fp32, 160 heads of 100 x 100, ragged, up to 2000 tokens: 254 us, of them 76 for
+// the states between segments.  Neither memory nor the matrix units (a fifth of the cycles) nor LDS (two fifths) are full: waves
+// wait for three fifths of their cycles, most at the two barriers a chunk, where owners and feeders meet.
 #pragma once
 #include "linear_attention.h"
 
@@ -483,12 +492,12 @@ struct Pass {
             if (J == I) {
                 const f32x4 jh = *reinterpret_cast<const f32x4 *>(&d.Gh[I * 16 + 4 * lg]), jl = *reinterpret_cast<const f32x4 *>(&d.Gl[I * 16 + 4 * lg]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) q[r] = 4 * lg + r > lr ? 0.0f : p[J < NJ + J0 ? J - J0 : 0][r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
+                for (int r = 0; r < 4; ++r) q[r] = 4 * lg + r > lr ? 0.0f : p[J <= JE ? J - J0 : 0][r] * scale_p * fast_exp2((gh - jh[r]) + (gl - jl[r]));
             } else if (J < I) {
                 const f32x4 f = *reinterpret_cast<const f32x4 *>(&d.F[J * 16 + 4 * lg]);
                 const float row = fast_exp2((gh - d.Gh[J * 16 + 15]) + (gl - d.Gl[J * 16 + 15])) * scale_p;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) q[r] = p[J < NJ + J0 ? J - J0 : 0][r] * (row * f[r]);
+                for (int r = 0; r < 4; ++r) q[r] = p[J <= JE ? J - J0 : 0][r] * (row * f[r]);
             }
             keep(P, I, J, q, lr, lg);
         }
@@ -787,13 +796,14 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
 // fetched element by element need the registers more).
 template <typename T, int DC, int DZ, int VEC, bool DOTS> constexpr int residents()
 {
-    const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * (DOTS ? 3 : Kind<T>::NC) * scores_plane<chunk<T>()>() * 2 + 4 * 1024;
+    constexpr int NC = DOTS ? 3 : Kind<T>::NC;
+    const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * NC * scores_plane<chunk<T>()>() * 2 + 4 * 1024;
     const int waves = owners<T, DZ>() + feeders<T, DZ>();
     return waves / 4 * (VEC && waves == 8 && tiles <= 80 * 1024 ? 2 : 1);
 }
 
 // DOTS: the sums of W o as well, x S and the scores to 24 bits for them: with 16 the decays' gradient, an fp32 output, is off by 2.3e-6
-// of its norm for 2000 tokens in bf16 (3.3e-7 with 24), by 6.5e-6 for 11 in fp16 (1.1e-6), at 1025 against 1131 us for 512 heads of 64.
+// of its norm for 2000 tokens in bf16 (3.3e-7 with 24), by 6.5e-6 for 11 in fp16 (1.1e-6), at 1025 against 1131 us for 1024 heads of 64.
 template <typename T, int DC, int DZ, int VEC, bool DOTS>
 __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ, VEC, DOTS>())) chunk_kernel(const Args a)
 {
