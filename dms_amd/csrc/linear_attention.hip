@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(64) decay_grad_heads_kernel(const float *part,
     if (threadIdx.x == 63) out[blockIdx.x] = (float)s;
 }
 
-// One token: S = a S + k^T v in place, o = scale q S.  Bound by reading and writing the state once.  A workgroup takes
+// One token: S = a S + k^T v in place, o = scale q S.  Bound by reading and writing the state once (256 streams of 16 heads of
+// 128 x 128: 537 MB in 101 us, 5.3 TB/s; 8 heads of 125 x 125: 5 us, a launch).  A workgroup takes
 // a head, or a slice of its columns where there are few heads (a row of S then still comes in whole 64-byte pieces);
 // V columns a thread (4 where every row is 16-byte aligned), rows over the threads, their partial o joined in LDS in
 // row order.

@@ -61,7 +61,7 @@ class LinearAttention(nn.Module):
             self.k_norm.fill_(1.0)
 
     def _product(self, x, w):
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or not x.shape[0]:
             return x.mm(w)
         return ops.tuned_matmul(x, w)                    # inference: BLAS library chosen per shape
 
@@ -70,9 +70,9 @@ class LinearAttention(nn.Module):
         T, B = x.shape[:2]
         rows = x.reshape(T * B, self.n_in)
         n = self.qk_heads * self.width
-        qkv = self._product(rows, self.weight).view(T, B, -1)
+        qkv = self._product(rows, self.weight).view(T, B, self.weight.shape[1])
         q, k, v = qkv.split([n, n, self.n_out], -1)
-        g = F.logsigmoid(self._product(rows, self.gate).view(T, B, -1).float() + self.gate_bias.float()) * self.DECAY_SCALE
+        g = F.logsigmoid(self._product(rows, self.gate).view(T, B, self.heads).float() + self.gate_bias.float()) * self.DECAY_SCALE
         q, k = ops.head_norm_rotary(q.view(T, B, self.qk_heads, self.width), k.view(T, B, self.qk_heads, self.width), self.q_norm,
                                     self.k_norm, positions, self.sections, self.base, self.eps)
         return q, k, v.view(T, B, self.heads, self.width), g

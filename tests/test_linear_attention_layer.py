@@ -134,6 +134,21 @@ def test_prompt_then_captured_steps(dtype):
         near(state[b], s[0], bound)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_nothing_to_read_leaves_the_state(grad):
+    layer = make(torch.float32, width=16, sections=(3,))
+    state = torch.randn(2, layer.heads, 16, 16, device=DEV)
+    with torch.set_grad_enabled(grad):
+        for T, B in ((0, 2), (3, 0)):
+            h, after = layer(torch.zeros(T, B, 40, device=DEV), state[:B], torch.zeros(T, B, 1, dtype=torch.int32, device=DEV))
+            assert h.shape == (T, B, layer.n_out) and torch.equal(after, state[:B])
+            if grad:
+                (h.sum() + after.sum()).backward()
+    if grad:
+        assert all(p.grad is None or not p.grad.any() for p in layer.parameters())
+
+
 def test_layer_refusals():
     with pytest.raises(ValueError, match="multiple"):
         dms_amd.LinearAttention(8, 30, 4)
