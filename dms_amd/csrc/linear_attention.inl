@@ -809,6 +809,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
 {
     constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<T, DZ>(), NTHR = 64 * (NO + NF);
     constexpr int NP = Kind<T>::NP, NC = DOTS ? 3 : Kind<T>::NC;
+    constexpr int ANCHOR = anchor_every(DC * DZ);
     constexpr bool WHOLE = DC == DZ;                 // rows of o fit x's tile
     constexpr int AHEAD = DC <= 64 && DZ <= 64 ? 2 : 1;   // chunks of rows in flight: with 128 columns one is as many bytes, and registers are short
     typedef Pass<T, DC, DZ, C, NO, NC, false> P;
@@ -902,10 +903,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(DOTS && dots ? ro.W : ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg);
         const bool fresh = w.seg == 0 && !ro.s_in, leaves = ro.s_out && w.seg == a.nseg - 1;
         P ps;
-        f32x4 *const keep = reinterpret_cast<f32x4 *>(held(DOTS && ro.keep ? ro.keep + (size_t)w.bh * anchors(a.T) * (DC * DZ) : nullptr));
-        const auto save = [&](int t0) {                  // the state that meets the other role's before token t0
-            ps.save(keep + (t0 / ANCHOR - 1) * (DC * DZ / 4) + wave * P::KT * P::NT * 64 + lane);
-        };
+        f32x4 *const keep = reinterpret_cast<f32x4 *>(held(DOTS && ro.keep ? ro.keep + (size_t)w.bh * anchors(a.T, ANCHOR) * (DC * DZ) : nullptr));
         ps.zero();
         ps.zero_rows();                                  // for good where the owner has no columns: its dots are 0
         if (w.seg == 0) {
@@ -921,8 +919,8 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         for (int ci = c0; ci < c1; ++ci) {
             const Decays<C> &d = sm.d[ci & 1];
             const int t0 = token0(ci);
-            const bool anchor = DOTS && keep && t0 > 0 && t0 % ANCHOR == 0;
-            if (anchor && !reverse) save(t0);
+            const int edge = reverse ? t0 : t0 + C;          // the state after this chunk is the one between the tokens edge - 1 and edge
+            const bool anchor = DOTS && keep && edge % ANCHOR == 0 && edge > 0 && edge < len;
             typename Rows<T, C, VEC>::Raw wf[DOTS ? P::CT : 1][P::NT];
             if (DOTS && dots) {                              // on their way while o is computed
                 const __amdgpu_buffer_rsrc_t rs = buffer(wrows.p + (long long)t0 * wrows.st);
@@ -939,7 +937,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
             else if (z0 < dz) ps.template from_chunk<false>(sm.y[ci & 1], sm.z, sm.p[ci & 1], d, z0, lr, lg);
             if (WHOLE && !out.f32) ps.lay_rows(sm.x[ci & 1], z0, lr, lg);
             else if (out.p) ps.store_rows(out, t0, len);
-            if (anchor && reverse) save(t0);
+            if (__builtin_expect(anchor, 0)) ps.save(keep + (size_t)(edge / ANCHOR - 1) * (DC * DZ / 4) + wave * P::KT * P::NT * 64 + lane);
             if (DOTS && dots)
                 ps.dot_rows(sm.dots[wave], reverse, lr, lg, [&](int I, int n) __attribute__((always_inline)) { return Rows<T, C, VEC>::value(wf[I][n]); });
             __syncthreads();

@@ -159,10 +159,11 @@ def test_backward(case):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,T,dk,dv,end", [("fp32", 1100, 16, 16, True), ("bf16", 1100, 16, 24, True), ("fp16", 513, 24, 16, False),
-                                               ("bf16", 257, 64, 64, False), ("fp32", 512, 33, 16, True)])
+                                               ("bf16", 257, 64, 64, False), ("fp32", 512, 33, 16, True), ("bf16", 1100, 100, 128, True),
+                                               ("fp32", 1025, 128, 100, False)])
 def test_gradient_of_the_decays_far_from_either_end(dtype, T, dk, dv, end):
-    """Lengths on both sides of every 256th token, where the gradient is known from the states that meet there.  In between it is
-    a sum of at most 256 dots that starts at one of them and is corrected at the next, so that its error stays below that of the two
+    """Lengths on both sides of every 256th token, where (at every second one for wide states) the gradient is known from the
+    states that meet there.  In between it is a sum of at most 256 (512) dots that starts at one of them and is corrected at the next, so that its error stays below that of the two
     and twice that of the dots: 24 bits of each operand beside every type (2 * 2^-26), 2^-20 for the exponents, and 7 roundings of
     2^-24 in at most 35 chunks with 64 for the dot and its chunk, 2^-15.7: 2^-15."""
     lengths = [n for n in (0, 1, 255, 256, 257, 511, 512, 513, 1024, 1025, 1100) if n <= T]
@@ -181,9 +182,10 @@ def test_gradient_of_the_decays_far_from_either_end(dtype, T, dk, dv, end):
     ends = (mag[1] * f64(ds).abs()).sum((-1, -2))          # what meets behind the last token
     flow = (size[0] * mag[2] + size[1] * mag[3]).sum(-1)
     bound = torch.zeros_like(want)
-    for t in range(0, T, 256):
-        far = torch.where((torch.tensor(lengths) > t + 256)[:, None], mag[5][min(t + 256, T - 1)], ends)
-        bound[t:t + 256] = mag[5][t] + far + 2 * flow[t:t + 256].sum(0)
+    step = 256 if max(dk, dv) <= 64 else 512
+    for t in range(0, T, step):
+        far = torch.where((torch.tensor(lengths) > t + step)[:, None], mag[5][min(t + step, T - 1)], ends)
+        bound[t:t + step] = mag[5][t] + far + 2 * flow[t:t + step].sum(0)
     bounded(got, want, bound, torch.float32, 2.0 ** -15)
 
 
