@@ -80,12 +80,12 @@ __device__ __forceinline__ void split8(const float (&x)[8], b16x8 (&p)[N])
     for (int k = 0; k < N; ++k) p[k] = __builtin_bit_cast(b16x8, w[k]);
 }
 
-// The products of planes a[i] b[j] that reach the precision of the finer operand, smallest first: f(i, j) does one of them, for
-// all tiles in turn (a matrix instruction that waits for the one before it costs as much as four that do not).
-template <int NA, int NB, typename F>
+// The products of planes a[i] b[j] that reach the precision of the finer operand, or of N planes, smallest first: f(i, j) does one
+// of them, for all tiles in turn (a matrix instruction that waits for the one before it costs as much as four that do not).
+template <int NA, int NB, int N = 1, typename F>
 __device__ __forceinline__ void plane_products(F f)
 {
-    constexpr int M = NA > NB ? NA : NB;
+    constexpr int L = NA > NB ? NA : NB, M = L > N ? L : N;
 #pragma unroll
     for (int s = M - 1; s >= 0; --s)
 #pragma unroll
@@ -480,7 +480,7 @@ struct Pass {
 #pragma unroll
                 for (int J = 0; J < NJ; ++J) yf[J][k] = *reinterpret_cast<const b16x8 *>(y + k * C * DC + at<DC>((J0 + J) * 16 + lr, 32 * s + 8 * lg));
             }
-            plane_products<NP, NP>([&](int i, int j) __attribute__((always_inline)) {
+            plane_products<NP, NP, NC>([&](int i, int j) __attribute__((always_inline)) {
 #pragma unroll
                 for (int J = 0; J < NJ; ++J) p[J] = mfma(yf[J][i], xf[j], p[J]);
             });
@@ -803,7 +803,7 @@ template <typename T, int DC, int DZ, int VEC, bool DOTS> constexpr int resident
 }
 
 // DOTS: the sums of W o as well, x S and the scores to 24 bits for them: with 16 the decays' gradient, an fp32 output, is off by 2.3e-6
-// of its norm for 2000 tokens in bf16 (3.3e-7 with 24), by 6.5e-6 for 11 in fp16 (1.1e-6), at 1025 against 1131 us for 1024 heads of 64.
+// of its norm for 2000 tokens in bf16 (3.3e-7 with 24), by 6.5e-6 for 11 in fp16 (1.3e-7), at 1025 against 1131 us for 1024 heads of 64.
 template <typename T, int DC, int DZ, int VEC, bool DOTS>
 __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ, VEC, DOTS>())) chunk_kernel(const Args a)
 {
