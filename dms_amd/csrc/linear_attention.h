@@ -95,7 +95,7 @@ inline int chunk_tokens(int dtype) { return dtype == DTYPE_BF16 ? 64 : 32; }
 
 // kind, bits:
 constexpr int STATES = 1;      // the states after each segment (from s_in for segment 0, from zero for the others), nothing else
-constexpr int DOTS_PASS = 2;   // the dots of W and o as well where a role wants them, and x S to 24 bits, as they are summed over the sequence
+constexpr int DOTS_PASS = 2;   // the dots of W and o as well where a role wants them
 // DC, DZ (of role[0]) in {32/32, 64/64, 64/128, 128/64, 128/128}.  Returns launch_status.
 template <typename T> int launch_chunks(const Args &a, int DC, int DZ, int kind, hipStream_t stream);
 extern template int launch_chunks<float>(const Args &, int, int, int, hipStream_t);

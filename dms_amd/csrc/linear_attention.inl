@@ -9,10 +9,10 @@
 // is summed in 64 bits and kept as two floats: the difference of two far sums keeps its low bits.
 //
 // All four products run on the bf16 matrix instruction (16x16x32).  An operand of t bits is the sum of bf16 planes
-// (bf16: 1, fp16: 2, fp32: 3; a number that the kernel itself computed: 2, and 3 beside fp32 and wherever the result is an
-// fp32 output or goes into one: the state, the dots W o of the decays' gradient), and a product of two is the sum of the plane
-// products that matter, smallest first, in fp32: 16 bits and more in o of bf16 and fp16 calls, 24 elsewhere.  Six bf16
-// products take 96 cycles where the fp32 instruction takes 256 for the same product.
+// (bf16: 1, fp16: 2, fp32: 3; a number that the kernel itself computed, a score or a state: 3 whatever the call's type), and a
+// product of two is the sum of the plane products that matter, smallest first, in fp32: 24 bits everywhere, so that
+// freezing the decays leaves the other gradients' bits as they are.  Six bf16 products take 96 cycles where the fp32 instruction
+// takes 256 for the same product.
 //
 // A workgroup takes one (sample, head, segment) and walks its chunks with two kinds of waves.  Owners have 16 columns of z each,
 // and with them that part of S, which stays in their accumulators from the first chunk to the last: converted, they are the
@@ -44,11 +44,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-template <typename T> struct Kind;      // planes of an operand of the call's type, and of a computed one
-template <> struct Kind<float> { static constexpr int NP = 3, NC = 3; };
-template <> struct Kind<__bf16> { static constexpr int NP = 1, NC = 2; };
-template <> struct Kind<_Float16> { static constexpr int NP = 2, NC = 2; };
-constexpr int NS = 3;                   // planes of 2^{G_C - G_j} z_j in the state: the state is an fp32 output
+template <typename T> struct Kind;      // planes of an operand of the call's type
+template <> struct Kind<float> { static constexpr int NP = 3; };
+template <> struct Kind<__bf16> { static constexpr int NP = 1; };
+template <> struct Kind<_Float16> { static constexpr int NP = 2; };
+constexpr int NC = 3;                   // planes of a computed one: scores, states, 2^{G_C - G_j} z_j
 
 // two numbers as sums of N bf16 pairs, each the rounded rest of the ones before it
 template <int N>
@@ -386,8 +386,8 @@ template <int C> __device__ __forceinline__ int score(int I, int lr, int col)
     return I < 2 ? at<32>(I * 16 + lr, col) : 32 * 32 + at<C>((I - 2) * 16 + lr, col);
 }
 
-// The part of a chunk that one pass (one Role) does, by its NW waves; x, y, z are LDS tiles of NP planes, what is computed has NC.
-template <typename T, int DC, int DZ, int C, int NW, int NC, bool STATE_ONLY>
+// The part of a chunk that one pass (one Role) does, by its NW waves; x, y, z are LDS tiles of NP planes.
+template <typename T, int DC, int DZ, int C, int NW, bool STATE_ONLY>
 struct Pass {
     static constexpr int NP = Kind<T>::NP;
     static constexpr int NT = DZ / 16 / NW, CT = C / 16, KT = DC / 16;     // tiles of 16: a wave's columns, tokens, rows of S
@@ -584,7 +584,7 @@ struct Pass {
         }
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
-            b16x8 zs[NT][NS];
+            b16x8 zs[NT][NC];
             const int row = 32 * s + 4 * lg;           // slots 4u + i of lane group g are token 32 s + 16 u + 4 g + i
             b16x8 zf[NT][NP];
 #pragma unroll
@@ -620,7 +620,7 @@ struct Pass {
                     for (int k = NP - 2; k >= 0; --k) w[j] += (float)zf[n][k][j];
                     w[j] *= j < 4 ? r0[j % 4] : r1[j % 4];
                 }
-                split8<NS>(w, zs[n]);
+                split8<NC>(w, zs[n]);
             }
             constexpr int TG = KT < 4 ? KT : 4;          // rows of S at a time
 #pragma unroll
@@ -633,7 +633,7 @@ struct Pass {
                         const __bf16 *q = y + k * C * DC + at<DC>(row + lr / 4, 16 * (t0 + t) + 4 * (lr % 4));
                         yf[t][k] = join(read_tr(q), read_tr(q + 16 * DC));
                     }
-                plane_products<NP, NS>([&](int i, int j) __attribute__((always_inline)) {
+                plane_products<NP, NC>([&](int i, int j) __attribute__((always_inline)) {
 #pragma unroll
                     for (int t = 0; t < TG; ++t)
 #pragma unroll
@@ -739,7 +739,7 @@ template <typename T, int DC, int DZ, int VEC>
 __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Args a)
 {
     constexpr int C = chunk<T>(), NW = owners<T, DZ>(), NTHR = 64 * NW, NP = Kind<T>::NP;
-    typedef Pass<T, DC, DZ, C, NW, 1, true> P;
+    typedef Pass<T, DC, DZ, C, NW, true> P;
     struct Shared {
         alignas(16) __bf16 y[NP * C * DC];
         alignas(16) __bf16 z[NP * C * DZ];
@@ -794,25 +794,23 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
 // and cost the memory twice as much).
 // Waves of a SIMD that the LDS leaves room for: two workgroups of 8 where the tiles take less than half of it (rows that are
 // fetched element by element need the registers more).
-template <typename T, int DC, int DZ, int VEC, bool DOTS> constexpr int residents()
+template <typename T, int DC, int DZ, int VEC> constexpr int residents()
 {
-    constexpr int NC = DOTS ? 3 : Kind<T>::NC;
     const int tiles = Kind<T>::NP * chunk<T>() * (4 * DC + DZ) * 2 + 2 * NC * scores_plane<chunk<T>()>() * 2 + 4 * 1024;
     const int waves = owners<T, DZ>() + feeders<T, DZ>();
     return waves / 4 * (VEC && waves == 8 && tiles <= 80 * 1024 ? 2 : 1);
 }
 
-// DOTS: the sums of W o as well, x S and the scores to 24 bits for them: with 16 the decays' gradient, an fp32 output, is off by 2.3e-6
-// of its norm for 2000 tokens in bf16 (3.3e-7 with 24), by 6.5e-6 for 11 in fp16 (1.3e-7), at 1025 against 1131 us for 1024 heads of 64.
+// DOTS: the sums of W o as well.
 template <typename T, int DC, int DZ, int VEC, bool DOTS>
-__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ, VEC, DOTS>())) chunk_kernel(const Args a)
+__global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (residents<T, DC, DZ, VEC>())) chunk_kernel(const Args a)
 {
     constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<T, DZ>(), NTHR = 64 * (NO + NF);
-    constexpr int NP = Kind<T>::NP, NC = DOTS ? 3 : Kind<T>::NC;
+    constexpr int NP = Kind<T>::NP;
     constexpr int ANCHOR = anchor_every(DC * DZ);
     constexpr bool WHOLE = DC == DZ;                 // rows of o fit x's tile
     constexpr int AHEAD = DC <= 64 && DZ <= 64 ? 2 : 1;   // chunks of rows in flight: with 128 columns one is as many bytes, and registers are short
-    typedef Pass<T, DC, DZ, C, NO, NC, false> P;
+    typedef Pass<T, DC, DZ, C, NO, false> P;
     struct Shared {
         alignas(16) __bf16 x[2][NP * C * DC];
         alignas(16) __bf16 y[2][NP * C * DC];

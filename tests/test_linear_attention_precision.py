@@ -1,0 +1,99 @@
+"""What linear attention keeps of its numbers (ops.linear_attention): cases where the result is an exact small number that a
+kernel with fewer bits cannot give, and bounds on the norm of the error.
+"""
+import pytest
+import torch
+
+from dms_amd import ops
+
+DEV = "cuda"
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+# ------------------------------------------------------------------------------------ 24 bits of scores and states
+# 2^20 + 2^10 + 1 takes 21 bits and has gaps too wide for two parts of 8 bits: less 2^20 + 2^10 it is 1, and 0 if its last bit was lost.
+BIG = torch.tensor([1024.0, 32.0, 1.0])
+LESS = torch.tensor([-1024.0, -32.0, 0.0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("width", [16, 48, 64, 128])
+@pytest.mark.parametrize("T,first,second,reader", [(3, 0, 1, 2), (64, 3, 20, 63), (60, 10, 12, 50), (200, 130, 140, 159)])
+def test_scores_keep_24_bits(dtype, width, T, first, second, reader):
+    """Two tokens of one chunk whose scores with a third are 2^20 + 2^10 + 1 and -(2^20 + 2^10): o and the gradients that read
+    them are exactly 1, each asked for alone and with the decays' gradient."""
+    def at(*rows):
+        x = torch.zeros(T, 1, 1, width)
+        for t, r in rows:
+            x[t, 0, 0, :len(r)] = r
+        return x.to(DTYPES[dtype]).to(DEV)
+
+    ones = torch.ones(width)
+    g = torch.zeros(T, 1, 1, device=DEV)
+    with torch.no_grad():
+        o, _ = ops.linear_attention(at((reader, BIG)), at((first, BIG), (second, LESS)), at((first, ones), (second, ones)), g, scale=1.0)
+    assert (o[reader] == 1).all()
+
+    back = (T - 1 - reader, T - 1 - second, T - 1 - first) if T != 200 else (reader - 29, reader - 19, reader)   # reader before the two
+    one, x, y = back
+    zero = at()
+    for leaf, q, k, v, do, token in (
+            ("q", zero, at((first, ones), (second, ones)), at((first, BIG), (second, LESS)), at((reader, BIG)), reader),
+            ("k", at((x, ones), (y, ones)), zero, at((one, BIG)), at((x, BIG), (y, LESS)), one),
+            ("v", at((x, BIG), (y, LESS)), at((one, BIG)), zero, at((x, ones), (y, ones)), one)):
+        for decays in (False, True):
+            args = {"q": q.clone(), "k": k.clone(), "v": v.clone(), "g": g.clone()}
+            args[leaf].requires_grad_()
+            args["g"].requires_grad_(decays)
+            o, _ = ops.linear_attention(**args, scale=1.0)
+            got = torch.autograd.grad(o, [args[leaf]] + ([args["g"]] if decays else []), do)[0]
+            assert (got[token] == 1).all(), (leaf, decays)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("width", [16, 64, 128])
+def test_states_keep_24_bits(dtype, width):
+    """States of 2^20 + 2^10 + 1 and -(2^20 + 2^10), read by a query, a key and a value of ones."""
+    state = torch.zeros(1, 1, width, width, device=DEV)
+    state[0, 0, 0], state[0, 0, 1] = 2.0 ** 20 + 1025, -(2.0 ** 20 + 1024)
+    x = torch.zeros(3, 1, 1, width, device=DEV, dtype=DTYPES[dtype])
+    two = x.clone()
+    two[1, 0, 0, :2] = 1
+    g = torch.zeros(3, 1, 1, device=DEV)
+    with torch.no_grad():
+        o, _ = ops.linear_attention(two, x, x, g, state, scale=1.0)
+    assert (o[1] == 1).all()
+    for decays in (False, True):
+        for leaf in "qkv":
+            args = {n: x.clone() for n in "qkv"}
+            args["g"] = g.clone().requires_grad_(decays)
+            args["state0"] = state.transpose(2, 3).contiguous() if leaf == "q" else torch.zeros_like(state)
+            if leaf != "q":
+                args["v" if leaf == "k" else "k"].copy_(two)
+            args[leaf].requires_grad_()
+            o, s = ops.linear_attention(**args, scale=1.0)
+            ds = torch.zeros_like(s) if leaf == "q" else (state.transpose(2, 3).contiguous() if leaf == "k" else state)
+            got = torch.autograd.grad([o, s], [args[leaf]] + ([args["g"]] if decays else []), [two if leaf == "q" else x, ds])[0]
+            assert (got[1] == 1).all(), (leaf, decays)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("dk,dv,H", [(64, 64, 3), (32, 100, 2), (125, 125, 2), (20, 32, 260)])
+def test_frozen_decays_leave_the_other_gradients_as_they_are(dtype, dk, dv, H):
+    gen = torch.Generator().manual_seed(dk)
+    T, B = 150, 1
+    make = lambda *shape: torch.randn(shape, generator=gen).to(DTYPES[dtype]).to(DEV)  # noqa: E731
+    q, k, v, do = make(T, B, H, dk), make(T, B, H, dk), make(T, B, H, dv), make(T, B, H, dv)
+    g = torch.nn.functional.logsigmoid(torch.randn(T, B, H, generator=gen)).to(DEV)
+    state, ds = (torch.randn(B, H, dk, dv, generator=gen).to(DEV) for _ in range(2))
+    got = []
+    for decays in (False, True):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v, state)]
+        gate = g.clone().requires_grad_(decays)
+        out = ops.linear_attention(*leaves[:3], gate, leaves[3])
+        got.append(torch.autograd.grad(out, leaves + ([gate] if decays else []), [do, ds])[:4])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
