@@ -159,7 +159,7 @@ struct Tile {
         static_assert((NTHR / PER) % 8 == 0, "units have to keep the row's permutation");
         lds = at<D>(reverse ? C - 1 - row : row, c);
         lds_step = (reverse ? -1 : 1) * (NTHR / PER) * D;
-        if (dcol <= 0 || row >= C) row = 1 << 20;
+        if (dcol <= 0 || row >= C) row = 1 << 30;        // behind every token: T <= 2^29, and the units' rows stay far below 2^31
     }
     // tokens t0 .. t0 + n - 1, zeros behind them
     __device__ __forceinline__ void fetch(Flight &f, long long t0, int n) const

@@ -1,0 +1,54 @@
+"""Linear attention (ops.linear_attention) over more than a million tokens and over far rows: padded columns stay zero and
+offsets hold wherever a token lies.
+"""
+import pytest
+import torch
+
+from dms_amd import ops
+
+DEV = "cuda"
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+NAMES = ("q", "k", "v", "g")
+
+
+def recurrence(q, k, v, g, scale):
+    """One sample, one head, float64: o (T, dv)."""
+    S, out = torch.zeros(q.shape[1], v.shape[1], dtype=torch.float64), []
+    for t in range(q.shape[0]):
+        S = S * g[t].exp() + k[t][:, None] * v[t]
+        out.append(scale * (q[t] @ S))
+    return torch.stack(out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dk,dv", [("bf16", 40, 40), ("bf16", 36, 100), ("fp32", 36, 20), ("fp32", 100, 100), ("fp16", 48, 72)])
+def test_columns_behind_a_row_stay_out_of_sequences_of_more_than_2_20_tokens(dtype, dk, dv):
+    """Rows lie in a wider tensor of NaN.  The chunks before the last 2^20 tokens know only their neighbours, as the decays of
+    exp(-1/2) leave e^-100 of a token after 200 others: the ends of the long sequence are the ends of short ones.
+
+    Bound, of the norm over 100 tokens: the output's half step (2^-8, 2^-11, 2^-24) and 2^-16 for the kernel's own sums, which
+    are right to 2^-20 of sums of absolute values that are at most 2^3 of the results' norm here."""
+    T, n, far = (1 << 20) + 700, 100, 300
+    gen = torch.Generator(device=DEV).manual_seed(dk)
+
+    def rows(d):
+        room = torch.full((T, 1, 1, d + 8), float("nan"), dtype=DTYPES[dtype], device=DEV)
+        room[..., :d] = torch.randn(T, 1, 1, d, generator=gen, device=DEV).to(DTYPES[dtype])
+        return room[..., :d]
+
+    dev = {"q": rows(dk), "k": rows(dk), "v": rows(dv), "g": torch.full((T, 1, 1), -0.5, device=DEV)}
+    do = rows(dv)
+    leaves = [dev[x].requires_grad_() for x in NAMES]
+    o, s = ops.linear_attention(**dev)
+    got = [o] + list(torch.autograd.grad(o, leaves, do))
+    for name, x in zip(("o",) + NAMES, got):
+        assert torch.isfinite(x).all(), name
+    assert torch.isfinite(s).all()
+    scale, bound = dk ** -0.5, torch.finfo(DTYPES[dtype]).eps / 2 + 2.0 ** -16
+    for lo, hi, first in ((0, far, 0), (T - far, T, far - n)):                # the first n tokens, the last n
+        short = [dev[x][lo:hi, 0, 0].detach().cpu().double().requires_grad_() for x in NAMES]
+        want = recurrence(*short, scale)
+        grads = torch.autograd.grad(want, short, do[lo:hi, 0, 0].cpu().double())
+        for name, x, y in zip(("o",) + NAMES, got, (want.detach(),) + grads):
+            x, y = x[lo:hi, 0, 0].detach().cpu().double()[first:first + n], y[first:first + n]
+            assert float((x - y).norm()) <= bound * float(y.norm()), (name, lo, float((x - y).norm() / y.norm()))
