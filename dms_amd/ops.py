@@ -12,6 +12,7 @@ import os
 import tempfile
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -38,6 +39,14 @@ def _chk(name, t, shape=None):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _no_tangents(name, *tensors):
+    """Refuses the dual tensors of torch.autograd.forward_ad: they need no gradient, so that a call would go past the autograd
+    function, and its result without a tangent would count as constant."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("dms_amd.%s: no forward-mode derivatives (an input has a tangent); backward ones exist" % name)
 
 
 def _chk_batch_strided(name, t, shape=None):
@@ -140,6 +149,7 @@ def tuned_matmul(a, b, acc=None, out=None):
     reproducible within a process and may differ in the last bits between processes.
     DMN_GEMM_TUNE=0 disables the timing (always rocBLAS).  Inference only (operands detached:
     torch.matmul folds -- and copies -- a broadcast operand that requires grad)."""
+    _no_tangents("tuned_matmul", a, b)                   # detached, they would be lost
     a, b = a.detach(), b.detach()
     key = (tuple(a.shape), tuple(b.shape), a.device.index)
     prev = torch.backends.cuda.preferred_blas_library()
@@ -922,12 +932,13 @@ def linear_attention(q, k, v, g, state0=None, lengths=None, scale=None):
     reads head h // (H // Hq) of q, and so on.  Head widths up to 128, B * H up to 2^17, tokens up to 2^24 elements apart.  state0 (B, H, dk, dv) float32 or None (zeros);
     lengths (B,) int32 or int64 on the device, or None: tokens of each sample, rows behind them are neither read nor do
     they change the state, and their outputs and gradients are zero.  scale: dk ** -0.5 if None.
-    Returns o (T, B, H, dv) and the state (B, H, dk, dv) after the last token, both under autograd (once)."""
+    Returns o (T, B, H, dv) and the state (B, H, dk, dv) after the last token, both under autograd (once; backward mode only)."""
     name = "linear_attention"
     if not torch.is_tensor(g) or g.dim() not in (1, 3):
         raise RuntimeError("dms_amd.%s: g must be (T, B, H) or (H,)" % name)
     if not torch.is_tensor(q) or q.dim() != 4:
         raise RuntimeError("dms_amd.%s: q must be (T, B, heads, width)" % name)
+    _no_tangents(name, q, k, v, g, state0)
     T, B, H = q.shape[0], q.shape[1], g.shape[-1]
     _chk_heads(name, q, k, v, H)
     if not g.is_cuda or g.dtype != torch.float32 or g.device != q.device or (g.dim() == 3 and g.shape != (T, B, H)):
@@ -957,6 +968,7 @@ def linear_attention_step(q, k, v, g, state, scale=None):
         raise RuntimeError("dms_amd.%s: g must be (B, H) or (H,)" % name)
     if not torch.is_tensor(q) or q.dim() != 3:
         raise RuntimeError("dms_amd.%s: q must be (B, heads, width)" % name)
+    _no_tangents(name, q, k, v, g, state)
     B, H = q.shape[0], g.shape[-1]
     _chk_heads(name, q, k, v, H)
     dk, dv = q.shape[2], v.shape[2]
@@ -1045,7 +1057,7 @@ class _HeadNormRotary(torch.autograd.Function):
 
 
 def head_norm_rotary(q, k, q_weight, k_weight, positions, sections, base=10000.0, eps=1e-6):
-    """RMS norm of every query and key head, then its rotation by positions on several axes, in one pass; under autograd (once).
+    """RMS norm of every query and key head, then its rotation by positions on several axes, in one pass; under autograd (once; backward mode only).
 
     q (T, B, Hq, D), k (T, B, Hk, D) in float32, bfloat16 or float16, unit stride along the last axis; D up to 256.
     q_weight, k_weight (D,) in float32 or the type of q (both alike), or None.  positions (T, B, axes), or (T, axes) for all
@@ -1056,6 +1068,7 @@ def head_norm_rotary(q, k, q_weight, k_weight, positions, sections, base=10000.0
     name = "head_norm_rotary"
     if not torch.is_tensor(q) or q.dim() != 4 or q.dtype not in _DTYPE_IDS:
         raise RuntimeError("dms_amd.%s: q must be a float32, bfloat16 or float16 tensor (T, B, heads, width)" % name)
+    _no_tangents(name, q, k, q_weight, k_weight)
     T, B, Hq, D = q.shape
     _chk_rows(name, "q", q, q.shape, q.dtype, q.device)
     if not torch.is_tensor(k) or k.dim() != 4:
