@@ -352,7 +352,8 @@ class _SRUCompute(torch.autograd.Function):
 
 
 def sru_compute(u, x, bias, c0=None, act="tanh", scale_x=1.0, h_t0=0):
-    """h, c_last = scan(u, x).  With autograd: full h is produced, then sliced."""
+    """h, c_last = scan(u, x).  With autograd (backward mode only): full h is produced, then sliced."""
+    _no_tangents("sru_compute", u, x, bias, c0)
     needs_grad = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (u, x, bias, c0))
     if needs_grad:
