@@ -22,17 +22,16 @@ struct Role {
     float *s_out;                 // state after the last step, the same with out_c / out_z, or null
     int in_c, in_z, out_c, out_z;
     float *dots;                  // (B, H, T) or null
-    float *keep;                  // with dots: the states that meet another role's at every anchor_every()-th token, or null
+    float *keep;                  // with dots: the states that meet another role's at every ANCHOR-th token, or null
     float scale_p, scale_x, scale_z;   // of the products inside a chunk, of x S, and of z in the state
     int reverse;                  // 1: time runs backwards; step s decays by the g of the token after it
     int last_decay;               // 1: s_out is decayed by g of token 0 as well
 };
 
-// The gradient of the decays is known from the two states that meet there at every so many tokens, a multiple of both chunks:
-// a state of 128 x 128 is worth more tokens than one of 64 x 64 (all gradients of 256 heads of 128 x 128, 2000 tokens: 512 apart 1381 us
-// in fp32 and 742 in bf16, decays' gradient off by 6.2e-7 of its norm; 256 apart 1429, 791 and 4.2e-7 to 4.9e-7).
-constexpr int anchor_every(int state_floats) { return state_floats > 64 * 128 ? 512 : 256; }
-__host__ __device__ inline int anchors(int T, int every) { return T > 0 ? (T - 1) / every : 0; }
+// The gradient of the decays is known from the two states that meet there at every so many tokens, a multiple of both chunks (with
+// every 512th, 256 heads of 128 x 128 and 2000 tokens: 2 to 6 % less time, 1.4 times the error).
+constexpr int ANCHOR = 256;
+__host__ __device__ inline int anchors(int T) { return T > 0 ? (T - 1) / ANCHOR : 0; }
 
 struct Args {
     Role role[3];

@@ -67,7 +67,7 @@ __device__ __forceinline__ double block_sum(double v, double *sh)
 // an earlier token s less what the tokens between took out of the keys' side over the queries':
 //   dg_t = dg_s - sum_{s <= i < t} (q_i . dq_i - k_i . dk_i)
 // The dots are right to fp32, and their running sum walks away from the truth with the root of the distance.  So dg is known
-// directly at every anchor_every()-th token, from the two states that meet there, at the first (<S_0, dS_0>) and behind the last
+// directly at every ANCHOR-th token, from the two states that meet there, at the first (<S_0, dS_0>) and behind the last
 // (<S_T, dS_T>; not without anchors: 512 heads of 125 x 125 would pay 20 us for 20 tokens): a sum starts at each and what it
 // misses at the next is spread over the way (2046 tokens: an error of 2.2e-6 of the norm without, 4.4e-7 with).
 //
@@ -89,12 +89,11 @@ __global__ void __launch_bounds__(256) meet_kernel(const f32x4 *before, const f3
 }
 
 // workgroups of a (sample, head) in the scan below
-__host__ __device__ static inline int stretches(int T, int every) { return (T + 4 * every - 1) / (4 * every); }
+__host__ __device__ static inline int stretches(int T) { return (T + 4 * ANCHOR - 1) / (4 * ANCHOR); }
 
 // A wave for each stretch between anchors, four a workgroup, in 64 bits; the result takes the dots' place, or its sum goes to
 // `part`: g and dg have the heads together, and 4 bytes of every line would be written from here (44 us for 1024 heads of 2000
 // tokens; this takes 16, the turn below 17).
-template <int ANCHOR>
 __global__ void __launch_bounds__(256)
 decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const float *s0, const float *ds0, const float *s_end, const float *ds_end,
                   const float *g, long long gt, long long gb, long long gh, const void *lengths, int lengths64, float *part, int T, int B, int H, int n)
@@ -102,7 +101,7 @@ decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const 
     constexpr int N = ANCHOR / 64;                         // tokens a lane
     __shared__ double sh[4];
     const int bh = blockIdx.x % (B * H), at = blockIdx.x / (B * H), b = bh / H, h = bh % H, tid = threadIdx.x, lane = tid & 63;
-    const int n_anchor = anchors(T, ANCHOR), len = valid_length(lengths, lengths64, b, T);
+    const int n_anchor = anchors(T), len = valid_length(lengths, lengths64, b, T);
     const float *pg = g + b * gb + h * gh;
     const auto meet = [&](const float *x, const float *y) {
         double v = 0.0;
@@ -147,7 +146,7 @@ decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const 
     }
     if (part) {
         sum = block_sum<256>(sum, sh);
-        if (tid == 0) part[(size_t)bh * stretches(T, ANCHOR) + at] = log2_decay(pg[0]) < -149.0 ? 0.0f : (float)sum;
+        if (tid == 0) part[(size_t)bh * stretches(T) + at] = log2_decay(pg[0]) < -149.0 ? 0.0f : (float)sum;
     }
 }
 
@@ -361,7 +360,7 @@ static void fill_common(Args &a, const float *g, const long long *gs, const void
 
 // the backward's passes: where each one's piece of the workspace begins
 struct BwdPlan {
-    int DK, DV, every;
+    int DK, DV;
     long long passes, keep[2], flow, dots, dq, dk, dv, ds0, end, part, total;
 };
 
@@ -379,16 +378,15 @@ static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, 
     }
     const auto take = [&at](long long n) { const long long o = at; at += up4(n); return o; };
     p.passes = take(most);                                 // of two launches the second begins when the first is done with it
-    p.every = anchor_every(p.DK * p.DV);
-    for (long long &keep : p.keep) keep = take(BH * anchors(T, p.every) * p.DK * p.DV);
-    p.flow = take(2 * BH * anchors(T, p.every));                    // doubles
+    for (long long &keep : p.keep) keep = take(BH * anchors(T) * p.DK * p.DV);
+    p.flow = take(2 * BH * anchors(T));                    // doubles
     p.dots = take(2 * rows);
     p.dq = take(Hq < H ? rows * dk : 0);
     p.dk = take(Hk < H ? rows * dk : 0);
     p.dv = take(Hv < H ? rows * dv : 0);
     p.ds0 = take(BH * dk * dv);
-    p.end = take(anchors(T, p.every) > 0 ? BH * dk * dv : 0);
-    p.part = take(BH * stretches(T, p.every));
+    p.end = take(anchors(T) > 0 ? BH * dk * dv : 0);
+    p.part = take(BH * stretches(T));
     p.total = at;
     return p;
 }
@@ -516,7 +514,7 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         t.f32 = 1;
         return t;
     };
-    const bool meet = grad_g && anchors(T, p.every) > 0;           // states of dq and dk between the first and the last
+    const bool meet = grad_g && anchors(T) > 0;           // states of dq and dk between the first and the last
     float *const end = meet && grad_state ? workspace + p.end : nullptr;
     Role role[3] = {};
     int n = 0;
@@ -583,22 +581,21 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
     }
     if (grad_g) {
         float *part = grad_g_per_head ? workspace + p.part : nullptr;
-        const int ns = stretches(T, p.every);
+        const int ns = stretches(T);
         if (part && T == 0) {
             decay_grad_heads_kernel<<<(unsigned)H, 64, 0, st>>>(nullptr, grad_g, 0, H, 1);
             return launch_status("linear_attention decay gradient");
         }
         double *flow = reinterpret_cast<double *>(workspace + p.flow);
         if (meet) {
-            meet_kernel<<<(unsigned)(B * H * anchors(T, p.every)), 256, 0, st>>>(reinterpret_cast<const f32x4 *>(workspace + p.keep[0]),
+            meet_kernel<<<(unsigned)(B * H * anchors(T)), 256, 0, st>>>(reinterpret_cast<const f32x4 *>(workspace + p.keep[0]),
                                                                         reinterpret_cast<const f32x4 *>(workspace + p.keep[1]), flow, p.DK * p.DV / 4);
             rc = launch_status("linear_attention decay gradient");
             if (rc) return rc;
         }
         if (T > 0) {
-            const auto scan = p.every == 256 ? decay_scan_kernel<256> : decay_scan_kernel<512>;
-            scan<<<(unsigned)(B * H * ns), 256, 0, st>>>(dots, dots + (size_t)T * B * H, flow, state0, ds0, end, grad_state, g, a.gt, a.gb, a.gh, lengths,
-                                                         lengths64, part, T, B, H, dk * dv);
+            decay_scan_kernel<<<(unsigned)(B * H * ns), 256, 0, st>>>(dots, dots + (size_t)T * B * H, flow, state0, ds0, end, grad_state, g, a.gt, a.gb,
+                                                                      a.gh, lengths, lengths64, part, T, B, H, dk * dv);
         }
         rc = launch_status("linear_attention decay gradient");
         if (rc) return rc;

@@ -807,7 +807,6 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
 {
     constexpr int C = chunk<T>(), NO = owners<T, DZ>(), NF = feeders<T, DZ>(), NTHR = 64 * (NO + NF);
     constexpr int NP = Kind<T>::NP;
-    constexpr int ANCHOR = anchor_every(DC * DZ);
     constexpr bool WHOLE = DC == DZ;                 // rows of o fit x's tile
     constexpr int AHEAD = DC <= 64 && DZ <= 64 ? 2 : 1;   // chunks of rows in flight: with 128 columns one is as many bytes, and registers are short
     typedef Pass<T, DC, DZ, C, NO, false> P;
@@ -901,7 +900,7 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         const Rows<T, C, VEC> out(ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg), wrows(DOTS && dots ? ro.W : ro.O, w.b, w.h, reverse, lr, z0 + 4 * lg);
         const bool fresh = w.seg == 0 && !ro.s_in, leaves = ro.s_out && w.seg == a.nseg - 1;
         P ps;
-        f32x4 *const keep = reinterpret_cast<f32x4 *>(held(DOTS && ro.keep ? ro.keep + (size_t)w.bh * anchors(a.T, ANCHOR) * (DC * DZ) : nullptr));
+        f32x4 *const keep = reinterpret_cast<f32x4 *>(held(DOTS && ro.keep ? ro.keep + (size_t)w.bh * anchors(a.T) * (DC * DZ) : nullptr));
         ps.zero();
         ps.zero_rows();                                  // for good where the owner has no columns: its dots are 0
         if (w.seg == 0) {

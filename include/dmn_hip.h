@@ -430,7 +430,7 @@ int dmn_linear_attention_fwd(int dtype, const void *q, const void *k, const void
  *            of shared heads: the sum over the heads that read them, in head order.
  *   grad_g   (T,B,H) contiguous, or (H) with grad_g_per_head = 1 (summed over t and b, always in the same order), or NULL.  Zero
  *            where exp(g) is zero in 32 bits.  It is the difference of what queries and keys give back, so that its error goes by
- *            the sizes of q . grad_q and k . grad_k, summed over at most 512 tokens: at every 256th (wide states: 512th) it is known from two states.
+ *            the sizes of q . grad_q and k . grad_k, summed over at most 256 tokens: at every 256th it is known from two states.
  *   workspace  dmn_linear_attention_workspace_floats(dtype, 1, ...) floats, 16-byte aligned.
  * No atomics: the same inputs give the same bits.
  */

@@ -97,3 +97,53 @@ def test_frozen_decays_leave_the_other_gradients_as_they_are(dtype, dk, dv, H):
         got.append(torch.autograd.grad(out, leaves + ([gate] if decays else []), [do, ds])[:4])
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------ the decays' gradient
+def recurrence(q, k, v, g, state, scale):
+    """One head, float64: q, k (T, B, dk), v (T, B, dv), g (T, B), state (B, dk, dv); returns o, state."""
+    out = []
+    for t in range(q.shape[0]):
+        state = state * g[t].exp()[:, None, None] + k[t][:, :, None] * v[t][:, None, :]
+        out.append(scale * (q[t][:, :, None] * state).sum(1))
+    return torch.stack(out), state
+
+
+def recurrence_grads(args, scale, do, ds):
+    leaves = [x.clone().requires_grad_() for x in args]
+    o, s = recurrence(*leaves, scale)
+    return [o.detach(), s.detach()] + list(torch.autograd.grad((o * do).sum() + (s * ds).sum(), leaves))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("dk,dv", [(24, 16), (64, 64), (64, 100), (100, 128), (128, 128)])
+def test_decays_gradient_does_not_carry_errors_past_a_256th_token(dtype, dk, dv):
+    """Tokens 0 to 249 are 2^6 times the others in q, k, v and their output's gradient, their dots 2^24 times; a reset behind
+    them.  From token 256 on the gradient starts anew from the states that meet there, so that it is right to 2^-15 of the
+    magnitudes of its own 256 tokens (derived for the gradient far from either end: twice the dots' errors, and the two ends')."""
+    T, B = 600, 1
+    gen = torch.Generator().manual_seed(dk + dv)
+    make = lambda *shape: torch.randn(shape, generator=gen)  # noqa: E731
+    q, k, v, do, ds, state = make(T, B, dk), make(T, B, dk), make(T, B, dv), make(T, B, dv), make(B, dk, dv), make(B, dk, dv)
+    for x in (q, k, v, do):
+        x[:250] *= 64
+    q, k, v, do = (x.to(DTYPES[dtype]) for x in (q, k, v, do))
+    g = 0.1 * torch.nn.functional.logsigmoid(make(T, B))
+    g[250] = -1e4                                              # a reset that autograd in 64 bits has a gradient of: 0
+    dev = [x.unsqueeze(2).to(DEV) for x in (q, k, v, g)] + [state.unsqueeze(1).to(DEV)]
+    dev[3].requires_grad_()
+    out = ops.linear_attention(*dev)
+    got, = torch.autograd.grad(out, [dev[3]], [do.unsqueeze(2).to(DEV), ds.unsqueeze(1).to(DEV)])
+    args = [x.double() for x in (q, k, v, g, state)]
+    scale = dk ** -0.5
+    want = recurrence_grads(args, scale, do.double(), ds.double())[5]
+    size = [x if i == 3 else x.abs() for i, x in enumerate(args)]
+    mag = recurrence_grads(size, scale, do.double().abs(), ds.double().abs())
+    flow = (size[0] * mag[2] + size[1] * mag[3]).sum(-1)
+    for t in (256, 512):
+        end = min(t + 256, T)
+        far = mag[5][end] if end < T else (mag[1] * ds.double().abs()).sum((-1, -2))
+        bound = mag[5][t] + far + 2 * flow[t:end].sum(0)
+        over = (got[t:end, :, 0].cpu().double() - want[t:end]).abs() - (2.0 ** -15 * bound + 2.0 ** -24 * want[t:end].abs())
+        assert float(over.max()) <= 0.0, (t, float(over.max()))
