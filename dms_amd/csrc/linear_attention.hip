@@ -96,7 +96,7 @@ __host__ __device__ static inline int stretches(int T) { return (T + 4 * ANCHOR 
 // tokens; this takes 16, the turn below 17).
 __global__ void __launch_bounds__(256)
 decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const float *s0, const float *ds0, const float *s_end, const float *ds_end,
-                  const float *g, long long gt, long long gb, long long gh, const void *lengths, int lengths64, float *part, int T, int B, int H, int n)
+                  const float *g, long long gt, long long gb, long long gh, const void *lengths, int lengths64, double *part, int T, int B, int H, int n)
 {
     constexpr int N = ANCHOR / 64;                         // tokens a lane
     __shared__ double sh[4];
@@ -146,7 +146,7 @@ decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const 
     }
     if (part) {
         sum = block_sum<256>(sum, sh);
-        if (tid == 0) part[(size_t)bh * stretches(T) + at] = log2_decay(pg[0]) < -149.0 ? 0.0f : (float)sum;
+        if (tid == 0) part[(size_t)bh * stretches(T) + at] = log2_decay(pg[0]) < -149.0 ? 0.0 : sum;
     }
 }
 
@@ -173,10 +173,10 @@ decay_turn_kernel(const float *scan, const float *g, long long gt, long long gb,
 }
 
 // one decay for each head: its gradient is the sum over samples and stretches, a wave for each head, always in the same order
-__global__ void __launch_bounds__(64) decay_grad_heads_kernel(const float *part, float *out, int B, int H, int stretches)
+__global__ void __launch_bounds__(64) decay_grad_heads_kernel(const double *part, float *out, int B, int H, int stretches)
 {
     double s = 0.0;
-    for (int e = threadIdx.x; e < B * stretches; e += 64) s += (double)part[((size_t)(e / stretches) * H + blockIdx.x) * stretches + e % stretches];
+    for (int e = threadIdx.x; e < B * stretches; e += 64) s += part[((size_t)(e / stretches) * H + blockIdx.x) * stretches + e % stretches];
     s = lane_sums(s);
     if (threadIdx.x == 63) out[blockIdx.x] = (float)s;
 }
@@ -386,7 +386,7 @@ static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, 
     p.dv = take(Hv < H ? rows * dv : 0);
     p.ds0 = take(BH * dk * dv);
     p.end = take(anchors(T) > 0 ? BH * dk * dv : 0);
-    p.part = take(BH * stretches(T));
+    p.part = take(2 * BH * stretches(T));                  // doubles: what they add up to may be far smaller than each
     p.total = at;
     return p;
 }
@@ -580,7 +580,7 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         if (rc) return rc;
     }
     if (grad_g) {
-        float *part = grad_g_per_head ? workspace + p.part : nullptr;
+        double *part = grad_g_per_head ? reinterpret_cast<double *>(workspace + p.part) : nullptr;
         const int ns = stretches(T);
         if (part && T == 0) {
             decay_grad_heads_kernel<<<(unsigned)H, 64, 0, st>>>(nullptr, grad_g, 0, H, 1);

@@ -147,3 +147,31 @@ def test_decays_gradient_does_not_carry_errors_past_a_256th_token(dtype, dk, dv)
         bound = mag[5][t] + far + 2 * flow[t:end].sum(0)
         over = (got[t:end, :, 0].cpu().double() - want[t:end]).abs() - (2.0 ** -15 * bound + 2.0 ** -24 * want[t:end].abs())
         assert float(over.max()) <= 0.0, (t, float(over.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("T", [901, 1301])
+def test_gradient_of_one_decay_for_each_head_sums_in_64_bits(dtype, T):
+    """Whole numbers in one column, no decay: every token's gradient is a whole number below 2^24, each sample's sum is beyond
+    it, and the samples cancel down to a number that 32 bits hold again: the result is exact only if no sum was rounded."""
+    B, H, width = 2, 3, 16
+    def ones(sign=None):                                       # noqa: E306
+        x = torch.zeros(T, B, H, width)
+        x[..., 0] = 1
+        if sign is not None:
+            x[:, 1, :, 0] = sign
+        return x
+    k, do = ones(), ones(-1.0)
+    k[0, 1, :, 0] = 2
+    S, R = k[..., 0].double().cumsum(0), do[..., 0].double().flip(0).cumsum(0).flip(0)
+    tokens = torch.cat([torch.zeros(1, B, H, dtype=torch.float64), S[:-1] * R[1:]])
+    parts = tokens.sum(0)
+    want = parts.sum(0)
+    assert float(tokens.abs().max()) < 2 ** 24 and float(parts.abs().min()) > 2 ** 24 and float(want.abs().max()) < 2 ** 24
+    assert (parts.float().double().sum(0) != want).all()       # with sums in 32 bits the test would not hold
+    q, k, v, do = (x.to(DTYPES[dtype]).to(DEV) for x in (ones(), k, ones(), do))
+    g = torch.zeros(H, device=DEV, requires_grad=True)
+    o, _ = ops.linear_attention(q, k, v, g, scale=1.0)
+    got, = torch.autograd.grad(o, g, do)
+    assert torch.equal(got.cpu().double(), want)
