@@ -41,7 +41,7 @@ struct Args {
     int lengths64;
     int T, B, H, nroles, nseg, seg_chunks;
     float *states;                // nseg > 1: (nroles, B*H, nseg) states, each in the kernel's own order
-    float *decays;                // nseg > 1: (nroles, B*H, nseg) decay over a segment
+    double *decays;               // nseg > 1: (nroles, B*H, nseg) decay over a segment
 };
 
 __device__ __forceinline__ int valid_length(const void *lengths, int lengths64, int b, int T)

@@ -6,21 +6,22 @@ namespace dmn {
 namespace la {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // states[seg] = state after segment seg, from what each segment added: one thread for 4 elements of the state, in
 // segment order (at most a few dozen), so the same bits every time.  8 segments are loaded at a time: what this costs is the
 // loads' latency (16 heads of 64 x 64 in 40 segments: one load at a time 15 us, so 5).
-__global__ void __launch_bounds__(64) combine_kernel(float *states, const float *decays, int nseg, int n4, long long total)
+__global__ void __launch_bounds__(64) combine_kernel(float *states, const double *decays, int nseg, int n4, long long total)
 {
     const long long e = (long long)blockIdx.x * 64 + threadIdx.x;
     if (e >= total) return;
     const long long row = e / n4;
     f32x4 *p = reinterpret_cast<f32x4 *>(states) + row * nseg * n4 + e % n4;
-    const float *d = decays + row * nseg;
-    f32x4 s = p[0];
+    const double *d = decays + row * nseg;
+    f64x4 s = __builtin_convertvector(p[0], f64x4);        // rounded where it is kept, not where it goes on
     for (int i = 1; i < nseg - 1; i += 8) {
         f32x4 add[8];
-        float decay[8];
+        double decay[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int at = i + k < nseg - 1 ? i + k : nseg - 2;
@@ -30,8 +31,8 @@ __global__ void __launch_bounds__(64) combine_kernel(float *states, const float 
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             if (i + k < nseg - 1) {
-                s = s * decay[k] + add[k];
-                p[(long long)(i + k) * n4] = s;
+                s = s * decay[k] + __builtin_convertvector(add[k], f64x4);
+                p[(long long)(i + k) * n4] = __builtin_convertvector(s, f32x4);
             }
     }
 }
@@ -311,7 +312,7 @@ static int run_passes(int dtype, Args &a, int DC, int DZ, int kind, float *ws, h
     if (a.nseg > 1) {
         const long long rows = (long long)a.nroles * a.B * a.H;
         a.states = ws;
-        a.decays = ws + rows * a.nseg * DC * DZ;
+        a.decays = reinterpret_cast<double *>(ws + rows * a.nseg * DC * DZ);
         int rc = launch(dtype, a, DC, DZ, kind | STATES, stream);
         if (rc) return rc;
         if (a.nseg > 2) {
@@ -327,7 +328,7 @@ static int run_passes(int dtype, Args &a, int DC, int DZ, int kind, float *ws, h
 
 static long long passes_floats(int nroles, long long BH, int nseg, int DC, int DZ)
 {
-    return nseg > 1 ? up4((long long)nroles * BH * nseg * DC * DZ) + up4((long long)nroles * BH * nseg) : 0;
+    return nseg > 1 ? up4((long long)nroles * BH * nseg * DC * DZ) + up4(2LL * nroles * BH * nseg) : 0;
 }
 
 static int check(const char *who, int dtype, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)

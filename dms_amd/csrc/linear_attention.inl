@@ -262,7 +262,7 @@ struct alignas(16) Decays {
     float Gh[C], Gl[C];        // G_i as two floats
     float E[C], R[C];          // 2^{G_i} scale_x, 2^{G_C - G_i} scale_z
     float F[C];                // 2^{G_e - G_i}, e the last row of i's 16
-    float tot;                 // 2^{G_C}
+    float tot, tot_rest;       // 2^{G_C} as two floats: it meets the state at every chunk, where a lasting decay's rounding would add up
 };
 
 // the log decay of a lane's step: of its token, or backwards of the token after it
@@ -271,6 +271,24 @@ __device__ __forceinline__ float fetch_decay(const float *pg, long long gt, int 
 {
     const int t = reverse ? t0 + C - lane : t0 + lane;
     return lane < C && t < len ? pg[(long long)t * gt] : 0.0f;
+}
+
+// 2^x as two floats where it lasts, |x| < 1/2: 1 + y + (y^2/2 + y^3/6 + ..), y = x ln 2, whose last term here leaves 2^-27.  A state
+// that decays faster meets it a few times only, and one float does.
+__device__ __forceinline__ void exp2_pair(double x, float &high, float &rest)
+{
+    const double y = x * 0.69314718055994530942;
+    const float yh = (float)y, one = 1.0f + yh;
+    float p = 1.0f / 5040;
+    p = __builtin_fmaf(p, yh, 1.0f / 720);
+    p = __builtin_fmaf(p, yh, 1.0f / 120);
+    p = __builtin_fmaf(p, yh, 1.0f / 24);
+    p = __builtin_fmaf(p, yh, 1.0f / 6);
+    p = __builtin_fmaf(p, yh, 0.5f);
+    const float more = (yh - (one - 1.0f)) + __builtin_fmaf(p, yh * yh, (float)(y - (double)yh)), h = one + more;
+    const bool lasts = fabsf(yh) < 0.34657359f;
+    high = lasts ? h : fast_exp2((float)x);
+    rest = lasts ? more - (h - one) : 0.0f;
 }
 
 // one wave; returns G_C
@@ -288,7 +306,7 @@ __device__ __forceinline__ double decays(float g, int lane, float scale_x, float
         d.E[lane] = fast_exp2(hi) * scale_x;
         d.R[lane] = fast_exp2((float)(tot - G)) * scale_z;
         d.F[lane] = fast_exp2((float)(end - G));
-        if (lane == 0) d.tot = fast_exp2((float)tot);
+        if (lane == 0) exp2_pair(tot, d.tot, d.tot_rest);
     }
     return tot;
 }
@@ -576,11 +594,13 @@ struct Pass {
     __device__ __forceinline__ void from_chunk(const __bf16 *y, const __bf16 *z, const __bf16 *P, const Decays<C> &d, int z0, int lr, int lg)
     {
         if (UPDATE) {
-            const float tot = d.tot;
+            const float tot = d.tot, rest = d.tot_rest;
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) S[t][n] *= tot;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[t][n][i] = __builtin_fmaf(S[t][n][i], tot, S[t][n][i] * rest);
         }
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
@@ -782,7 +802,7 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
     }
     f32x4 *const states = reinterpret_cast<f32x4 *>(a.states + ((size_t)(w.ri * BH + w.bh) * a.nseg + w.seg) * (DC * DZ)) + wave * P::KT * P::NT * 64 + lane;
     ps.save(states);
-    if (tid == NTHR - 64) a.decays[(size_t)(w.ri * BH + w.bh) * a.nseg + w.seg] = fast_exp2((float)gsum);
+    if (tid == NTHR - 64) a.decays[(size_t)(w.ri * BH + w.bh) * a.nseg + w.seg] = exp2(gsum);
 }
 
 // One pass.  The first waves own the state's columns, the others feed them: they fetch and lay out the tiles, keep the

@@ -175,3 +175,33 @@ def test_gradient_of_one_decay_for_each_head_sums_in_64_bits(dtype, T):
     o, _ = ops.linear_attention(q, k, v, g, scale=1.0)
     got, = torch.autograd.grad(o, g, do)
     assert torch.equal(got.cpu().double(), want)
+
+
+# ------------------------------------------------------------------------------------ decays that last
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,chunk", [("bf16", 64), ("fp32", 32), ("fp16", 32)])
+@pytest.mark.parametrize("H,chunks", [(256, 1024), (1, 4096)])
+def test_one_decay_for_every_token_does_not_add_up_its_rounding(dtype, chunk, H, chunks):
+    """A state that only decays, by the same factor for every chunk, forwards and (its gradient) backwards, in one piece and cut
+    into segments.  The factor is one that 32 bits miss by a quarter of a step, 2^-26, or more: kept there, it is off by
+    chunks * 2^-26 after them.  What remains is a rounding of the state for each chunk, at most 2^-24 and of either sign over its
+    elements: sqrt(chunks) * 2^-24 of the norm."""
+    T, width = chunks * chunk, 16
+    for i in range(1000):                                      # until the chunk's factor lies that far from a float
+        g = torch.full((H,), -8.0 / T * (1 + i / 1000))
+        factor = (chunk * g[0].double()).exp()
+        if 2.0 ** -26 <= abs(float(factor.float().double() / factor - 1)):
+            break
+    else:
+        raise AssertionError("no such decay")
+    gen = torch.Generator().manual_seed(1)
+    state, ds = (torch.randn(1, H, width, width, generator=gen).to(DEV) for _ in range(2))
+    x = torch.zeros(1, 1, 1, width, dtype=DTYPES[dtype], device=DEV).expand(T, 1, H, width)
+    state.requires_grad_()
+    _, s = ops.linear_attention(x, x, x, g.to(DEV), state)
+    grad, = torch.autograd.grad(s, state, ds)
+    whole = (T * g[0].double()).exp()
+    for got, start in ((s, state), (grad, ds)):
+        want = start.detach().double().cpu() * whole
+        off = (got.detach().cpu().double() - want).norm() / want.norm()
+        assert float(off) <= chunks ** 0.5 * 2.0 ** -24, float(off)
