@@ -593,15 +593,7 @@ struct Pass {
     template <bool UPDATE>
     __device__ __forceinline__ void from_chunk(const __bf16 *y, const __bf16 *z, const __bf16 *P, const Decays<C> &d, int z0, int lr, int lg)
     {
-        if (UPDATE) {
-            const float tot = d.tot, rest = d.tot_rest;
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) S[t][n][i] = __builtin_fmaf(S[t][n][i], tot, S[t][n][i] * rest);
-        }
+        const float tot = d.tot, rest = d.tot_rest;
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
             b16x8 zs[NT][NC];
@@ -642,10 +634,15 @@ struct Pass {
                 }
                 split8<NC>(w, zs[n]);
             }
-            constexpr int TG = KT < 4 ? KT : 4;          // rows of S at a time
+            constexpr int TG = 2;                        // rows of S at a time: with 4 the registers of 16 waves do not do
 #pragma unroll
             for (int t0 = 0; t0 < KT; t0 += TG) {
                 b16x8 yf[TG][NP];
+                f32x4 add[TG][NT];                       // apart from S: every product would round it
+#pragma unroll
+                for (int t = 0; t < TG; ++t)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) add[t][n] = (f32x4){0, 0, 0, 0};
 #pragma unroll
                 for (int t = 0; t < TG; ++t)
 #pragma unroll
@@ -657,8 +654,17 @@ struct Pass {
 #pragma unroll
                     for (int t = 0; t < TG; ++t)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) S[t0 + t][n] = mfma(yf[t][i], zs[n][j], S[t0 + t][n]);
+                        for (int n = 0; n < NT; ++n) add[t][n] = mfma(yf[t][i], zs[n][j], add[t][n]);
                 });
+#pragma unroll
+                for (int t = 0; t < TG; ++t)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = S[t0 + t][n][i];
+                            S[t0 + t][n][i] = s == 0 ? __builtin_fmaf(x, tot, __builtin_fmaf(x, rest, add[t][n][i])) : x + add[t][n][i];
+                        }
             }
         }
     }

@@ -205,3 +205,27 @@ def test_one_decay_for_every_token_does_not_add_up_its_rounding(dtype, chunk, H,
         want = start.detach().double().cpu() * whole
         off = (got.detach().cpu().double() - want).norm() / want.norm()
         assert float(off) <= chunks ** 0.5 * 2.0 ** -24, float(off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("width,T", [(16, 8192), (64, 4096), (128, 4096)])
+def test_a_state_is_rounded_once_for_32_tokens(dtype, width, T):
+    """No decay, terms of either sign: the state grows with the root of the tokens, |S_n|^2 = |S_N|^2 n / N after n of N times 32
+    tokens.  A rounding to nearest is off by 2^-24 / sqrt(3) of the number in the mean square; one for each 32 tokens adds up to
+    sqrt(N / 2) of that, and what the tokens add, |S_N|^2 over all, is a chain of at most 8 roundings itself:
+    2^-24 / sqrt(3) sqrt(N / 2 + 8) of the norm over at least 2^16 elements.  (A rounding for each product would be 2 to 6 for 32.)"""
+    H = 256
+    gen = torch.Generator(device=DEV).manual_seed(width)
+    a, b = (torch.randn(T, 1, H, width, generator=gen, device=DEV).to(DTYPES[dtype]) for _ in range(2))
+    zero = torch.zeros(1, 1, 1, width, dtype=DTYPES[dtype], device=DEV).expand(T, 1, H, width)
+    want = torch.bmm(a[:, 0].permute(1, 2, 0).double().contiguous(), b[:, 0].transpose(0, 1).double().contiguous())
+    g = torch.zeros(H, device=DEV)
+    with torch.no_grad():
+        _, s = ops.linear_attention(zero, a, b, g, scale=1.0)
+    state = torch.zeros(1, H, width, width, device=DEV, requires_grad=True)
+    o, _ = ops.linear_attention(a, zero, zero, g, state, scale=1.0)
+    ds, = torch.autograd.grad(o, state, b)
+    for x in (s, ds):
+        off = float((x[0].double() - want).norm() / want.norm())
+        assert off <= 2.0 ** -24 * ((T / 64 + 8) / 3) ** 0.5, off
