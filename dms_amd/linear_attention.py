@@ -63,7 +63,7 @@ class LinearAttention(nn.Module):
     def _product(self, x, w):
         if torch.is_grad_enabled() or not x.shape[0]:
             return x.mm(w)
-        return ops.tuned_matmul(x, w)                    # inference: BLAS library chosen per shape
+        return ops.tuned_matmul(x, w, any_rows=True)     # inference: BLAS library chosen per shape, prompts' lengths in powers of two
 
     def _heads(self, x, positions):
         """q, k, v (T, B, heads, width) and the log decays (T, B, heads) of x (T, B, n_in)."""

@@ -138,20 +138,23 @@ def _time_matmul(name, a, b, reps=3):
     return e0.elapsed_time(e1)
 
 
-def tuned_matmul(a, b, acc=None, out=None):
+def tuned_matmul(a, b, acc=None, out=None, any_rows=False):
     """torch.matmul(a, b) (+ acc, accumulated in place, when given: a (M, K), b (B, K, N),
     acc (B, M, N); or written into `out` (B, M, N), which like acc may be a row-slice view of a
     larger (B, rows, N) buffer: unit stride along N) with the BLAS library (rocBLAS / hipBLASLt) chosen PER SHAPE: neither
     wins everywhere on MI355X (profiles/r1_conv1x1_backend_probe.txt: hipBLASLt is 10-25 % faster
     on DPN92's conv2_x / conv4_x 1x1 shapes, rocBLAS on the others and on the mSRU projections).
-    The choice is timed once per shape on first use (a few launches and one event wait; not
+    The choice is timed once per shape and type on first use (a few launches and one event wait; not
     during stream capture, where rocBLAS is used) and cached for the process, so results are
     reproducible within a process and may differ in the last bits between processes.
+    any_rows: for callers whose a has another number of rows at every call (prompt lengths): one choice for all between two powers
+    of two, so that a new length does not stop for a timing.
     DMN_GEMM_TUNE=0 disables the timing (always rocBLAS).  Inference only (operands detached:
     torch.matmul folds -- and copies -- a broadcast operand that requires grad)."""
     _no_tangents("tuned_matmul", a, b)                   # detached, they would be lost
     a, b = a.detach(), b.detach()
-    key = (tuple(a.shape), tuple(b.shape), a.device.index)
+    shape = ((a.shape[0] - 1).bit_length(),) + tuple(a.shape[1:]) if any_rows else tuple(a.shape)
+    key = (shape, any_rows, tuple(b.shape), a.dtype, a.device.index)
     prev = torch.backends.cuda.preferred_blas_library()
     try:
         choice = _BMM_CHOICE.get(key)
