@@ -25,7 +25,9 @@ class LinearAttention(nn.Module):
     * ``num_heads``: heads of the state; ``num_qk_heads`` (a divisor, default all): query and key heads, each shared by
       ``num_heads // num_qk_heads`` value heads.  hidden is num_heads heads of at most 128 columns.
     * ``sections``: pairs of every head that each position axis turns, () for a layer without positions.
-    * float32, bfloat16 or float16 parameters and inputs; the gate's bias, the decays and the state are float32.
+    * float32, bfloat16 or float16 parameters and inputs; the gate's bias (``layer.bfloat16()`` and the like leave it alone), the
+      decays and the state are float32.  The gate's product is rounded to the layer's type like every projection, then joined
+      with its bias in float32.
     * parameters: ``weight (n_in, (2*num_qk_heads + num_heads) * width)`` = [q | k | v], ``gate (n_in, num_heads)``,
       ``gate_bias (num_heads)``, ``q_norm``, ``k_norm (width)``, ``out (hidden, hidden)``.
     """
@@ -45,7 +47,7 @@ class LinearAttention(nn.Module):
         self.sections, self.base, self.eps = tuple(sections), float(base), float(eps)
         self.weight = nn.Parameter(torch.empty(input_size, (2 * num_qk_heads + num_heads) * self.width))
         self.gate = nn.Parameter(torch.empty(input_size, num_heads))
-        self.gate_bias = nn.Parameter(torch.empty(num_heads))
+        self.gate_bias = nn.Parameter(torch.empty(num_heads, dtype=torch.float32))
         self.q_norm = nn.Parameter(torch.empty(self.width))
         self.k_norm = nn.Parameter(torch.empty(self.width))
         self.out = nn.Parameter(torch.empty(hidden_size, hidden_size))
@@ -59,6 +61,19 @@ class LinearAttention(nn.Module):
             self.gate_bias.zero_()
             self.q_norm.fill_(1.0)
             self.k_norm.fill_(1.0)
+
+    def _apply(self, fn, recurse=True):
+        """Device moves and conversions; a conversion to 16 bits leaves the gate's bias in float32, where small updates of a
+        decay that is close to 1 are not lost."""
+        bias, grad = self.gate_bias.data, self.gate_bias.grad
+        grad = None if grad is None else grad.data         # what a conversion in place does not reach
+        super()._apply(fn, recurse)
+        if self.gate_bias.dtype in (torch.bfloat16, torch.float16) and bias.dtype == torch.float32:
+            self.gate_bias.grad = None
+            self.gate_bias.data = bias.to(self.gate_bias.device)
+            if grad is not None:
+                self.gate_bias.grad = grad.to(self.gate_bias.device)
+        return self
 
     def _product(self, x, w):
         if torch.is_grad_enabled() or not x.shape[0]:
