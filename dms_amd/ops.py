@@ -803,6 +803,7 @@ def dpn_merge(base, y, c1c, bn=None):
 # ------------------------------------------------------------------------------------
 _DTYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 LINEAR_ATTENTION_MAX_WIDTH = 128
+_MAX_TOKEN_STRIDE = (1 << 24) + (1 << 20)            # what the entry points take, in elements
 
 
 def _on(device):
@@ -908,7 +909,7 @@ class _LinearAttention(torch.autograd.Function):
         with _on(dev):
             if grad_o is None:
                 grad_o = torch.zeros(dv, device=dev, dtype=q.dtype).expand(T, B, H, dv)
-            elif dv > 1 and grad_o.stride(3) != 1:
+            elif (dv > 1 and grad_o.stride(3) != 1) or (T > 1 and grad_o.stride(0) > _MAX_TOKEN_STRIDE):      # not the caller's choice
                 grad_o = grad_o.contiguous()
             if grad_state is not None:
                 grad_state = grad_state.contiguous()

@@ -52,3 +52,19 @@ def test_columns_behind_a_row_stay_out_of_sequences_of_more_than_2_20_tokens(dty
         for name, x, y in zip(("o",) + NAMES, got, (want.detach(),) + grads):
             x, y = x[lo:hi, 0, 0].detach().cpu().double()[first:first + n], y[first:first + n]
             assert float((x - y).norm()) <= bound * float(y.norm()), (name, lo, float((x - y).norm() / y.norm()))
+
+
+@pytest.mark.gpu
+def test_gradient_of_the_output_in_rows_too_far_apart():
+    """What flows back is whatever the next operator made, here a slice of a far wider tensor: the result is that of its copy."""
+    T, H, d = 3, 2, 16
+    gen = torch.Generator().manual_seed(4)
+    leaves = [torch.randn(T, 1, H, d, generator=gen).bfloat16().to(DEV).requires_grad_() for _ in range(3)]
+    g = torch.full((T, 1, H), -0.1, device=DEV, requires_grad=True)
+    o, _ = ops.linear_attention(*leaves, g)
+    do = torch.randn(T, 1, H, d, generator=gen).bfloat16().to(DEV)
+    room = torch.full((T, (1 << 24) + (1 << 20) + 8), float("nan"), dtype=torch.bfloat16, device=DEV)
+    room[:, :H * d] = do.view(T, H * d)
+    want = torch.autograd.grad(o, leaves + [g], do, retain_graph=True)
+    got = torch.autograd.grad(o, leaves + [g], torch.as_strided(room, do.shape, (room.shape[1], H * d, d, 1)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
