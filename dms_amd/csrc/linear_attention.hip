@@ -359,13 +359,13 @@ static void fill_common(Args &a, const float *g, const long long *gs, const void
     a.decays = nullptr;
 }
 
-// the backward's passes: where each one's piece of the workspace begins
+// the backward's passes: where each one's piece of the workspace begins; decays: their gradient is wanted
 struct BwdPlan {
     int DK, DV;
     long long passes, keep[2], flow, dots, dq, dk, dv, ds0, end, part, total;
 };
 
-static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)
+static BwdPlan plan_bwd(int dtype, bool decays, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)
 {
     BwdPlan p;
     pad_pair(dk, dv, &p.DK, &p.DV);
@@ -379,15 +379,16 @@ static BwdPlan plan_bwd(int dtype, int T, int B, int H, int Hq, int Hk, int Hv, 
     }
     const auto take = [&at](long long n) { const long long o = at; at += up4(n); return o; };
     p.passes = take(most);                                 // of two launches the second begins when the first is done with it
-    for (long long &keep : p.keep) keep = take(BH * anchors(T) * p.DK * p.DV);
-    p.flow = take(2 * BH * anchors(T));                    // doubles
-    p.dots = take(2 * rows);
+    const long long for_decays = decays ? BH : 0;
+    for (long long &keep : p.keep) keep = take(for_decays * anchors(T) * p.DK * p.DV);
+    p.flow = take(2 * for_decays * anchors(T));            // doubles
+    p.dots = take(2 * for_decays * T);
     p.dq = take(Hq < H ? rows * dk : 0);
     p.dk = take(Hk < H ? rows * dk : 0);
     p.dv = take(Hv < H ? rows * dv : 0);
-    p.ds0 = take(BH * dk * dv);
-    p.end = take(anchors(T) > 0 ? BH * dk * dv : 0);
-    p.part = take(2 * BH * stretches(T));                  // doubles: what they add up to may be far smaller than each
+    p.ds0 = take(for_decays * dk * dv);
+    p.end = take(anchors(T) > 0 ? for_decays * dk * dv : 0);
+    p.part = take(2 * for_decays * stretches(T));          // doubles: what they add up to may be far smaller than each
     p.total = at;
     return p;
 }
@@ -441,7 +442,7 @@ using namespace dmn::la;
 extern "C" long long dmn_linear_attention_workspace_floats(int dtype, int backward, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv)
 {
     if (check("dmn_linear_attention_workspace_floats", dtype, T, B, H, Hq, Hk, Hv, dk, dv)) return -1;
-    if (backward) return plan_bwd(dtype, T, B, H, Hq, Hk, Hv, dk, dv).total;
+    if (backward) return plan_bwd(dtype, backward != 2, T, B, H, Hq, Hk, Hv, dk, dv).total;
     int DC, DZ, nseg, seg_chunks;
     pad_pair(dk, dv, &DC, &DZ);
     plan_segments(dtype, T, (long long)B * H, &nseg, &seg_chunks);
@@ -502,7 +503,7 @@ extern "C" int dmn_linear_attention_bwd(int dtype, const void *q, const void *k,
         return 0;
     }
     if (!workspace || (size_t)workspace % 16) return fail(-7, "%s: needs a 16-byte aligned workspace", who);
-    const BwdPlan p = plan_bwd(dtype, T, B, H, Hq, Hk, Hv, dk, dv);
+    const BwdPlan p = plan_bwd(dtype, grad_g != nullptr, T, B, H, Hq, Hk, Hv, dk, dv);
     float *dots = workspace + p.dots, *ds0 = grad_state0;
     const bool need_ds0 = grad_state0 || (grad_g && state0);
     if (!ds0) ds0 = workspace + p.ds0;

@@ -918,7 +918,7 @@ class _LinearAttention(torch.autograd.Function):
             gv = torch.empty((T, B, Hv, dv), device=dev, dtype=q.dtype) if need[2] else None
             gg = torch.empty(g.shape, device=dev, dtype=torch.float32) if need[3] else None
             gs = torch.empty((B, H, dk, dv), device=dev, dtype=torch.float32) if state0 is not None and need[4] else None
-            ws = torch.empty(max(_workspace("dmn_linear_attention_workspace_floats", dt, 1, *sizes), 4), device=dev,
+            ws = torch.empty(max(_workspace("dmn_linear_attention_workspace_floats", dt, 1 if need[3] else 2, *sizes), 4), device=dev,
                              dtype=torch.float32)
             _lib.call("dmn_linear_attention_bwd", dt, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(state0), _ptr(lengths),
                       int(lengths is not None and lengths.dtype == torch.int64), _ptr(grad_o), _ptr(grad_state), _ptr(gq),

@@ -431,7 +431,8 @@ int dmn_linear_attention_fwd(int dtype, const void *q, const void *k, const void
  *   grad_g   (T,B,H) contiguous, or (H) with grad_g_per_head = 1 (summed over t and b, always in the same order), or NULL.  Zero
  *            where exp(g) is zero in 32 bits.  It is the difference of what queries and keys give back, so that its error goes by
  *            the sizes of q . grad_q and k . grad_k, summed over at most 256 tokens: at every 256th it is known from two states.
- *   workspace  dmn_linear_attention_workspace_floats(dtype, 1, ...) floats, 16-byte aligned.
+ *   workspace  dmn_linear_attention_workspace_floats(dtype, 1, ...) floats, 16-byte aligned, never NULL; (dtype, 2, ...) are enough
+ *            where grad_g is NULL.
  * No atomics: the same inputs give the same bits.
  */
 int dmn_linear_attention_bwd(int dtype, const void *q, const void *k, const void *v, const float *g, const float *state0,
