@@ -68,3 +68,48 @@ def test_gradient_of_the_output_in_rows_too_far_apart():
     want = torch.autograd.grad(o, leaves + [g], do, retain_graph=True)
     got = torch.autograd.grad(o, leaves + [g], torch.as_strided(room, do.shape, (room.shape[1], H * d, d, 1)))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_gradients_at_offsets_beyond_32_bits():
+    """Rows 2^24 + 8 elements apart in the forward and backward pass: the last ones start behind 2^32 elements."""
+    T, H, d, gap = 260, 2, 64, (1 << 24) + 8
+    gen = torch.Generator().manual_seed(2)
+    small = [torch.randn(T, 1, H, d, generator=gen).bfloat16().to(DEV) for _ in range(4)]
+    g = torch.nn.functional.logsigmoid(torch.randn(T, 1, H, generator=gen)).to(DEV)
+    room = torch.empty((T - 1) * gap + 4 * H * d, dtype=torch.bfloat16, device=DEV)
+    far = [torch.as_strided(room, (T, 1, H, d), (gap, H * d, d, 1), i * H * d) for i in range(4)]
+    for x, y in zip(far, small):
+        x.copy_(y)
+
+    def run(q, k, v, do):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, g)]
+        out = ops.linear_attention(*leaves)
+        return list(out) + list(torch.autograd.grad(out[0], leaves, do))
+
+    for a, b in zip(run(*far), run(*small)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_decays_gradient_at_meeting_states_beyond_32_bits():
+    """2^27 + 1024 tokens of one wide head: the states that meet at every 256th token take more than 2^31 groups of four.  All
+    tokens are alike, so that far from either end S = k^T v / (1 - a), dS = scale q^T do / (1 - a) and the gradient is
+    a <S, dS>, for every token the same.  Bound: sums of 24-bit products over the at most 60 tokens that exp(-t/2) leaves, the two
+    states' and 256 dots' of the size of (1 - a)^2 / a = 0.26 of the gradient: 2^-15 of it."""
+    T, d = (1 << 27) + 1024, 65
+    if torch.cuda.mem_get_info()[0] + torch.cuda.memory_reserved() < 120 << 30:
+        pytest.skip("needs 120 GiB of free GPU memory")
+    torch.cuda.empty_cache()
+    gen = torch.Generator().manual_seed(3)
+    one = [torch.rand(1, 1, 1, d, generator=gen).bfloat16().to(DEV) for _ in range(4)]
+    q, k, v, do = (x.expand(T, 1, 1, d) for x in one)
+    g = torch.full((T, 1, 1), -0.5, device=DEV, requires_grad=True)
+    o, _ = ops.linear_attention(q, k, v, g)
+    got, = torch.autograd.grad(o, g, do)
+    a, (q, k, v, do) = torch.tensor(-0.5, dtype=torch.float64).exp(), (x.double().cpu().flatten() for x in one)
+    want = float(a * d ** -0.5 * (q @ k) * (v @ do) / (1 - a) ** 2)
+    off = (got[512:T - 512] - want).abs_().max()
+    assert float(off) <= 2.0 ** -15 * want, float(off) / want
+    del o, got
+    torch.cuda.empty_cache()

@@ -229,3 +229,50 @@ def test_a_state_is_rounded_once_for_32_tokens(dtype, width, T):
     for x in (s, ds):
         off = float((x[0].double() - want).norm() / want.norm())
         assert off <= 2.0 ** -24 * ((T / 64 + 8) / 3) ** 0.5, off
+
+
+# ------------------------------------------------------------------------------------ by the norm
+def norm_case(seed, T, dk, dv):
+    gen = torch.Generator().manual_seed(seed)
+    rnd = lambda *shape: torch.randn(shape, generator=gen)  # noqa: E731
+    B = 2
+    args = [rnd(T, B, dk), rnd(T, B, dk), rnd(T, B, dv), 0.2 * torch.nn.functional.logsigmoid(1 + rnd(T, B)), rnd(B, dk, dv)]
+    return args, rnd(T, B, dv), rnd(B, dk, dv), dk ** -0.5
+
+
+# Of the norm.  Three planes leave 2^-26 of an operand in the mean, a sum passes about 32 roundings of 2^-24 / sqrt(3) with what it
+# has gathered, sqrt(32) of them in the mean square: 2^-22.3, and three such stages (scores, state, output) below 2^-21.  The
+# decays' gradient gathers the dots of up to 256 tokens, whose errors grow with the root of the distance to a meeting state as
+# the gradient itself does with the root of what a state remembers, here about 20 tokens: sqrt(128 / 20) of that.
+NORM, NORM_DECAYS = 2.0 ** -21, 2.0 ** -19.6
+NAMES = ("o", "state", "q", "k", "v", "g", "state0")
+NORM_CASES = [(20, 64, 64), (300, 64, 64), (700, 100, 36), (290, 128, 128), (1100, 32, 24)]
+
+
+def norm_of_error(got, want):
+    return float((got.detach().cpu().double().reshape(want.shape) - want).norm() / want.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,dk,dv", NORM_CASES)
+def test_fp32_results_by_their_norm(T, dk, dv):
+    args, do, ds, scale = norm_case(T, T, dk, dv)
+    dev = [x.unsqueeze(2 if i < 4 else 1).to(DEV).requires_grad_() for i, x in enumerate(args)]
+    out = ops.linear_attention(*dev)
+    got = list(out) + list(torch.autograd.grad(out, dev, [do.unsqueeze(2).to(DEV), ds.unsqueeze(1).to(DEV)]))
+    want = recurrence_grads([x.double() for x in args], scale, do.double(), ds.double())
+    for name, x, y in zip(NAMES, got, want):
+        assert norm_of_error(x, y) <= (NORM_DECAYS if name == "g" else NORM), (name, norm_of_error(x, y))
+
+
+@pytest.mark.parametrize("at,T", [(0, 300), (1, 300), (2, 300), (4, 20)])        # the first state fades
+def test_a_lost_plane_would_be_seen(at, T):
+    """The same bounds reject 64-bit results of inputs of which one kept two planes, 16 bits, only."""
+    args, do, ds, scale = norm_case(T, T, 64, 64)
+    args = [x.double() for x in args]
+    want = recurrence_grads(args, scale, do.double(), ds.double())
+    high = args[at].bfloat16().double()
+    spoilt = list(args)
+    spoilt[at] = high + (args[at] - high).bfloat16().double()
+    got = recurrence_grads(spoilt, scale, do.double(), ds.double())
+    assert any(norm_of_error(x, y) > (NORM_DECAYS if name == "g" else NORM) for name, x, y in zip(NAMES, got, want))
