@@ -262,7 +262,7 @@ struct alignas(16) Decays {
     float Gh[C], Gl[C];        // G_i as two floats
     float E[C], R[C];          // 2^{G_i} scale_x, 2^{G_C - G_i} scale_z
     float F[C];                // 2^{G_e - G_i}, e the last row of i's 16
-    float tot, tot_rest;       // 2^{G_C} as two floats: it meets the state at every chunk, where a lasting decay's rounding would add up
+    float tot;                 // 2^{G_C}
 };
 
 // the log decay of a lane's step: of its token, or backwards of the token after it
@@ -273,9 +273,10 @@ __device__ __forceinline__ float fetch_decay(const float *pg, long long gt, int 
     return lane < C && t < len ? pg[(long long)t * gt] : 0.0f;
 }
 
-// 2^x as two floats where it lasts, |x| < 1/2: 1 + y + (y^2/2 + y^3/6 + ..), y = x ln 2, whose last term here leaves 2^-27.  A state
-// that decays faster meets it a few times only, and one float does.
-__device__ __forceinline__ void exp2_pair(double x, float &high, float &rest)
+// 2^x as a float for the decay of a chunk.  It meets the state at every one, where the rounding of a decay that lasts, |x| < 1/2, would
+// add up: there `carry`, what the factors so far have left out, goes into the next, and their product stays right to one step.
+// 1 + y + (y^2/2 + y^3/6 + ..), y = x ln 2, in two floats: the first term left out is below 2^-27.
+__device__ __forceinline__ float chunk_decay(double x, float &carry)
 {
     const double y = x * 0.69314718055994530942;
     const float yh = (float)y, one = 1.0f + yh;
@@ -285,15 +286,15 @@ __device__ __forceinline__ void exp2_pair(double x, float &high, float &rest)
     p = __builtin_fmaf(p, yh, 1.0f / 24);
     p = __builtin_fmaf(p, yh, 1.0f / 6);
     p = __builtin_fmaf(p, yh, 0.5f);
-    const float more = (yh - (one - 1.0f)) + __builtin_fmaf(p, yh * yh, (float)(y - (double)yh)), h = one + more;
+    const float more = (yh - (one - 1.0f)) + __builtin_fmaf(one, carry, __builtin_fmaf(p, yh * yh, (float)(y - (double)yh))), a = one + more;
     const bool lasts = fabsf(yh) < 0.34657359f;
-    high = lasts ? h : fast_exp2((float)x);
-    rest = lasts ? more - (h - one) : 0.0f;
+    carry = lasts ? (more - (a - one)) * fast_rcp(a) : 0.0f;
+    return lasts ? a : fast_exp2((float)x);
 }
 
 // one wave; returns G_C
 template <int C>
-__device__ __forceinline__ double decays(float g, int lane, float scale_x, float scale_z, Decays<C> &d)
+__device__ __forceinline__ double decays(float g, int lane, float scale_x, float scale_z, float &carry, Decays<C> &d)
 {
     const double G = lane_sums(log2_decay(g));
     const double tot = lane_value(G, C - 1);
@@ -306,7 +307,8 @@ __device__ __forceinline__ double decays(float g, int lane, float scale_x, float
         d.E[lane] = fast_exp2(hi) * scale_x;
         d.R[lane] = fast_exp2((float)(tot - G)) * scale_z;
         d.F[lane] = fast_exp2((float)(end - G));
-        if (lane == 0) exp2_pair(tot, d.tot, d.tot_rest);
+        const float a = chunk_decay(tot, carry);
+        if (lane == 0) d.tot = a;
     }
     return tot;
 }
@@ -593,7 +595,7 @@ struct Pass {
     template <bool UPDATE>
     __device__ __forceinline__ void from_chunk(const __bf16 *y, const __bf16 *z, const __bf16 *P, const Decays<C> &d, int z0, int lr, int lg)
     {
-        const float tot = d.tot, rest = d.tot_rest;
+        const float tot = d.tot;
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
             b16x8 zs[NT][NC];
@@ -663,7 +665,7 @@ struct Pass {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float x = S[t0 + t][n][i];
-                            S[t0 + t][n][i] = s == 0 ? __builtin_fmaf(x, tot, __builtin_fmaf(x, rest, add[t][n][i])) : x + add[t][n][i];
+                            S[t0 + t][n][i] = s == 0 ? __builtin_fmaf(x, tot, add[t][n][i]) : x + add[t][n][i];
                         }
             }
         }
@@ -788,7 +790,7 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
     tz.init(ro.Z, w.b, w.h, tid, ro.reverse);
     typename decltype(ty)::Flight fy;
     typename decltype(tz)::Flight fz;
-    float g = 0.0f;
+    float g = 0.0f, carry = 0.0f;
     double gsum = 0.0;
     const auto fetch = [&](int ci) {
         const int t0 = token0(ci);
@@ -798,7 +800,7 @@ __global__ void __launch_bounds__((64 * owners<T, DZ>())) state_kernel(const Arg
     };
     if (w.c0 < w.c1) fetch(w.c0);
     for (int ci = w.c0; ci < w.c1; ++ci) {
-        if (wave == NW - 1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, sm.d[ci & 1]);
+        if (wave == NW - 1) gsum += decays<C>(g, lane, ro.scale_x, ro.scale_z, carry, sm.d[ci & 1]);
         __syncthreads();                              // nobody reads the last chunk's tiles any more
         ty.store(fy, sm.y, tid);
         tz.store(fz, sm.z, tid);
@@ -880,10 +882,11 @@ __global__ void __launch_bounds__((64 * (owners<T, DZ>() + feeders<T, DZ>())), (
         const auto fetch_z = [&](int ci, Chunk &f) __attribute__((always_inline)) {
             if (ci < c1) tz.fetch(f.z, token0(ci), len - token0(ci));
         };
+        float carry = 0.0f;
         const auto store_xy = [&](int ci, const Chunk &f) __attribute__((always_inline)) {
             tx.store(f.x, sm.x[ci & 1], ft);
             ty.store(f.y, sm.y[ci & 1], ft);
-            if (fw == 0) decays<C>(f.g, lane, scale_x, scale_z, sm.d[ci & 1]);
+            if (fw == 0) decays<C>(f.g, lane, scale_x, scale_z, carry, sm.d[ci & 1]);
         };
         const auto flush = [&](int ci) __attribute__((always_inline)) {
             if (o) tx.drain(sm.x[ci & 1], ft, o + token0(ci) * o_st, o_st, len - token0(ci));
