@@ -6,8 +6,8 @@
 // Backward, with u = dy turned back:  dw = sum u x r,  dx = r u w - x r^3 mean(x u w),  r = rsqrt(mean(x^2) + eps).
 //
 // Bound by memory: x is read and y written once (backward: x and dy read, dx written), in 16-byte pieces where the rows
-// allow it (bf16, 32 heads of 64 for 163840 tokens: 257 us, 5.2 TB/s, the rate of a copy; fp32, 12 heads of 100 for 128000: 261 us
-// and 395 backward, 4.7 TB/s).  A group of 2^lg lanes takes a token and walks its heads, so that cosines and sines are computed once for all of
+// allow it (bf16, 32 heads of 64 for 163840 tokens: 258 us, 5.2 TB/s, the rate of a copy; fp32, 12 heads of 100 for 128000: 251 us
+// and 381 backward, 4.9 TB/s; bf16 and fp16, 32 heads of 64 for 128000: 195 us, 5.4 TB/s, and 320 and 325 backward, 4.9 and 4.8).  A group of 2^lg lanes takes a token and walks its heads, so that cosines and sines are computed once for all of
 // them: a lane keeps those of its own E/2 pairs.  The angle is formed in turns and in 64 bits (a position of 2^20 radians
 // has lost 4 digits in 32), reduced there, and only the rest of the turn goes on in 32.
 #include "common.h"

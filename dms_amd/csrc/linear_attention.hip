@@ -9,8 +9,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // states[seg] = state after segment seg, from what each segment added: one thread for 4 elements of the state, in
-// segment order (at most a few dozen), so the same bits every time.  8 segments are loaded at a time: what this costs is the
-// loads' latency (16 heads of 64 x 64 in 40 segments: one load at a time 15 us, so 5).
+// segment order (at most NUM_CU), so the same bits every time.  8 segments are loaded at a time, as what this costs is the
+// loads' latency: 16 heads of 64 x 64 in 16 segments 4.4 us, one head of 32768 tokens in 256 segments 27 us of 45 in all.
 __global__ void __launch_bounds__(64) combine_kernel(float *states, const double *decays, int nseg, int n4, long long total)
 {
     const long long e = (long long)blockIdx.x * 64 + threadIdx.x;
@@ -73,7 +73,7 @@ __device__ __forceinline__ double block_sum(double v, double *sh)
 // misses at the next is spread over the way (2046 tokens: an error of 2.2e-6 of the norm without, 4.4e-7 with).
 //
 // flow[bh][i] = <S, dS> between the tokens before and from the anchor i + 1 on, n4 fours of either state in the same order.  Bound by
-// reading them: 42 us, 5.6 TB/s, for 1024 heads of 64 x 64 and 2000 tokens; every 512th token would halve that, and leave 1.4 times
+// reading them: 41 us, 5.7 TB/s, for 1024 heads of 64 x 64 and 2000 tokens; every 512th token would halve that, and leave 1.4 times
 // the error.
 __global__ void __launch_bounds__(256) meet_kernel(const f32x4 *before, const f32x4 *behind, double *flow, int n4)
 {
@@ -94,7 +94,7 @@ __host__ __device__ static inline int stretches(int T) { return (T + 4 * ANCHOR 
 
 // A wave for each stretch between anchors, four a workgroup, in 64 bits; the result takes the dots' place, or its sum goes to
 // `part`: g and dg have the heads together, and 4 bytes of every line would be written from here (44 us for 1024 heads of 2000
-// tokens; this takes 16, the turn below 17).
+// tokens; this takes 15, the turn below 17).
 __global__ void __launch_bounds__(256)
 decay_scan_kernel(float *dots_q, const float *dots_k, const double *flow, const float *s0, const float *ds0, const float *s_end, const float *ds_end,
                   const float *g, long long gt, long long gb, long long gh, const void *lengths, int lengths64, double *part, int T, int B, int H, int n)
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(64) decay_grad_heads_kernel(const double *part
 }
 
 // One token: S = a S + k^T v in place, o = scale q S.  Bound by reading and writing the state once (256 streams of 16 heads of
-// 128 x 128: 537 MB in 101 us, 5.3 TB/s; 8 heads of 125 x 125: 5 us, a launch).  A workgroup takes
+// 128 x 128: 537 MB in 99 us, 5.4 TB/s; 8 heads of 125 x 125: 5 us, a launch).  A workgroup takes
 // a head, or a slice of its columns where there are few heads (a row of S then still comes in whole 64-byte pieces);
 // V columns a thread (4 where every row is 16-byte aligned), rows over the threads, their partial o joined in LDS in
 // row order.
@@ -253,8 +253,12 @@ static void pad_pair(int dc, int dz, int *DC, int *DZ)
 }
 
 // Segments: a sequence is cut where the (sample, head) pairs alone leave compute units without a workgroup, into as many as give
-// each one, at the cost of reading y and z once more for the states between segments.  16 heads of 5120 tokens: 33 us with
-// 16 segments, 35 with 32, 38 with 48; 32 heads of 1999 tokens with their backward: 272 us with 8, 281 with 16, 316 with 24.
+// each one, at the cost of reading y and z once more for the states between segments.  16 heads of 5120 tokens: 33.7 us with
+// 16 segments, 34.0 with 32, 37.8 with 48; 32 heads of 1999 tokens with their backward: 256 us with 8, 262 with 16, 287 with 24.
+// From 129 pairs on that is two segments, which pays where two workgroups fit a compute unit (64 x 64: 130 ragged fp32 sequences of
+// up to 2000 tokens 138 us, uncut 153; 250 of 2000: 191 and 196) and where few ragged ones leave units idle (128 x 128, 130 ragged, fp32: 227 us,
+// uncut 278), but not for 128 x 128 with more or full sequences, whose workgroups then take two turns (130 of 2000: 370 us, uncut 304;
+// 250 ragged: 373 and 302).
 static void plan_segments(int dtype, int T, long long passes, int *nseg, int *seg_chunks)
 {
     const int C = chunk_tokens(dtype), nchunks = (T + C - 1) / C;

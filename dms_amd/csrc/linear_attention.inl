@@ -22,11 +22,13 @@
 //
 // The gradients are the same kernel in other roles: dq on (dO, v, k) forward, dk on (v, dO, q) and dv on (k, q, dO) backward.
 //
-// Measured (copies here reach 5.1 TB/s): bf16, 512 heads of 64 x 64, 5120 tokens: 315 us, 1.36 GB of inputs and outputs, 4.3 TB/s
-// (566 us with one kind of wave that does all); bf16, 1024 heads, 2000 tokens, all gradients: 1110 us for three roles that
-// read 11 and write 3 tensors of 262 MB, 3.3 TB/s; fp32, 160 heads of 100 x 100, ragged, up to 2000 tokens: 254 us, of them 76 for
-// the states between segments.  Neither memory nor the matrix units (a fifth of the cycles) nor LDS (two fifths) are full: waves
-// wait for three fifths of their cycles, most at the two barriers a chunk, where owners and feeders meet.
+// Measured (copies here reach 5.1 TB/s): bf16, 512 heads of 64 x 64, 5120 tokens: 360 us, 1.36 GB of inputs and outputs, 3.8 TB/s
+// (566 us with one kind of wave that does all; 314 with scores and states of 16 bits, 339 with 24, the rest for what lasting decays
+// and sums in the state keep); bf16, 1024 heads, 2000 tokens, all gradients: 990 us for three roles that together read 2.90 GB
+// through the L2 (11 tensors of 262 MB) and write 1.06 (3 tensors, the states that meet), 4.0 TB/s; fp32, 160 heads of 100 x 100,
+// ragged, up to 2000 tokens: 246 us, of them 73 for the states between segments.  Neither memory nor the matrix units (26 % of the
+// cycles in the first case, 20 in the second) nor LDS (45 and 37 %) are full: waves wait for 57 and 62 % of their cycles, most
+// at the two barriers a chunk, where owners and feeders meet.
 #pragma once
 #include "linear_attention.h"
 
@@ -745,7 +747,9 @@ template <int C>
 struct Place {
     int bh, seg, ri, b, h, len, live, c0, c1;
 
-    // The roles of a head sit 8 blocks apart: on the same XCD and started together, so that what they all read comes once from memory.
+    // The roles of a head sit 8 blocks apart: on the same XCD and started together, where they find a little of what the others have
+    // read (1024 heads of 64 x 64, 2000 tokens, bf16: 2.90 GB through the L2 and 1321 us in all, 3.14 and 1355 with role after role;
+    // 256 heads of 128 x 128: no difference).
     __device__ __forceinline__ Place(const Args &a)
     {
         const int BH = a.B * a.H, per = BH * a.nroles, in = blockIdx.x % per;

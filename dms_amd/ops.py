@@ -936,7 +936,8 @@ def linear_attention(q, k, v, g, state0=None, lengths=None, scale=None):
     sequences can be packed one behind the other).  H, the heads of the state, is a multiple of Hq, Hk and Hv: head h
     reads head h // (H // Hq) of q, and so on.  Head widths up to 128, B * H up to 2^17, tokens up to 2^24 elements apart.  state0 (B, H, dk, dv) float32 or None (zeros);
     lengths (B,) int32 or int64 on the device, or None: tokens of each sample, rows behind them are neither read nor do
-    they change the state, and their outputs and gradients are zero.  scale: dk ** -0.5 if None.
+    they change the state, and their outputs and gradients are zero.  scale: dk ** -0.5 if None.  A token that is not finite spoils
+    the outputs of its chunk too (64 tokens in bfloat16, 32 else) and the decays' gradient of its 256 tokens.
     Returns o (T, B, H, dv) and the state (B, H, dk, dv) after the last token, both under autograd (once; backward mode only)."""
     name = "linear_attention"
     if not torch.is_tensor(g) or g.dim() not in (1, 3):

@@ -417,7 +417,8 @@ int dmn_dpn_stage_pass(float *buf, float *act, float *out,
  *   workspace  dmn_linear_attention_workspace_floats(dtype, 0, ...) floats, 16-byte aligned (NULL when that is 0).  Calls that
  *            overlap need one each.
  * Sums and states are fp32; products run on bf16 planes that together carry 24 bits of every fp32 input, score and state whatever
- * the dtype, so an infinity in a token that counts makes NaN.  A token that is not finite spoils its chunk's outputs.
+ * the dtype, so an infinity in a token that counts makes NaN.  A token that is not finite spoils its chunk's outputs (64
+ * tokens in bf16, 32 else; before it as well), and in the gradients the decays' of the 256 tokens between two meeting states.
  */
 long long dmn_linear_attention_workspace_floats(int dtype, int backward, int T, int B, int H, int Hq, int Hk, int Hv, int dk, int dv);
 int dmn_linear_attention_fwd(int dtype, const void *q, const void *k, const void *v, const float *g, const float *state0,
