@@ -276,3 +276,36 @@ def test_a_lost_plane_would_be_seen(at, T):
     spoilt[at] = high + (args[at] - high).bfloat16().double()
     got = recurrence_grads(spoilt, scale, do.double(), ds.double())
     assert any(norm_of_error(x, y) > (NORM_DECAYS if name == "g" else NORM) for name, x, y in zip(NAMES, got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("T", [65, 200, 256])
+def test_decays_gradient_is_tied_behind_the_last_token(dtype, T):
+    """Tokens of the first half 2^6 times the others in q, k, v and their output's gradient, their dots 2^24 times; a reset behind
+    them.  What the sum has missed up to there, E, stays with it; known behind the last token as well, E is spread over the T tokens:
+    E (1 - t / T) is left at t, E / T at the last, twice that for its rounding, where a sum that only starts right leaves E."""
+    B, dk, dv, half = 16, 32, 32, T // 2
+    gen = torch.Generator().manual_seed(T)
+    make = lambda *shape: torch.randn(shape, generator=gen)  # noqa: E731
+    q, k, v, do, ds, state = make(T, B, dk), make(T, B, dk), make(T, B, dv), make(T, B, dv), make(B, dk, dv), make(B, dk, dv)
+    for x in (q, k, v, do):
+        x[:half] *= 64
+    q, k, v, do = (x.to(DTYPES[dtype]) for x in (q, k, v, do))
+    g = 0.1 * torch.nn.functional.logsigmoid(make(T, B))
+    g[half] = -1e4
+    dev = [x.unsqueeze(2).to(DEV) for x in (q, k, v, g)] + [state.unsqueeze(1).to(DEV)]
+    dev[3].requires_grad_()
+    got, = torch.autograd.grad(ops.linear_attention(*dev), [dev[3]], [do.unsqueeze(2).to(DEV), ds.unsqueeze(1).to(DEV)])
+    args = [x.double() for x in (q, k, v, g, state)]
+    want = recurrence_grads(args, dk ** -0.5, do.double(), ds.double())[5]
+    off = (got[:, :, 0].cpu().double() - want).abs()
+    first, last = off[half + 1], off[-1]
+    missed = first / (1 - (half + 1) / T)
+    # the small tokens' own errors: 2^-15 of their magnitudes, as for every such sum
+    size = [x if i == 3 else x.abs() for i, x in enumerate(args)]
+    mag = recurrence_grads(size, dk ** -0.5, do.double().abs(), ds.double().abs())
+    flow = (size[0] * mag[2] + size[1] * mag[3]).sum(-1)[half + 1:].sum(0)
+    own = 2.0 ** -15 * ((mag[1] * ds.double().abs()).sum((-1, -2)) + 2 * flow)
+    assert (last <= 2 * missed / T + own).all(), (last / missed).max()
+    assert float(missed.median()) > 8 * float(own.median())    # else nothing was told apart
